@@ -225,6 +225,108 @@ uint32_t qb_rope_static(const float *x, size_t x_len, float *y, size_t y_len, si
                         void *stream);
 
 /* ------------------------------------------------------------------ */
+/* Paged cache operators                                               */
+/* ------------------------------------------------------------------ */
+/* No counterpart in the reference, whose cache belongs to one session
+ * (src/kv_cache.rs:479-590): the cache write and the attention of a
+ * session's step as operators of their own, over caller-owned pages and any
+ * mix of sequences.
+ *
+ * A cache is one layer's K and V page pools, [pages][kv_heads][16][head_dim]
+ * each (a session's page layout).  A sequence is a row of a page table:
+ * position p is row p % 16 of page tables[s][p / 16].  INT8 rows (one
+ * token's one head) carry one FP32 scale each, [pages][kv_heads][16].
+ *
+ * A step gives each sequence `count` new tokens at positions start ..
+ * start + count - 1; the tokens of all sequences are packed in sequence
+ * order, and K, V, Q and Y hold one row per packed token.  A plan is a step
+ * laid out for the device: qb_paged_plan_build checks it and fills `words`
+ * on the host, the caller copies the words to the device, and every call of
+ * the step (each layer's write and attention) takes the plan and that copy.
+ * Plans are never written by a call, so calls may share one on any streams.
+ *
+ * The calls below launch on `stream` and do not synchronize, allocate or
+ * read values back, so they can be captured; a value that is not finite
+ * flows through (see each call) instead of being an error.  Pools, scales,
+ * words and workspace are 16-byte aligned (QB_INVALID_PARAMETERS). */
+#define QB_PAGE_TOKENS 16
+enum { QB_PAGED_F32 = 0, QB_PAGED_BF16 = 1, QB_PAGED_INT8 = 2 };
+
+typedef struct {
+    void *k, *v;                 /* DEVICE page pools */
+    float *k_scales, *v_scales;  /* DEVICE, QB_PAGED_INT8 only (else NULL) */
+    size_t pages, kv_heads, head_dim;
+    uint32_t dtype;              /* QB_PAGED_* */
+} qb_paged_cache;
+
+typedef struct {
+    const int32_t *tables;           /* HOST [sequences][pages_per_sequence] */
+    const uint32_t *starts, *counts; /* HOST [sequences] */
+    size_t sequences, pages_per_sequence;
+    size_t pages, kv_heads, head_dim, query_heads;
+    /* A token at position p sees the positions j <= p, with window > 0 only
+     * those with j > p - window or j < sinks (window = 0: no window, sinks
+     * without effect). */
+    size_t window, sinks;
+    uint32_t value_dtype;            /* Q, K, V, Y: QB_PAGED_F32 or _BF16 */
+    uint32_t cache_dtype;            /* QB_PAGED_* */
+} qb_paged_step;
+
+typedef struct {
+    size_t sequences, pages_per_sequence, tokens, pages, query_heads, kv_heads, head_dim, window, sinks;
+    size_t words;                /* 32-bit words of the plan */
+    size_t workspace_bytes;      /* DEVICE workspace of one attention call */
+    uint32_t value_dtype, cache_dtype;
+    uint32_t shared_rows;        /* nonzero: two new tokens may fall on one page, so the plan cannot write */
+    uint32_t small_kind, small_unit, tile_unit, small_items, tile_items, merges;
+    uint32_t off_seqs, off_slots, off_small, off_tile, off_merges;
+} qb_paged_plan;
+
+/* Lays `step` out in words[0, capacity) (HOST) and fills *out.  HOST only.
+ * Table entries are checked where the step's calls follow them: the pages
+ * that hold new tokens and the pages that a new token sees (entries of
+ * pages before the window may be stale).
+ *  - QB_ZERO_DIMENSION (no sequence, head, page or new token; a sequence
+ *    without new tokens is allowed), QB_UNSUPPORTED (a dtype),
+ *    QB_INVALID_SHAPE (query_heads not a multiple of kv_heads, head_dim
+ *    above 256), QB_DIMENSION_OVERFLOW;
+ *  - QB_FULL: start + count passes the table row (index = the sequence);
+ *  - QB_INVALID_PARAMETERS: a page id that is not below `pages`
+ *    (index = its place in `tables`, actual = the id);
+ *  - QB_INVALID_LENGTH: capacity too small (buffer 2, expected = words);
+ *  - QB_RESOURCE_BUDGET: a workspace above 2^31 floats. */
+uint32_t qb_paged_plan_build(const qb_paged_step *step, int32_t *words, size_t capacity,
+                             qb_paged_plan *out);
+/* Stores the packed rows K, V [tokens][kv_heads][head_dim] (DEVICE, of the
+ * plan's value_dtype, *_stride elements between tokens, *_len elements from
+ * the first to the last) at their positions; every other cache row is left
+ * as it was.  FP32 rows are stored as they are, BF16 rounds to nearest
+ * even, INT8 is qb_quantize_int8's encode with one group per row: scale =
+ * max|x| / 127 (1 where that is 0), q = clamp(round(x / scale)); a row with a
+ * value that is not finite stores scale NaN and zeros, so it reads back NaN.
+ * QB_INVALID_SHAPE: the cache is not of the plan's kind;
+ * QB_INVALID_STATE: the plan's shared_rows. */
+uint32_t qb_kv_write(const void *k, size_t k_len, size_t k_stride, const void *v, size_t v_len,
+                     size_t v_stride, const qb_paged_cache *cache, const qb_paged_plan *plan,
+                     const int32_t *words, void *stream);
+/* Reads the same rows back: f32(q) * scale, rounded once to value_dtype. */
+uint32_t qb_kv_read(const qb_paged_cache *cache, const qb_paged_plan *plan, const int32_t *words,
+                    void *k, size_t k_len, size_t k_stride, void *v, size_t v_len, size_t v_stride,
+                    void *stream);
+/* Causal grouped-query attention of the step's tokens over their sequences
+ * (their own rows included, so write them first): Y [tokens][query_heads]
+ * [head_dim] (contiguous) = softmax(scale * q.k over the visible positions)
+ * V for Q rows q_stride elements apart; query head h reads KV head
+ * h / (query_heads / kv_heads).  FP32 sums and softmax.  A position that a
+ * row does not see has no influence on it, whatever the cache holds there.
+ * `workspace`: at least the plan's workspace_bytes, its content on entry
+ * irrelevant; calls that can overlap in time need one each.
+ * QB_INVALID_PARAMETERS: scale not finite and positive. */
+uint32_t qb_paged_attention(const void *q, size_t q_len, size_t q_stride, const qb_paged_cache *cache,
+                            const qb_paged_plan *plan, const int32_t *words, void *y, size_t y_len,
+                            float scale, void *workspace, size_t workspace_bytes, void *stream);
+
+/* ------------------------------------------------------------------ */
 /* Model: ModelConfig / Decoder (src/model.rs:12-25,191-273)           */
 /* ------------------------------------------------------------------ */
 

@@ -11,5 +11,5 @@ from .api import (  # noqa: F401
     LinearError, ModelError, OpError, QbError, QuantError, RopeError, Sampler, Sampling, SamplingError,
     StateError, Temperature, Role, TextStream, Tokenizer, TokenizerError, render_chat,
     embedding, linear, linear_int8, linear_int8_lanes4, linear_lanes4, masked_softmax,
-    residual_add, rmsnorm, rope, silu, softmax, tp_shard_of)
+    kv_read, kv_write, paged_attention, PagedCache, PagedPlan, residual_add, rmsnorm, rope, silu, softmax, tp_shard_of)
 from . import synthetic  # noqa: F401

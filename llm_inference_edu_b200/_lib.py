@@ -33,6 +33,10 @@ SIGNATURES = {
     "qb_softmax": ([P, S, P, S, P, S, S, S, P], U32),
     "qb_rope": ([P, S, P, S, S, S, S, S, F, P], U32),
     "qb_rope_static": ([P, S, P, S, S, S, S, S, F, P], U32),
+    "qb_paged_plan_build": ([P, P, S, P], U32),
+    "qb_kv_write": ([P, S, S, P, S, S, P, P, P, P], U32),
+    "qb_kv_read": ([P, P, P, P, S, S, P, S, S, P], U32),
+    "qb_paged_attention": ([P, S, S, P, P, P, P, S, F, P, S, P], U32),
     "qb_model_create": ([P, U32, U32, C.c_int, P], U32),
     "qb_model_set_tensor": ([U64, C.c_int64, U32, U32, P, S], U32),
     "qb_model_finalize": ([U64], U32),
@@ -127,6 +131,26 @@ class ModelConfigC(C.Structure):
     _fields_ = [(n, S) for n in ("vocab_size", "layers", "hidden_dim", "query_heads", "kv_heads",
                                  "head_dim", "ff_dim", "max_tokens")] + \
                [("rope_base", F), ("norm_epsilon", F)]
+
+
+class PagedCacheC(C.Structure):
+    _fields_ = [("k", P), ("v", P), ("k_scales", P), ("v_scales", P), ("pages", S), ("kv_heads", S),
+                ("head_dim", S), ("dtype", U32)]
+
+
+class PagedStepC(C.Structure):
+    _fields_ = [("tables", P), ("starts", P), ("counts", P)] + \
+               [(n, S) for n in ("sequences", "pages_per_sequence", "pages", "kv_heads", "head_dim",
+                                 "query_heads", "window", "sinks")] + \
+               [("value_dtype", U32), ("cache_dtype", U32)]
+
+
+class PagedPlanC(C.Structure):
+    _fields_ = [(n, S) for n in ("sequences", "pages_per_sequence", "tokens", "pages", "query_heads",
+                                 "kv_heads", "head_dim", "window", "sinks", "words", "workspace_bytes")] + \
+               [(n, U32) for n in ("value_dtype", "cache_dtype", "shared_rows", "small_kind", "small_unit",
+                                   "tile_unit", "small_items", "tile_items", "merges", "off_seqs", "off_slots", "off_small", "off_tile",
+                                   "off_merges")]
 
 
 class SessionInfo(C.Structure):

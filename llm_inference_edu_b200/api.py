@@ -8,6 +8,10 @@ Names, argument meaning and error behaviour follow the Rust crate
   embedding, residual_add, rmsnorm, silu, softmax, masked_softmax
                                 src/ops.rs:67-257
   rope                          src/rope.rs:38
+  PagedCache, PagedPlan, kv_write, kv_read, paged_attention
+                                no counterpart: the cache write and the
+                                attention of src/kv_cache.rs:479-590 over
+                                caller-owned pages and any mix of sequences
   Decoder                       src/model.rs:59-340
   CachedSession                 src/kv_cache.rs:156-475
   GenerationSession, Sampling   src/generation.rs:98-338, src/sampling.rs
@@ -230,6 +234,237 @@ def rope(x, y, tokens: int, heads: int, head_dim: int, start_position: int, base
          stream=None):
     _check(lib().qb_rope(_ptr(x), x.numel(), _ptr(y), y.numel(), tokens, heads, head_dim,
                          start_position, base, _stream(stream)), RopeError)
+
+
+# ---------------------------------------------------- paged cache operators --
+
+PAGE_TOKENS = 16
+PAGED_DTYPES = {"f32": 0, "bf16": 1, "int8": 2}
+
+
+def _paged_dtype(t) -> str:
+    import torch
+    try:
+        return {torch.float32: "f32", torch.bfloat16: "bf16", torch.int8: "int8"}[t.dtype]
+    except KeyError:
+        raise ValueError(f"unsupported element type {t.dtype}") from None
+
+
+class PagedCache:
+    """One layer's K and V pages: pools [pages][kv_heads][16][head_dim] of
+    "f32", "bf16" or "int8" elements, INT8 rows with one FP32 scale each
+    ([pages][kv_heads][16]).  No counterpart in the reference, whose cache
+    belongs to one session (src/kv_cache.rs:156-200).  The constructor
+    allocates zeroed pools; ``from_tensors`` takes the caller's."""
+
+    def __init__(self, pages: int, kv_heads: int, head_dim: int, dtype: str = "bf16", device=None):
+        import torch
+        dev = torch.device("cuda" if device is None else device)
+        dt = {"f32": torch.float32, "bf16": torch.bfloat16, "int8": torch.int8}[dtype]
+        shape = (pages, kv_heads, PAGE_TOKENS, head_dim)
+        k, v = (torch.zeros(shape, dtype=dt, device=dev) for _ in range(2))
+        ks = vs = None
+        if dtype == "int8":
+            ks, vs = (torch.zeros(shape[:3], dtype=torch.float32, device=dev) for _ in range(2))
+        self._take(k, v, ks, vs)
+
+    @classmethod
+    def from_tensors(cls, k, v, k_scales=None, v_scales=None) -> "PagedCache":
+        self = cls.__new__(cls)
+        self._take(k, v, k_scales, v_scales)
+        return self
+
+    def _take(self, k, v, ks, vs):
+        import torch
+        dtype = _paged_dtype(k)
+        if k.dim() != 4 or k.shape[2] != PAGE_TOKENS or v.shape != k.shape or v.dtype != k.dtype:
+            raise ValueError("pools must be two [pages][kv_heads][16][head_dim] tensors of one type")
+        if (dtype == "int8") != (ks is not None) or (ks is None) != (vs is None):
+            raise ValueError("k_scales and v_scales come with int8 pools, and only with them")
+        held = [k, v] if ks is None else [k, v, ks, vs]
+        for t in held[2:]:
+            if t.dtype != torch.float32 or t.shape != k.shape[:3]:
+                raise ValueError("scales must be FP32 [pages][kv_heads][16]")
+        ptrs = [_ptr(t) for t in held] + [None] * (4 - len(held))
+        if any(t.device != k.device for t in held):
+            raise ValueError("pools and scales must be on one device")
+        self.k, self.v, self.k_scales, self.v_scales = k, v, ks, vs
+        self.pages, self.kv_heads, _, self.head_dim = k.shape
+        self.dtype, self.device = dtype, k.device
+        self._c = _lib.PagedCacheC(*ptrs, self.pages, self.kv_heads, self.head_dim, PAGED_DTYPES[dtype])
+        self._ref = C.byref(self._c)
+
+    def logical_bytes(self) -> int:
+        return sum(t.numel() * t.element_size() for t in (self.k, self.v, self.k_scales, self.v_scales)
+                   if t is not None)
+
+
+def _paged_plan_words(tables, starts, counts, pages, kv_heads, head_dim, query_heads, window, sinks, value_dtype,
+                      cache_dtype):
+    """qb_paged_plan_build over host arrays: (words, plan struct)."""
+    tables, starts, counts = (np.asarray(x) for x in (tables, starts, counts))
+    for name, x in (("tables", tables), ("starts", starts), ("counts", counts)):
+        if x.size and x.dtype.kind not in "iu":
+            raise ValueError(f"{name} must hold integers")
+        if name != "tables" and x.size and (x.min() < 0 or x.max() >= 2**32):
+            raise ValueError(f"{name} must be in 0 .. 2**32 - 1")
+    if tables.dtype != np.int32:
+        # An id that no page can have stays one (refused where it is used).
+        tables = np.where((tables < 0) | (tables >= 2**31), -1, tables)
+    tables = np.ascontiguousarray(tables, dtype=np.int32)
+    starts = np.ascontiguousarray(starts, dtype=np.uint32)
+    counts = np.ascontiguousarray(counts, dtype=np.uint32)
+    if tables.ndim != 2 or starts.shape != tables.shape[:1] or counts.shape != starts.shape:
+        raise ValueError("tables must be [sequences][pages], starts and counts [sequences]")
+    for name, x in (("window", window), ("sinks", sinks)):
+        if x < 0:
+            raise ValueError(f"{name} must not be negative")
+    step = _lib.PagedStepC(tables.ctypes.data, starts.ctypes.data, counts.ctypes.data, tables.shape[0],
+                           tables.shape[1], pages, kv_heads, head_dim, query_heads, window, sinks,
+                           PAGED_DTYPES[value_dtype], PAGED_DTYPES[cache_dtype])
+    plan = _lib.PagedPlanC()
+    size = 4096 + 4 * tables.size + 2 * int(counts.sum(dtype=np.int64))
+    while True:
+        words = np.empty(size, dtype=np.int32)
+        status = lib().qb_paged_plan_build(C.byref(step), words.ctypes.data, size, C.byref(plan))
+        if status == 3:
+            d = _lib.Detail()
+            lib().qb_last_detail(C.byref(d))
+            if d.buffer == 2 and d.expected > size:
+                size = d.expected
+                continue
+        _check(status, CacheError)
+        return words[:plan.words], plan
+
+
+class PagedPlan:
+    """One step over a paged cache: sequence s of ``tables`` (page ids,
+    [sequences][pages]) gets ``counts[s]`` new tokens at positions
+    ``starts[s]``..., packed in sequence order in every tensor of the step.
+    With ``window`` > 0 a token sees its last ``window`` positions (itself
+    included) and the first ``sinks``.  ``dtype`` ("f32" or "bf16") is the
+    type of Q, K, V and Y.  Checked here, once, and laid out on the cache's
+    device; every layer's calls of the step take the same plan with a cache
+    of the same kind.  Calls never write it.  A captured call goes on using
+    the plan's and the cache's memory: keep both for as long as the graph."""
+
+    def __init__(self, cache: PagedCache, tables, starts, counts, query_heads: int, window: int = 0, sinks: int = 0,
+                 dtype: str = "f32"):
+        import torch
+        words, self._c = _paged_plan_words(tables, starts, counts, cache.pages, cache.kv_heads, cache.head_dim,
+                                           query_heads, window, sinks, dtype, cache.dtype)
+        self.device, self.dtype = cache.device, dtype
+        self._torch_dtype = {"f32": torch.float32, "bf16": torch.bfloat16}.get(dtype)
+        # Complete on return, so any stream may use it.
+        self.words = torch.from_numpy(words).to(cache.device)
+        self._stream = torch.cuda.current_stream(cache.device).cuda_stream
+        self._ref = C.byref(self._c)
+        self._words = C.c_void_p(self.words.data_ptr())
+        self.tokens, self.query_heads = self._c.tokens, query_heads
+
+    def workspace_bytes(self) -> int:
+        return self._c.workspace_bytes
+
+
+def _paged_rows(t, plan, heads: int, head_dim: int, name: str):
+    """(pointer, length, stride) of packed rows [tokens][heads][head_dim],
+    each row contiguous."""
+    if t.device != plan.device:
+        raise ValueError(f"{name} must be on the plan's device")
+    if t.dtype != plan._torch_dtype:
+        raise ValueError(f"{name} must be of the plan's type")
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 3 or shape[1] != heads or shape[2] != head_dim:
+        raise ValueError(f"{name} must be [tokens][{heads}][{head_dim}]")
+    if (stride[2] != 1 and head_dim > 1) or (stride[1] != head_dim and heads > 1):
+        raise ValueError(f"{name}'s rows must be contiguous")
+    # One token has no distance to the next; its stride may be anything.
+    step = stride[0] if shape[0] > 1 else heads * head_dim
+    return t.data_ptr(), (shape[0] - 1) * step + heads * head_dim if shape[0] else 0, step
+
+
+class _PagedCall:
+    """Device and stream of one call; memory that was not allocated on that
+    stream is marked as used by it."""
+
+    def __init__(self, plan, cache, stream, *tensors):
+        import torch
+        if cache.device != plan.device:
+            raise ValueError("the cache must be on the plan's device")
+        self.guard = None
+        if torch.cuda.current_device() != plan.device.index:
+            self.guard = torch.cuda.device(plan.device)
+            self.guard.__enter__()
+        if stream is None:
+            self.stream = torch.cuda.current_stream(plan.device).cuda_stream
+        else:
+            self.stream = int(stream)
+            ext = torch.cuda.ExternalStream(self.stream, device=plan.device) if self.stream else \
+                torch.cuda.default_stream(plan.device)
+            held = tensors + tuple(t for t in (cache.k, cache.v, cache.k_scales, cache.v_scales) if t is not None)
+            for t in held:
+                t.record_stream(ext)
+        if self.stream != plan._stream:
+            plan.words.record_stream(torch.cuda.ExternalStream(self.stream, device=plan.device) if self.stream else
+                                     torch.cuda.default_stream(plan.device))
+
+    def done(self):
+        if self.guard is not None:
+            self.guard.__exit__(None, None, None)
+
+
+def kv_write(k, v, cache: PagedCache, plan: PagedPlan, stream=None):
+    """Stores the step's K and V rows [tokens][kv_heads][head_dim] (slices
+    of a fused row are fine) at their positions, quantized for an INT8
+    cache; all other cache rows stay as they are."""
+    h, d = cache.kv_heads, cache.head_dim
+    kr, vr = _paged_rows(k, plan, h, d, "k"), _paged_rows(v, plan, h, d, "v")
+    call = _PagedCall(plan, cache, stream, k, v)
+    try:
+        _check(lib().qb_kv_write(*kr, *vr, cache._ref, plan._ref, plan._words, call.stream), CacheError)
+    finally:
+        call.done()
+
+
+def kv_read(cache: PagedCache, plan: PagedPlan, k, v, stream=None):
+    """Reads the step's rows back into k and v [tokens][kv_heads][head_dim];
+    a plan that starts at 0 reads whole sequences."""
+    h, d = cache.kv_heads, cache.head_dim
+    kr, vr = _paged_rows(k, plan, h, d, "k"), _paged_rows(v, plan, h, d, "v")
+    call = _PagedCall(plan, cache, stream, k, v)
+    try:
+        _check(lib().qb_kv_read(cache._ref, plan._ref, plan._words, *kr, *vr, call.stream), CacheError)
+    finally:
+        call.done()
+
+
+def paged_attention(q, cache: PagedCache, plan: PagedPlan, y, scale: Optional[float] = None, stream=None):
+    """Causal grouped-query attention of the step's tokens over their
+    sequences' pages, their own rows (``kv_write``) included: y [tokens]
+    [query_heads][head_dim] = softmax(scale q.k) v over the positions each
+    token sees; scale = 1 / sqrt(head_dim) by default."""
+    import torch
+    h, d = plan.query_heads, cache.head_dim
+    qr, yr = _paged_rows(q, plan, h, d, "q"), _paged_rows(y, plan, h, d, "y")
+    if not y.is_contiguous():
+        raise ValueError("y must be contiguous")
+    call = _PagedCall(plan, cache, stream, q, y)
+    try:
+        ws, need = None, plan._c.workspace_bytes
+        if need:
+            # From the call's own stream, so that calls never share one.
+            if stream is None:
+                ws = torch.empty(need, dtype=torch.uint8, device=plan.device)
+            else:
+                ext = torch.cuda.ExternalStream(call.stream, device=plan.device) if call.stream else \
+                    torch.cuda.default_stream(plan.device)
+                with torch.cuda.stream(ext):
+                    ws = torch.empty(need, dtype=torch.uint8, device=plan.device)
+        _check(lib().qb_paged_attention(*qr, cache._ref, plan._ref, plan._words, yr[0], yr[1],
+                                        float(d ** -0.5 if scale is None else scale),
+                                        None if ws is None else ws.data_ptr(), need, call.stream), CacheError)
+    finally:
+        call.done()
 
 
 # ---------------------------------------------------------------- model --

@@ -1,0 +1,141 @@
+// Attention over the paged cache: the entry point, the row-by-row kernel and
+// the merge of partial results.
+#include <math.h>
+
+#include "paged.cuh"
+
+namespace qb {
+namespace paged {
+namespace {
+
+constexpr int kRowsWarps = 4;
+
+// One CTA an item, its rows dealt to the warps.
+template <typename TV, typename TC>
+__global__ void __launch_bounds__(kRowsWarps * 32) attend_rows(const Args a) {
+    const Item it = *(const Item *)(a.words + a.off_items + (size_t)blockIdx.x * 12);
+    for (int r = threadIdx.x >> 5; r < it.rows; r += kRowsWarps) attend_row<TV, TC>(a, it, r, 64, threadIdx.x & 31);
+}
+
+// Joins the partial results of a row block, one warp a row: M = max m_z,
+// y = sum_z o_z 2^(m_z - M) / sum_z l_z 2^(m_z - M), in part order.
+constexpr int kMergeWarps = 8;
+
+template <typename TV>
+__global__ void __launch_bounds__(kMergeWarps * 32) merge_rows(const Args a) {
+    const Merge mg = *(const Merge *)(a.words + a.off_merges + (size_t)blockIdx.x * 8);
+    const SeqRec sq = *(const SeqRec *)(a.words + a.off_seqs + mg.seq * 4);
+    const int lane = threadIdx.x & 31, hd = a.hd;
+    for (int r = threadIdx.x >> 5; r < mg.rows; r += kMergeWarps) {
+        const float *w = a.ws + mg.slot;
+        float m = -INFINITY;
+        bool nan = false;
+        for (int z = lane; z < mg.parts; z += 32) {
+            const float mz = w[(size_t)z * mg.stride + (size_t)mg.rows * hd + r];
+            m = fmaxf(m, mz);
+            nan |= mz != mz;
+        }
+#pragma unroll
+        for (int off = 16; off; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
+        if (__any_sync(0xffffffffu, nan)) m = __uint_as_float(0x7fffffffu);
+        const float base = m == -INFINITY ? 0.0f : m;
+        float l = 0.0f, o[kMaxHeadDim / 32];
+#pragma unroll
+        for (int i = 0; i < kMaxHeadDim / 32; ++i) o[i] = 0.0f;
+        for (int z = 0; z < mg.parts; ++z) {
+            const float *p = w + (size_t)z * mg.stride;
+            const float f = exp2f(p[(size_t)mg.rows * hd + r] - base);
+            l = fmaf(f, p[(size_t)mg.rows * (hd + 1) + r], l);
+#pragma unroll
+            for (int i = 0; i < kMaxHeadDim / 32; ++i)
+                if (lane + 32 * i < hd) o[i] = fmaf(f, p[(size_t)r * hd + lane + 32 * i], o[i]);
+        }
+        const int row = mg.row0 + r;
+        const size_t tok = (size_t)sq.tok0 + row / a.G, qh = (size_t)mg.kvh * a.G + row % a.G;
+        TV *y = (TV *)a.y + (tok * a.H + qh) * hd;
+#pragma unroll
+        for (int i = 0; i < kMaxHeadDim / 32; ++i)
+            if (lane + 32 * i < hd) store_value(y, lane + 32 * i, __fdiv_rn(o[i], l));
+    }
+}
+
+template <typename TV>
+uint32_t run_rows(const Args &a, uint32_t ct, cudaStream_t st) {
+    if (ct == QB_PAGED_F32)
+        attend_rows<TV, float><<<a.items, kRowsWarps * 32, 0, st>>>(a);
+    else if (ct == QB_PAGED_BF16)
+        attend_rows<TV, uint16_t><<<a.items, kRowsWarps * 32, 0, st>>>(a);
+    else
+        attend_rows<TV, int8_t><<<a.items, kRowsWarps * 32, 0, st>>>(a);
+    QB_CUDA(cudaGetLastError());
+    return QB_OK;
+}
+
+}  // namespace
+
+uint32_t admit(const qb_paged_cache *c, const qb_paged_plan *p, const int32_t *words);
+uint32_t admit_rows(size_t buffer, size_t len, size_t stride, size_t width, size_t tokens);
+
+}  // namespace paged
+}  // namespace qb
+
+using namespace qb;
+using namespace qb::paged;
+
+extern "C" {
+
+uint32_t qb_paged_attention(const void *q, size_t q_len, size_t q_stride, const qb_paged_cache *cache,
+                            const qb_paged_plan *plan, const int32_t *words, void *y, size_t y_len, float scale,
+                            void *workspace, size_t workspace_bytes, void *stream) {
+    clear_detail();
+    uint32_t s = admit(cache, plan, words);
+    if (s) return s;
+    const size_t width = plan->query_heads * plan->head_dim;
+    if ((s = admit_rows(0, q_len, q_stride, width, plan->tokens))) return s;
+    if ((s = admit_rows(2, y_len, width, width, plan->tokens))) return s;
+    if (!q || !y || !(isfinite(scale) && scale > 0.0f)) return QB_INVALID_PARAMETERS;
+    if (workspace_bytes < plan->workspace_bytes) {
+        set_detail(3, plan->workspace_bytes, workspace_bytes);
+        return QB_INVALID_LENGTH;
+    }
+    if (plan->workspace_bytes && (!workspace || ((uintptr_t)workspace & 15))) return QB_INVALID_PARAMETERS;
+    Args a{};
+    a.words = words;
+    a.off_seqs = plan->off_seqs;
+    a.off_merges = plan->off_merges;
+    a.merges = (int)plan->merges;
+    a.H = (int)plan->query_heads;
+    a.KV = (int)plan->kv_heads;
+    a.G = a.H / a.KV;
+    a.hd = (int)plan->head_dim;
+    a.window = (int)plan->window;
+    a.sinks = (int)(plan->sinks < 0x7fffffffu ? plan->sinks : 0x7fffffffu);
+    a.c = (float)((double)scale * 1.4426950408889634);
+    a.q = q;
+    a.q_stride = q_stride;
+    a.y = y;
+    a.k = (const uint8_t *)cache->k;
+    a.v = (const uint8_t *)cache->v;
+    a.ks = cache->dtype == QB_PAGED_INT8 ? cache->k_scales : nullptr;
+    a.vs = cache->dtype == QB_PAGED_INT8 ? cache->v_scales : nullptr;
+    a.ws = (float *)workspace;
+    cudaStream_t st = (cudaStream_t)stream;
+    const bool wide = plan->value_dtype == QB_PAGED_F32;
+    if (plan->small_items) {
+        a.off_items = plan->off_small;
+        a.items = (int)plan->small_items;
+        s = wide ? run_rows<float>(a, plan->cache_dtype, st) : run_rows<uint16_t>(a, plan->cache_dtype, st);
+        if (s) return s;
+    }
+    if (plan->tile_items) return QB_UNSUPPORTED;
+    if (plan->merges) {
+        if (wide)
+            merge_rows<float><<<a.merges, kMergeWarps * 32, 0, st>>>(a);
+        else
+            merge_rows<uint16_t><<<a.merges, kMergeWarps * 32, 0, st>>>(a);
+        QB_CUDA(cudaGetLastError());
+    }
+    return QB_OK;
+}
+
+}  // extern "C"
