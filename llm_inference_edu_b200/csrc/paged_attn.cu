@@ -2,7 +2,7 @@
 // the merge of partial results.
 #include <math.h>
 
-#include "paged.cuh"
+#include "paged_attn.cuh"
 
 namespace qb {
 namespace paged {
@@ -124,7 +124,10 @@ uint32_t qb_paged_attention(const void *q, size_t q_len, size_t q_stride, const 
     if (plan->small_items) {
         a.off_items = plan->off_small;
         a.items = (int)plan->small_items;
-        s = wide ? run_rows<float>(a, plan->cache_dtype, st) : run_rows<uint16_t>(a, plan->cache_dtype, st);
+        if (plan->small_kind)
+            s = cuda_status(step_attention(a, wide, (int)plan->cache_dtype, (int)plan->small_kind, st));
+        else
+            s = wide ? run_rows<float>(a, plan->cache_dtype, st) : run_rows<uint16_t>(a, plan->cache_dtype, st);
         if (s) return s;
     }
     if (plan->tile_items) return QB_UNSUPPORTED;

@@ -31,7 +31,7 @@ struct Grid {
 
 // The plain form of every variant: 8 rows and 64 keys a unit, one warp a row.
 Grid rows_grid() { return Grid{64, 8, 148 * 4, 1, 1, 2}; }
-Grid step_grid(int, int, bool) { return rows_grid(); }
+Grid step_grid(int, int, bool) { return Grid{kPage, 8, 148 * 2, 16, 8, 32}; }
 Grid tile_grid(int, int, bool) { return rows_grid(); }
 
 Block block_of(const qb_paged_step &s, const Grid &g, int seq, int kvh, int row0, int rows, int G) {
@@ -181,7 +181,7 @@ uint32_t build(const qb_paged_step &s, int32_t *words, size_t capacity, qb_paged
 
     const int G = (int)(s.query_heads / s.kv_heads), hd = (int)s.head_dim;
     const bool wide = s.value_dtype == QB_PAGED_F32;
-    const bool fast = false;
+    const bool fast = (hd == 64 || hd == 128) && s.cache_dtype != QB_PAGED_F32;
     const Grid small = fast ? step_grid(hd, (int)s.cache_dtype, wide) : rows_grid();
     const Grid tile = tile_grid(hd, (int)s.cache_dtype, wide);
     // Two n8 tiles a block only where some sequence of the list has use for them.
@@ -192,7 +192,7 @@ uint32_t build(const qb_paged_step &s, int32_t *words, size_t capacity, qb_paged
     std::vector<Block> bs, bt;
     for (size_t i = 0; i < s.sequences; ++i) {
         const int64_t r = (int64_t)s.counts[i] * G;
-        const bool to_tile = fast && r > kStepRows;
+        const bool to_tile = false;
         const Grid &g = to_tile ? tile : small;
         const int64_t step = to_tile ? g.block : fast ? 8 * nt : g.block;
         for (size_t h = 0; h < s.kv_heads; ++h)
