@@ -14,7 +14,7 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "libqwen_b200.so")
-SOURCES = ["ops.cu", "decode.cu", "prefill.cu", "tc_gemm.cu", "tp.cu", "sampling.cu", "runtime.cu", "static_scratch.cu", "paged_plan.cpp", "paged_kv.cu", "paged_attn.cu", "paged_step.cu", "synthetic.cpp", "loader.cpp", "bridge.cpp", "tokenizer.cpp"]
+SOURCES = ["ops.cu", "decode.cu", "prefill.cu", "tc_gemm.cu", "tp.cu", "sampling.cu", "runtime.cu", "static_scratch.cu", "paged_plan.cpp", "paged_kv.cu", "paged_attn.cu", "paged_step.cu", "paged_tile.cu", "synthetic.cpp", "loader.cpp", "bridge.cpp", "tokenizer.cpp"]
 HEADERS = ["common.cuh", "decode.cuh", "prefill.cuh", "multitoken.cuh", "tc_gemm.cuh", "tp.cuh", "sampling.cuh", "paged.cuh", "paged_attn.cuh", "json.h", "unicode_tables.inc"]
 
 NVCC_FLAGS = [

@@ -130,7 +130,11 @@ uint32_t qb_paged_attention(const void *q, size_t q_len, size_t q_stride, const 
             s = wide ? run_rows<float>(a, plan->cache_dtype, st) : run_rows<uint16_t>(a, plan->cache_dtype, st);
         if (s) return s;
     }
-    if (plan->tile_items) return QB_UNSUPPORTED;
+    if (plan->tile_items) {
+        a.off_items = plan->off_tile;
+        a.items = (int)plan->tile_items;
+        QB_CUDA(tile_attention(a, wide, (int)plan->cache_dtype, plan->pages * plan->kv_heads * kPage, st));
+    }
     if (plan->merges) {
         if (wide)
             merge_rows<float><<<a.merges, kMergeWarps * 32, 0, st>>>(a);

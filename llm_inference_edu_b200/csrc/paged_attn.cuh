@@ -23,6 +23,8 @@ __device__ __forceinline__ uint32_t s8x2_to_bf16x2(uint32_t t) {
 
 // One CTA an item; nt: n8 tiles of an item's rows.
 cudaError_t step_attention(const Args &a, bool wide, int cache, int nt, cudaStream_t st);
+// One CTA an item; pool_rows: rows of a pool (pages * kv_heads * 16).
+cudaError_t tile_attention(const Args &a, bool wide, int cache, size_t pool_rows, cudaStream_t st);
 
 }  // namespace paged
 }  // namespace qb

@@ -32,7 +32,7 @@ struct Grid {
 // The plain form of every variant: 8 rows and 64 keys a unit, one warp a row.
 Grid rows_grid() { return Grid{64, 8, 148 * 4, 1, 1, 2}; }
 Grid step_grid(int, int, bool) { return Grid{kPage, 8, 148 * 2, 16, 8, 32}; }
-Grid tile_grid(int, int, bool) { return rows_grid(); }
+Grid tile_grid(int, int, bool wide) { return Grid{wide ? 64 : 128, wide ? 128 : 256, 148, wide ? 4 : 3, 2, wide ? 4 : 2}; }
 
 Block block_of(const qb_paged_step &s, const Grid &g, int seq, int kvh, int row0, int rows, int G) {
     Block b{seq, kvh, row0, rows, 0, 0, 0, 0, 0};
@@ -192,7 +192,7 @@ uint32_t build(const qb_paged_step &s, int32_t *words, size_t capacity, qb_paged
     std::vector<Block> bs, bt;
     for (size_t i = 0; i < s.sequences; ++i) {
         const int64_t r = (int64_t)s.counts[i] * G;
-        const bool to_tile = false;
+        const bool to_tile = fast && r > kStepRows;
         const Grid &g = to_tile ? tile : small;
         const int64_t step = to_tile ? g.block : fast ? 8 * nt : g.block;
         for (size_t h = 0; h < s.kv_heads; ++h)

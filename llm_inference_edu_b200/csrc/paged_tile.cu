@@ -1,0 +1,821 @@
+// Attention of many rows (prompt chunks) over the paged cache on the
+// tcgen05 tensor cores, one CTA an item.
+//
+// The packed rows of one sequence and KV head (token-major, the group's
+// query heads innermost) are the M = 128 of the MMAs, so a group of seven
+// heads fills the tile and the causal edge of 128 rows is only 18 tokens
+// long.  Two softmax streams alternate on the tensor cores: while one
+// exponentiates its scores, the products of the other run.
+//   rows > 128 (BF16 values): each stream has its own 128 rows and both use
+//     every key tile, so a key tile is loaded once for 256 rows;
+//   otherwise: both streams have the same rows and take every other key tile;
+//     their results are joined at the end.
+// Per key tile of a stream: S = Q K^T into tensor memory; each thread of the
+// stream's warpgroup owns a row, finds the maximum (which may lag by 2^8, so
+// O is rarely rescaled), writes the weights back over S as the bf16 A
+// operand of O += P V, and keeps the row's sum in FP32.
+// FP32 values: Q and the weights are three bf16 planes (exact to 2^-24) and
+// a key tile has 64 keys, so that three planes fit where S was.
+// BF16 values: one plane each; the weights' single rounding (2^-9 of each at
+// most) is of the size of the result's own.
+// K tiles are K-major operands as TMA leaves them (128-byte swizzle, a box a
+// page); V tiles are the MN-major operand in the same layout.  INT8 pages
+// are copied raw and widened to bf16 by a warpgroup (exact); their scales
+// multiply scores and weights in the softmax.
+// Every wait is bounded: a role that gives up raises the abort flag, copies
+// and MMAs in flight are drained, TMEM is freed and the item's rows are NaN.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
+#include <atomic>
+#include <mutex>
+
+#include "paged_attn.cuh"
+
+namespace qb {
+namespace paged {
+namespace {
+
+constexpr unsigned long long kWaitNs = 2000000000ull;
+
+template <typename TV, typename TC, int HD_>
+struct Tile {
+    static constexpr bool kInt8 = sizeof(TC) == 1;
+    static constexpr int HD = HD_;
+    static constexpr int NP = sizeof(TV) == 4 ? 3 : 1;  // planes of Q and of the weights
+    static constexpr int KT = NP == 1 ? 128 : 64;       // keys a tile
+    static constexpr int QT = NP == 1 ? 2 : 1;          // row tiles an item may have
+    static constexpr int PN = HD / 64;                  // 64-element panels of a row
+    static constexpr int kTileBytes = KT * HD * 2;
+    static constexpr int kQBytes = QT * NP * PN * 128 * 128;
+    // Operand stages of each ring, raw INT8 pieces of 64 keys, scale slots.
+    static constexpr int NS = kTileBytes == 32768 ? 2 : kInt8 && HD == 128 ? 3 : 4;
+    static constexpr int kPiece = 64 * HD;
+    static constexpr int RS = kInt8 ? (HD == 128 ? 3 : 4) : 0;
+    static constexpr int D = kInt8 ? 4 : 0;
+    static constexpr int kThreads = kInt8 ? 512 : 384;
+    static constexpr size_t kv_off = kQBytes, raw_off = kv_off + (size_t)2 * NS * kTileBytes,
+                            scl_off = raw_off + (size_t)RS * kPiece, ctl_off = scl_off + (size_t)D * 2 * KT * 4;
+    static constexpr size_t bytes = ctl_off + 1024 + 1024;
+    static_assert(bytes <= 232448, "shared memory of a CTA");
+};
+
+// Barriers and flags, after the tiles.
+struct Ctl {
+    uint64_t q_full, done;
+    uint64_t s_full[2], p_full[2];
+    uint64_t k_full[4], k_empty[4], v_land[4], v_full[4], v_empty[4];
+    uint64_t raw_full[4], raw_empty[4], scl_full[4], scl_empty[4];
+    uint32_t tmem;
+    int abort_;
+    uint8_t bad[256];
+};
+static_assert(sizeof(Ctl) <= 1024, "control block");
+
+__device__ __noinline__ bool wait_slow(uint64_t *bar, uint32_t parity, volatile int *abort_) {
+    const uint64_t t0 = globaltimer_ns();
+#pragma unroll 1
+    for (unsigned it = 1;; ++it) {
+        if (mbar_try_wait_suspend(bar, parity, 1000)) return true;
+        if ((it & 15u) == 0 && (*abort_ || globaltimer_ns() - t0 > kWaitNs)) {
+            *abort_ = 1;
+            return false;
+        }
+    }
+}
+__device__ __forceinline__ bool wait(uint64_t *bar, uint32_t parity, Ctl *ctl) {
+    return mbar_try_wait(bar, parity) || wait_slow(bar, parity, &ctl->abort_);
+}
+// Copies and MMAs already issued: bounded by time alone.
+__device__ __noinline__ bool wait_issued(uint64_t *bar, uint32_t parity) {
+    const uint64_t t0 = globaltimer_ns();
+#pragma unroll 1
+    while (!mbar_try_wait_suspend(bar, parity, 1000))
+        if (globaltimer_ns() - t0 > kWaitNs) return false;
+    return true;
+}
+
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void commit(uint64_t *bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar))
+                 : "memory");
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc)
+        : "memory");
+}
+// A from tensor memory (bf16 pairs along the columns).
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc)
+        : "memory");
+}
+__device__ __forceinline__ void tma_2d(void *dst, const CUtensorMap *m, int x, int y, uint64_t *bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
+            smem_addr(dst)),
+        "l"((uint64_t)m), "r"(x), "r"(y), "r"(smem_addr(bar))
+        : "memory");
+}
+
+#define QB_R8(v, o) "=r"(v[o]), "=r"(v[o + 1]), "=r"(v[o + 2]), "=r"(v[o + 3]), "=r"(v[o + 4]), "=r"(v[o + 5]), "=r"(v[o + 6]), "=r"(v[o + 7])
+// 32 columns of this warp's 32 lanes; valid after wait_ld.
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&v)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : QB_R8(v, 0), QB_R8(v, 8), QB_R8(v, 16), QB_R8(v, 24)
+        : "r"(taddr));
+}
+#undef QB_R8
+#define QB_R8(v, o) "r"(v[o]), "r"(v[o + 1]), "r"(v[o + 2]), "r"(v[o + 3]), "r"(v[o + 4]), "r"(v[o + 5]), "r"(v[o + 6]), "r"(v[o + 7])
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+        QB_R8(v, 0), QB_R8(v, 8), QB_R8(v, 16), QB_R8(v, 24)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16};" ::"r"(taddr),
+        QB_R8(v, 0), QB_R8(v, 8)
+        : "memory");
+}
+#undef QB_R8
+__device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Shared-memory operand descriptors, 128-byte swizzle.  K-major: 8-row
+// groups 1024 bytes apart.  MN-major: 64-element panels `panel` bytes apart,
+// groups of 8 reduction rows 1024 bytes apart.
+__device__ __forceinline__ uint64_t desc_k(uint32_t saddr) {
+    return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) |
+           ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+__device__ __forceinline__ uint64_t desc_mn(uint32_t saddr, uint32_t panel) {
+    return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)(panel >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+           ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+// BF16 operands, FP32 result, M = 128; b_mn: B is MN-major.
+__host__ __device__ constexpr uint32_t idesc(int n, bool b_mn) {
+    return (1u << 4) | (1u << 7) | (1u << 10) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | (8u << 24);
+}
+
+// (a0, a1) * (b0, b1) + (c0, c1) in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
+        "fma.rn.f32x2 x, x, y, z;\n\tmov.b64 {%0, %1}, x;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+        "mul.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+        "add.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+
+// The order in which the tiles of both operands are produced: K one tile
+// ahead of V.  Position x: K 0, K 1, V 0, K 2, V 1, ..., V n-1.
+__device__ __forceinline__ void nth(int x, int n, bool &is_k, int &tile) {
+    if (x == 0) {
+        is_k = true;
+        tile = 0;
+    } else if (x < 2 * n - 1) {
+        is_k = x & 1;
+        tile = is_k ? (x + 1) / 2 : x / 2 - 1;
+    } else {
+        is_k = false;
+        tile = n - 1;
+    }
+}
+
+template <typename TV, typename TC, int HD>
+__global__ void __launch_bounds__(Tile<TV, TC, HD>::kThreads, 1)
+    attend_tile(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv, const Args a) {
+    using T = Tile<TV, TC, HD>;
+    constexpr int NP = T::NP, KT = T::KT, NS = T::NS, PN = T::PN, RS = T::RS, D = T::D;
+    constexpr int kPages = KT / kPage;
+    extern __shared__ uint8_t raw_[];
+    uint8_t *sm = (uint8_t *)(((uintptr_t)raw_ + 1023) & ~(uintptr_t)1023);
+    uint8_t *s_q = sm, *s_k = sm + T::kv_off, *s_v = s_k + (size_t)NS * T::kTileBytes;
+    uint8_t *s_raw = sm + T::raw_off;
+    float *s_scl = (float *)(sm + T::scl_off);  // [D][k, v][KT]
+    Ctl *ctl = (Ctl *)(sm + T::ctl_off);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const Item it = *(const Item *)(a.words + a.off_items + (size_t)blockIdx.x * 12);
+    const SeqRec sq = *(const SeqRec *)(a.words + a.off_seqs + it.seq * 4);
+    const int32_t *table = a.words + sq.table;
+    const int nk = it.i1 - it.i0;
+    const bool shared = it.rows > 128;
+    const int steps = shared ? 2 * nk : nk;
+    auto key0 = [&](int i) {  // first key of the item's i-th tile
+        const int u = it.i0 + i;
+        return (u < it.ns ? u : it.u0 + u - it.ns) * KT;
+    };
+    auto none = [&](int j) { return j >= it.hi || (j < it.w0 && j >= a.sinks); };  // hidden from every row
+    // Some row sees a key of page j (in units of pages).
+    auto page_seen = [&](int j) { return j * kPage < it.hi && ((j + 1) * kPage > it.w0 || j * kPage < a.sinks); };
+
+    if (threadIdx.x == 0) {
+        mbar_init(&ctl->q_full, 256);
+        mbar_init(&ctl->done, 1);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&ctl->s_full[i], 1);
+            mbar_init(&ctl->p_full[i], 128);
+        }
+        for (int i = 0; i < 4; ++i) {
+            mbar_init(&ctl->k_full[i], T::kInt8 ? 4 : 1);
+            mbar_init(&ctl->v_full[i], T::kInt8 ? 4 : 1);
+            mbar_init(&ctl->k_empty[i], 1);
+            mbar_init(&ctl->v_empty[i], 1);
+            mbar_init(&ctl->v_land[i], 1);
+            mbar_init(&ctl->raw_full[i], 1);
+            mbar_init(&ctl->raw_empty[i], 4);
+            mbar_init(&ctl->scl_full[i], 1);
+            mbar_init(&ctl->scl_empty[i], shared ? 8 : 4);
+        }
+        ctl->abort_ = 0;
+        fence_mbar_init();
+    }
+    if (threadIdx.x < 256) ctl->bad[threadIdx.x] = 0;
+    if (warp == 11) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&ctl->tmem))
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = ctl->tmem;
+
+    if (warp == 8) {
+        // Producer: BF16 boxes straight into the operand stages (one lane a
+        // page), INT8 pages raw into the pieces.
+        if constexpr (!T::kInt8) {
+            int x = 0;
+#pragma unroll 1
+            for (; x < 2 * nk; ++x) {
+                bool is_k;
+                int i;
+                nth(x, nk, is_k, i);
+                const int st = i % NS;
+                if (i >= NS && !__all_sync(0xffffffffu, wait(is_k ? &ctl->k_empty[st] : &ctl->v_empty[st], (uint32_t)((i / NS - 1) & 1), ctl)))
+                    break;
+                const int pj = key0(i) / kPage + lane;
+                const bool on = lane < kPages && page_seen(pj);
+                const int pages = __popc(__ballot_sync(0xffffffffu, on));
+                uint64_t *bar = is_k ? &ctl->k_full[st] : &ctl->v_land[st];
+                if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)pages * (kPage * HD * 2));
+                __syncwarp();
+                if (on) {
+                    const int row = (table[pj] * a.KV + it.kvh) * kPage;
+                    uint8_t *dst = (is_k ? s_k : s_v) + (size_t)st * T::kTileBytes + lane * (kPage * 128);
+#pragma unroll
+                    for (int p = 0; p < PN; ++p) tma_2d(dst + (size_t)p * KT * 128, is_k ? &mk : &mv, p * 64, row, bar);
+                }
+                __syncwarp();
+            }
+            // Every copy issued must land before the CTA can exit.
+            for (int y = x - 1; y >= 0 && y >= x - 2 * NS - 1; --y) {
+                bool is_k;
+                int i;
+                nth(y, nk, is_k, i);
+                // Later phases of the stage cannot exist: only its last use is waited for.
+                const int last = ([&] {
+                    for (int z = x - 1; z > y; --z) {
+                        bool k2;
+                        int i2;
+                        nth(z, nk, k2, i2);
+                        if (k2 == is_k && i2 % NS == i % NS) return false;
+                    }
+                    return true;
+                })();
+                if (last) wait_issued(is_k ? &ctl->k_full[i % NS] : &ctl->v_land[i % NS], (uint32_t)((i / NS) & 1));
+            }
+        } else {
+            constexpr int per = KT / 64;
+            int z = 0;  // pieces issued
+#pragma unroll 1
+            for (; z < 2 * nk * per; ++z) {
+                bool is_k;
+                int i;
+                nth(z / per, nk, is_k, i);
+                const int st = z % RS;
+                if (z >= RS && !__all_sync(0xffffffffu, wait(&ctl->raw_empty[st], (uint32_t)((z / RS - 1) & 1), ctl))) break;
+                const int pj = key0(i) / kPage + z % per * 4 + lane;
+                const bool on = lane < 4 && page_seen(pj);
+                const int pages = __popc(__ballot_sync(0xffffffffu, on));
+                if (lane == 0) mbar_arrive_expect_tx(&ctl->raw_full[st], (uint32_t)pages * (kPage * HD));
+                __syncwarp();
+                if (on)
+                    bulk_copy_g2s(s_raw + (size_t)st * T::kPiece + lane * (kPage * HD),
+                                  (is_k ? a.k : a.v) + ((size_t)table[pj] * a.KV + it.kvh) * (kPage * HD), kPage * HD,
+                                  &ctl->raw_full[st]);
+                __syncwarp();
+            }
+            for (int y = z > RS ? z - RS : 0; y < z; ++y) wait_issued(&ctl->raw_full[y % RS], (uint32_t)((y / RS) & 1));
+        }
+    } else if (warp == 9) {
+        if (lane == 0) {
+            constexpr uint32_t is = idesc(KT, false), io = idesc(HD, true);
+            auto tile_of = [&](int t) { return shared ? t >> 1 : t; };
+            auto first = [&](int t) { return !shared || !(t & 1); };
+            auto last = [&](int t) { return !shared || (t & 1); };
+            auto scores = [&](int t) {
+                const int i = tile_of(t), st = i % NS, s = t & 1;
+                if (first(t) && !wait(&ctl->k_full[st], (uint32_t)((i / NS) & 1), ctl)) return false;
+                fence_after();
+                const uint32_t q = smem_addr(s_q) + (shared ? s : 0) * (PN * 16384);
+                const uint32_t k = smem_addr(s_k) + st * T::kTileBytes;
+#pragma unroll
+                for (int pl = 0; pl < NP; ++pl)
+#pragma unroll
+                    for (int ks = 0; ks < HD / 16; ++ks)
+                        mma_ss(tmem + s * 256, desc_k(q + (pl * PN + ks / 4) * 16384) + 2 * (ks % 4),
+                               desc_k(k + ks / 4 * (KT * 128)) + 2 * (ks % 4), is, (pl | ks) != 0);
+                commit(&ctl->s_full[s]);
+                if (last(t)) commit(&ctl->k_empty[st]);
+                return true;
+            };
+            bool ok = wait(&ctl->q_full, 0u, ctl);
+            if (ok) ok = scores(0);
+            if (ok && steps > 1) ok = scores(1);
+#pragma unroll 1
+            for (int t = 0; ok && t < steps; ++t) {
+                const int i = tile_of(t), st = i % NS, s = t & 1;
+                if (!wait(&ctl->p_full[s], (uint32_t)((t >> 1) & 1), ctl)) break;
+                if (first(t) && !wait(&ctl->v_full[st], (uint32_t)((i / NS) & 1), ctl)) break;
+                fence_after();
+                const uint32_t v = smem_addr(s_v) + st * T::kTileBytes;
+#pragma unroll
+                for (int pl = 0; pl < NP; ++pl)
+#pragma unroll
+                    for (int kb = 0; kb < KT / 16; ++kb)
+                        mma_ts(tmem + s * 256 + 128, tmem + s * 256 + pl * (KT / 2) + kb * 8,
+                               desc_mn(v + kb * 2048, KT * 128), io, t > 1 || (pl | kb) != 0);
+                if (last(t)) commit(&ctl->v_empty[st]);
+                if (t + 2 < steps) ok = scores(t + 2);
+            }
+            commit(&ctl->done);
+        }
+        __syncwarp();
+    } else if (warp == 10) {
+        if constexpr (!T::kInt8) {
+            // V rows that no row sees may hold anything (0 * inf is not 0).
+#pragma unroll 1
+            for (int i = 0; i < nk; ++i) {
+                const int st = i % NS, j0 = key0(i);
+                if (!__all_sync(0xffffffffu, wait(&ctl->v_land[st], (uint32_t)((i / NS) & 1), ctl))) break;
+                bool fix = false;
+                for (int j = j0 + lane; j < j0 + KT; j += 32) fix |= none(j);
+                if (__any_sync(0xffffffffu, fix)) {
+                    uint32_t *v = (uint32_t *)(s_v + (size_t)st * T::kTileBytes);
+                    for (int r = 0; r < KT; ++r)
+                        if (none(j0 + r))
+#pragma unroll
+                            for (int p = 0; p < PN; ++p) v[p * (KT * 32) + r * 32 + lane] = 0u;
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                }
+                if (lane == 0) mbar_arrive(&ctl->v_full[st]);
+            }
+        } else {
+            // The scales of every tile's keys, a 64-byte copy a page and pool.
+            int i = 0;
+#pragma unroll 1
+            for (; i < nk; ++i) {
+                const int st = i % D;
+                if (i >= D && !__all_sync(0xffffffffu, wait(&ctl->scl_empty[st], (uint32_t)((i / D - 1) & 1), ctl))) break;
+                const int pj = key0(i) / kPage + lane;
+                const bool on = lane < kPages && page_seen(pj);
+                const int pages = __popc(__ballot_sync(0xffffffffu, on));
+                if (lane == 0) mbar_arrive_expect_tx(&ctl->scl_full[st], (uint32_t)pages * 128u);
+                __syncwarp();
+                if (on) {
+                    const size_t at = ((size_t)table[pj] * a.KV + it.kvh) * kPage;
+                    bulk_copy_g2s(s_scl + (st * 2) * KT + lane * kPage, a.ks + at, 64, &ctl->scl_full[st]);
+                    bulk_copy_g2s(s_scl + (st * 2 + 1) * KT + lane * kPage, a.vs + at, 64, &ctl->scl_full[st]);
+                }
+                __syncwarp();
+            }
+            for (int y = i > D ? i - D : 0; y < i; ++y) wait_issued(&ctl->scl_full[y % D], (uint32_t)((y / D) & 1));
+        }
+    } else if (warp >= 12) {
+        if constexpr (T::kInt8) {
+            // INT8 -> bf16 (exact), 64 keys a piece, into the operand layout.
+            constexpr int per = KT / 64, units = T::kPiece / 16 / 128;
+            const int ct = threadIdx.x - 384;
+            bool ok = true;
+#pragma unroll 1
+            for (int z = 0; ok && z < 2 * nk * per; ++z) {
+                bool is_k;
+                int i;
+                nth(z / per, nk, is_k, i);
+                const int rs = z % RS, st = i % NS, half = z % per;
+                ok = half != 0 || i < NS ||
+                     wait(is_k ? &ctl->k_empty[st] : &ctl->v_empty[st], (uint32_t)((i / NS - 1) & 1), ctl);
+                ok = __all_sync(0xffffffffu, ok && wait(&ctl->raw_full[rs], (uint32_t)((z / RS) & 1), ctl));
+                if (!ok) break;
+                const uint8_t *src = s_raw + (size_t)rs * T::kPiece;
+                uint8_t *dst = (is_k ? s_k : s_v) + (size_t)st * T::kTileBytes + half * (64 * 128);
+                uint4 w[units];
+#pragma unroll
+                for (int u = 0; u < units; ++u) w[u] = *(const uint4 *)(src + (u * 128 + ct) * 16);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&ctl->raw_empty[rs]);
+#pragma unroll
+                for (int u = 0; u < units; ++u) {
+                    const int e = u * 128 + ct, key = e / (HD / 16), q = e % (HD / 16);
+                    uint4 o0, o1;
+                    o0.x = s8x2_to_bf16x2(__byte_perm(w[u].x, 0u, 0x4140u));
+                    o0.y = s8x2_to_bf16x2(__byte_perm(w[u].x, 0u, 0x4342u));
+                    o0.z = s8x2_to_bf16x2(__byte_perm(w[u].y, 0u, 0x4140u));
+                    o0.w = s8x2_to_bf16x2(__byte_perm(w[u].y, 0u, 0x4342u));
+                    o1.x = s8x2_to_bf16x2(__byte_perm(w[u].z, 0u, 0x4140u));
+                    o1.y = s8x2_to_bf16x2(__byte_perm(w[u].z, 0u, 0x4342u));
+                    o1.z = s8x2_to_bf16x2(__byte_perm(w[u].w, 0u, 0x4140u));
+                    o1.w = s8x2_to_bf16x2(__byte_perm(w[u].w, 0u, 0x4342u));
+                    uint8_t *r = dst + (q / 4) * (KT * 128) + key * 128;
+                    *(uint4 *)(r + ((((q % 4) * 2) ^ (key & 7)) << 4)) = o0;
+                    *(uint4 *)(r + ((((q % 4) * 2 + 1) ^ (key & 7)) << 4)) = o1;
+                }
+                fence_proxy_async_smem();
+                if (half == per - 1) {
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(is_k ? &ctl->k_full[st] : &ctl->v_full[st]);
+                }
+            }
+        }
+    } else if (warp < 8) {
+        // ---- Q into its planes, then this stream's softmax ----
+        const int s = warp >> 2;
+        {
+            const int nrows = shared ? 256 : 128;
+            const bool vec = (((uintptr_t)a.q | (a.q_stride * sizeof(TV))) & 15) == 0;
+            for (int u = threadIdx.x; u < nrows * (HD / 8); u += 256) {
+                const int r = u / (HD / 8), ch = u % (HD / 8);
+                float v[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = 0.0f;
+                if (r < it.rows) {
+                    const int row = it.row0 + r;
+                    const TV *q = (const TV *)a.q + (size_t)(sq.tok0 + row / a.G) * a.q_stride +
+                                  (size_t)(it.kvh * a.G + row % a.G) * HD + ch * 8;
+                    if (vec) {
+                        if constexpr (NP == 3) {
+                            const float4 x = *(const float4 *)q, y = *(const float4 *)(q + 4);
+                            v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+                            v[4] = y.x; v[5] = y.y; v[6] = y.z; v[7] = y.w;
+                        } else {
+                            const uint4 x = *(const uint4 *)q;
+                            v[0] = bf16_lo(x.x); v[1] = bf16_hi(x.x); v[2] = bf16_lo(x.y); v[3] = bf16_hi(x.y);
+                            v[4] = bf16_lo(x.z); v[5] = bf16_hi(x.z); v[6] = bf16_lo(x.w); v[7] = bf16_hi(x.w);
+                        }
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) v[e] = load_value(q, e);
+                    }
+                }
+                const int rr = r & 127;
+#pragma unroll
+                for (int pl = 0; pl < NP; ++pl) {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        w[e] = pack_bf16(v[2 * e], v[2 * e + 1]);
+                        v[2 * e] -= bf16_lo(w[e]);
+                        v[2 * e + 1] -= bf16_hi(w[e]);
+                    }
+                    uint8_t *dst = s_q + ((r >> 7) * PN + pl * PN + ch / 8) * 16384 + rr * 128 + (((ch & 7) ^ (rr & 7)) << 4);
+                    *(uint4 *)dst = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+            }
+            fence_proxy_async_smem();
+            mbar_arrive(&ctl->q_full);
+        }
+        const int r_in = (warp & 3) * 32 + lane;               // row of the tile
+        const int r = (shared ? s * 128 : 0) + r_in;           // row of the item
+        const int rmax = it.row0 + it.rows - 1;
+        const int pos = sq.start + min(it.row0 + r, rmax) / a.G;
+        const int rb = it.row0 + (shared ? s * 128 : 0);
+        const int p_lo = sq.start + min(rb, rmax) / a.G, p_hi = sq.start + min(rb + 127, rmax) / a.G;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t ts = tmem + s * 256 + lanes, to = ts + 128;
+        const int n_steps = shared ? nk : (nk - s + 1) / 2;
+        const float c = a.c;
+        float m = -INFINITY;   // in units of log2
+        float2 l2 = make_float2(0.0f, 0.0f);
+        bool ok = true;
+#pragma unroll 1
+        for (int n = 0; n < n_steps; ++n) {
+            const int i = shared ? n : 2 * n + s, j0 = key0(i);
+            const bool whole = j0 + KT - 1 <= p_lo && (a.window == 0 || j0 > p_hi - a.window || j0 + KT <= a.sinks);
+            if (!(ok = __all_sync(0xffffffffu, wait(&ctl->s_full[s], (uint32_t)(n & 1), ctl)))) break;
+            fence_after();
+            const float *ks = nullptr, *vs = nullptr;
+            if constexpr (T::kInt8) {
+                if (!(ok = __all_sync(0xffffffffu, wait(&ctl->scl_full[i % D], (uint32_t)((i / D) & 1), ctl)))) break;
+                ks = s_scl + (i % D * 2) * KT;
+                vs = ks + KT;
+            }
+            // A chunk of 32 scores: scaled by the keys' scales, hidden ones -inf.
+            auto finish = [&](uint32_t (&x)[32], int ch) {
+                if constexpr (T::kInt8) {
+#pragma unroll
+                    for (int e = 0; e < 32; e += 4) {
+                        const float4 f = *(const float4 *)(ks + ch * 32 + e);
+                        float2 u = mul2(make_float2(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), make_float2(f.x, f.y));
+                        float2 w = mul2(make_float2(__uint_as_float(x[e + 2]), __uint_as_float(x[e + 3])), make_float2(f.z, f.w));
+                        x[e] = __float_as_uint(u.x);
+                        x[e + 1] = __float_as_uint(u.y);
+                        x[e + 2] = __float_as_uint(w.x);
+                        x[e + 3] = __float_as_uint(w.y);
+                    }
+                }
+                if (!whole) {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e)
+                        if (!sees(pos, j0 + ch * 32 + e, a.window, a.sinks)) x[e] = 0xff800000u;
+                }
+            };
+            float bm = -INFINITY;
+            uint32_t hold[KT == 64 ? 2 : 1][32];
+#pragma unroll
+            for (int ch = 0; ch < KT / 32; ++ch) {
+                uint32_t(&x)[32] = hold[KT == 64 ? ch : 0];
+                tmem_ld32(ts + ch * 32, x);
+                wait_ld();
+                finish(x, ch);
+                float m0 = __uint_as_float(x[0]), m1 = __uint_as_float(x[1]);
+#pragma unroll
+                for (int e = 2; e < 32; e += 2) {
+                    m0 = fmaxf(m0, __uint_as_float(x[e]));
+                    m1 = fmaxf(m1, __uint_as_float(x[e + 1]));
+                }
+                bm = fmaxf(bm, fmaxf(m0, m1));
+            }
+            bm *= c;
+            const bool grow = bm > m + 8.0f;
+            if (__any_sync(0xffffffffu, grow)) {
+                const float mn = fmaxf(m, bm), f = m == mn ? 1.0f : ex2(m - mn);
+                m = mn;
+                l2.x *= f;
+                l2.y *= f;
+                if (n > 0) {
+                    // The products that were issued before these scores are done.
+#pragma unroll 1
+                    for (int d = 0; d < HD; d += 32) {
+                        uint32_t x[32];
+                        tmem_ld32(to + d, x);
+                        wait_ld();
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * f);
+                        tmem_st32(to + d, x);
+                    }
+                }
+            }
+            const float base = m == -INFINITY ? 0.0f : m;
+            const float2 c2 = make_float2(c, c), b2 = make_float2(-base, -base);
+#pragma unroll
+            for (int ch = 0; ch < KT / 32; ++ch) {
+                uint32_t(&x)[32] = hold[KT == 64 ? ch : 0];
+                if constexpr (KT != 64) {
+                    tmem_ld32(ts + ch * 32, x);
+                    wait_ld();
+                    finish(x, ch);
+                }
+                float2 p[16];
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    p[e] = fma2(make_float2(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1])), c2, b2);
+                    p[e].x = ex2(p[e].x);
+                    p[e].y = ex2(p[e].y);
+                    l2 = add2(l2, p[e]);
+                }
+                if constexpr (T::kInt8) {
+#pragma unroll
+                    for (int e = 0; e < 16; e += 2) {
+                        const float4 f = *(const float4 *)(vs + ch * 32 + 2 * e);
+                        const float2 u = mul2(p[e], make_float2(f.x, f.y)), w = mul2(p[e + 1], make_float2(f.z, f.w));
+                        if (whole) {
+                            p[e] = u;
+                            p[e + 1] = w;
+                        } else {
+                            // A hidden key's scale may be anything.
+                            p[e].x = p[e].x == 0.0f ? 0.0f : u.x;
+                            p[e].y = p[e].y == 0.0f ? 0.0f : u.y;
+                            p[e + 1].x = p[e + 1].x == 0.0f ? 0.0f : w.x;
+                            p[e + 1].y = p[e + 1].y == 0.0f ? 0.0f : w.y;
+                        }
+                    }
+                }
+#pragma unroll
+                for (int pl = 0; pl < NP; ++pl) {
+                    uint32_t w[16];
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        w[e] = pack_bf16(p[e].x, p[e].y);
+                        if (pl + 1 < NP) {
+                            p[e].x -= bf16_lo(w[e]);
+                            p[e].y -= bf16_hi(w[e]);
+                        }
+                    }
+                    tmem_st16(ts + pl * (KT / 2) + ch * 16, w);
+                }
+            }
+            wait_st();
+            fence_before();
+            mbar_arrive(&ctl->p_full[s]);
+            if constexpr (T::kInt8) {
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&ctl->scl_empty[i % D]);
+            }
+        }
+        float l = l2.x + l2.y;
+        const bool fin = __all_sync(0xffffffffu, wait_issued(&ctl->done, 0u) && ok && !ctl->abort_);
+        fence_after();
+        // ---- the rows' results ----
+        bool write = r < it.rows;
+        float f0 = 1.0f;
+        float *s_o = (float *)s_k;  // stream 1's part where both had the same rows
+        constexpr int OS = HD + 4;
+        float *s_ml = s_o + 128 * OS;
+        if (!shared && nk > 1) {
+            if (s == 1) {
+                s_ml[r_in] = m;
+                s_ml[128 + r_in] = l;
+#pragma unroll 1
+                for (int d = 0; d < HD; d += 32) {
+                    uint32_t x[32];
+                    tmem_ld32(to + d, x);
+                    wait_ld();
+#pragma unroll
+                    for (int e = 0; e < 32; e += 4)
+                        *(uint4 *)(s_o + r_in * OS + d + e) = make_uint4(x[e], x[e + 1], x[e + 2], x[e + 3]);
+                }
+            }
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+        }
+        float f1 = 0.0f;
+        if (!shared) {
+            write = write && s == 0;
+            if (nk > 1 && s == 0) {
+                const float m1 = s_ml[r_in], l1 = s_ml[128 + r_in], mn = fmaxf(m, m1), base = mn == -INFINITY ? 0.0f : mn;
+                f0 = m == base ? 1.0f : ex2(m - base);
+                f1 = m1 == base ? 1.0f : ex2(m1 - base);
+                l = f0 * l + f1 * l1;
+                m = mn;
+            }
+        }
+        if (shared || s == 0) {
+            const int row = it.row0 + r;
+            const size_t at = ((size_t)(sq.tok0 + row / a.G) * a.H + it.kvh * a.G + row % a.G) * HD;
+            const bool vec = ((uintptr_t)a.y & 15) == 0;
+            const float nan = __uint_as_float(0x7fffffffu);
+            bool bad = false;
+#pragma unroll 1
+            for (int d = 0; d < HD; d += 32) {
+                uint32_t x[32];
+                tmem_ld32(to + d, x);
+                wait_ld();
+                float o[32];
+#pragma unroll
+                for (int e = 0; e < 32; ++e) {
+                    o[e] = __uint_as_float(x[e]) * f0;
+                    if (f1 != 0.0f) o[e] = fmaf(f1, s_o[r_in * OS + d + e], o[e]);
+                    bad |= !isfinite(o[e]);
+                    if (!fin) o[e] = nan;
+                    if (it.slot < 0) o[e] = __fdiv_rn(o[e], l);
+                }
+                if (!write) continue;
+                if (it.slot >= 0) {
+                    float *w = a.ws + it.slot + (size_t)r * HD + d;
+#pragma unroll
+                    for (int e = 0; e < 32; e += 2) *(float2 *)(w + e) = make_float2(o[e], o[e + 1]);
+                } else if constexpr (NP == 3) {
+                    float *y = (float *)a.y + at + d;
+                    if (vec) {
+#pragma unroll
+                        for (int e = 0; e < 32; e += 4) *(float4 *)(y + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) y[e] = o[e];
+                    }
+                } else {
+                    uint16_t *y = (uint16_t *)a.y + at + d;
+                    if (vec) {
+#pragma unroll
+                        for (int e = 0; e < 32; e += 8)
+                            *(uint4 *)(y + e) = make_uint4(pack_bf16(o[e], o[e + 1]), pack_bf16(o[e + 2], o[e + 3]),
+                                                           pack_bf16(o[e + 4], o[e + 5]), pack_bf16(o[e + 6], o[e + 7]));
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) y[e] = bf16_bits(o[e]);
+                    }
+                }
+            }
+            if (write && it.slot >= 0) {
+                a.ws[it.slot + (size_t)it.rows * HD + r] = fin ? m : nan;
+                a.ws[it.slot + (size_t)it.rows * (HD + 1) + r] = l;
+            }
+            // A result that is not finite may be a hidden value's doing (a key
+            // that only some of the rows see) or the planes' (an infinity
+            // times planes of both signs): such rows are done again below.
+            if (write && bad && fin) ctl->bad[r] = 1;
+        }
+    }
+    fence_before();
+    const int redo = __syncthreads_or(warp < 8 && ctl->bad[threadIdx.x & 255]);
+    fence_after();
+    if (warp == 11)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    if (redo)
+        for (int r = warp; r < it.rows; r += T::kThreads / 32)
+            if (ctl->bad[r]) attend_row<TV, TC>(a, it, r, KT, lane);
+}
+
+// ------------------------------------------------------------------ host ----
+
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+    static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+    static std::once_flag once;
+    std::call_once(once, [] {
+        void *p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+            fn = (PFN_cuTensorMapEncodeTiled_v12000)p;
+    });
+    return fn;
+}
+
+// A pool as rows of HD bf16 elements, boxes of one page's 64-element panel.
+bool encode_pool(CUtensorMap &m, const void *base, int hd, size_t rows) {
+    auto fn = encode_fn();
+    if (!fn) return false;
+    cuuint64_t dims[2] = {(cuuint64_t)hd, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)hd * 2};
+    cuuint32_t box[2] = {64, kPage}, es[2] = {1, 1};
+    return fn(&m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, (void *)base, dims, strides, box, es,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename TV, typename TC, int HD>
+cudaError_t launch(const Args &a, size_t pool_rows, cudaStream_t st) {
+    using T = Tile<TV, TC, HD>;
+    // At least what keeps one CTA on an SM: an item takes all of its TMEM.
+    const int smem = (int)(T::bytes > 120 * 1024 ? T::bytes : 120 * 1024);
+    static std::atomic<bool> configured[64];
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+    if (!configured[dev].load()) {
+        e = cudaFuncSetAttribute(attend_tile<TV, TC, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (e != cudaSuccess) return e;
+        configured[dev].store(true);
+    }
+    alignas(64) CUtensorMap mk = {}, mv = {};
+    if (!T::kInt8 && (!encode_pool(mk, a.k, HD, pool_rows) || !encode_pool(mv, a.v, HD, pool_rows)))
+        return cudaErrorInvalidValue;
+    attend_tile<TV, TC, HD><<<a.items, T::kThreads, smem, st>>>(mk, mv, a);
+    return cudaGetLastError();
+}
+
+template <typename TV>
+cudaError_t launch_tv(const Args &a, int cache, size_t rows, cudaStream_t st) {
+    if (cache == QB_PAGED_BF16)
+        return a.hd == 64 ? launch<TV, uint16_t, 64>(a, rows, st) : launch<TV, uint16_t, 128>(a, rows, st);
+    return a.hd == 64 ? launch<TV, int8_t, 64>(a, rows, st) : launch<TV, int8_t, 128>(a, rows, st);
+}
+
+}  // namespace
+
+cudaError_t tile_attention(const Args &a, bool wide, int cache, size_t pool_rows, cudaStream_t st) {
+    return wide ? launch_tv<float>(a, cache, pool_rows, st) : launch_tv<uint16_t>(a, cache, pool_rows, st);
+}
+
+}  // namespace paged
+}  // namespace qb
