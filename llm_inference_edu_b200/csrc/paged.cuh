@@ -92,7 +92,8 @@ __device__ __forceinline__ bool sees(int p, int j, int window, int sinks) {
 // (head widths other than 64 and 128, FP32 caches) and, by those variants,
 // for items whose partly hidden units hold values that are not finite.
 template <typename TV, typename TC>
-__device__ __noinline__ void attend_row(const Args &a, const Item &it, int r, int unit, int lane) {
+__device__ __noinline__ void attend_row(const Args &a, const Item *item, int r, int unit, int lane) {
+    const Item it = *item;
     const SeqRec sq = *(const SeqRec *)(a.words + a.off_seqs + it.seq * 4);
     const int32_t *table = a.words + sq.table;
     const int row = it.row0 + r, p = sq.start + row / a.G;

@@ -12,51 +12,77 @@ constexpr int kRowsWarps = 4;
 
 // One CTA an item, its rows dealt to the warps.
 template <typename TV, typename TC>
-__global__ void __launch_bounds__(kRowsWarps * 32) attend_rows(const Args a) {
-    const Item it = *(const Item *)(a.words + a.off_items + (size_t)blockIdx.x * 12);
-    for (int r = threadIdx.x >> 5; r < it.rows; r += kRowsWarps) attend_row<TV, TC>(a, it, r, 64, threadIdx.x & 31);
+__global__ void __launch_bounds__(kRowsWarps * 32) attend_rows(const __grid_constant__ Args a) {
+    const Item *it = (const Item *)(a.words + a.off_items + (size_t)blockIdx.x * 12);
+    for (int r = threadIdx.x >> 5; r < it->rows; r += kRowsWarps) attend_row<TV, TC>(a, it, r, 64, threadIdx.x & 31);
 }
 
-// Joins the partial results of a row block, one warp a row: M = max m_z,
-// y = sum_z o_z 2^(m_z - M) / sum_z l_z 2^(m_z - M), in part order.
-constexpr int kMergeWarps = 8;
+// Joins the partial results of one row, one CTA a row: M = max m_z,
+// y = sum_z o_z 2^(m_z - M) / sum_z l_z 2^(m_z - M).  The parts are dealt to
+// the warps and the warps' sums added in order, so the result does not
+// depend on timing.  Bound by latency: every load of a warp's parts is
+// independent of the others.
+constexpr int kMergeWarps = 4;
+
+template <typename TV, int V>  // V: dimensions a lane
+__global__ void __launch_bounds__(kMergeWarps * 32) merge_rows(const __grid_constant__ Args a) {
+    __shared__ float s_o[kMergeWarps][32 * V], s_l[kMergeWarps];
+    const Merge mg = *(const Merge *)(a.words + a.off_merges + (size_t)blockIdx.x * 8);
+    const int r = blockIdx.y;
+    if (r >= mg.rows) return;
+    const SeqRec sq = *(const SeqRec *)(a.words + a.off_seqs + mg.seq * 4);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, hd = a.hd;
+    const float *w = a.ws + mg.slot, *wm = w + (size_t)mg.rows * hd + r, *wl = wm + mg.rows;
+    float m = -INFINITY;
+    bool nan = false;
+    for (int z = lane; z < mg.parts; z += 32) {
+        const float mz = wm[(size_t)z * mg.stride];
+        m = fmaxf(m, mz);
+        nan |= mz != mz;
+    }
+#pragma unroll
+    for (int off = 16; off; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
+    if (__any_sync(0xffffffffu, nan)) m = __uint_as_float(0x7fffffffu);
+    const float base = m == -INFINITY ? 0.0f : m;
+    float l = 0.0f, o[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) o[i] = 0.0f;
+#pragma unroll 4
+    for (int z = warp; z < mg.parts; z += kMergeWarps) {
+        const size_t at = (size_t)z * mg.stride;
+        const float f = exp2f(wm[at] - base);
+        l = fmaf(f, wl[at], l);
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (lane + 32 * i < hd) o[i] = fmaf(f, w[at + (size_t)r * hd + lane + 32 * i], o[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) s_o[warp][lane + 32 * i] = o[i];
+    if (lane == 0) s_l[warp] = l;
+    __syncthreads();
+    const int row = mg.row0 + r;
+    const size_t tok = (size_t)sq.tok0 + row / a.G, qh = (size_t)mg.kvh * a.G + row % a.G;
+    TV *y = (TV *)a.y + (tok * a.H + qh) * hd;
+    for (int d = threadIdx.x; d < hd; d += kMergeWarps * 32) {
+        float v = 0.0f, ll = 0.0f;
+#pragma unroll
+        for (int x = 0; x < kMergeWarps; ++x) {
+            v += s_o[x][d];
+            ll += s_l[x];
+        }
+        store_value(y, d, __fdiv_rn(v, ll));
+    }
+}
 
 template <typename TV>
-__global__ void __launch_bounds__(kMergeWarps * 32) merge_rows(const Args a) {
-    const Merge mg = *(const Merge *)(a.words + a.off_merges + (size_t)blockIdx.x * 8);
-    const SeqRec sq = *(const SeqRec *)(a.words + a.off_seqs + mg.seq * 4);
-    const int lane = threadIdx.x & 31, hd = a.hd;
-    for (int r = threadIdx.x >> 5; r < mg.rows; r += kMergeWarps) {
-        const float *w = a.ws + mg.slot;
-        float m = -INFINITY;
-        bool nan = false;
-        for (int z = lane; z < mg.parts; z += 32) {
-            const float mz = w[(size_t)z * mg.stride + (size_t)mg.rows * hd + r];
-            m = fmaxf(m, mz);
-            nan |= mz != mz;
-        }
-#pragma unroll
-        for (int off = 16; off; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
-        if (__any_sync(0xffffffffu, nan)) m = __uint_as_float(0x7fffffffu);
-        const float base = m == -INFINITY ? 0.0f : m;
-        float l = 0.0f, o[kMaxHeadDim / 32];
-#pragma unroll
-        for (int i = 0; i < kMaxHeadDim / 32; ++i) o[i] = 0.0f;
-        for (int z = 0; z < mg.parts; ++z) {
-            const float *p = w + (size_t)z * mg.stride;
-            const float f = exp2f(p[(size_t)mg.rows * hd + r] - base);
-            l = fmaf(f, p[(size_t)mg.rows * (hd + 1) + r], l);
-#pragma unroll
-            for (int i = 0; i < kMaxHeadDim / 32; ++i)
-                if (lane + 32 * i < hd) o[i] = fmaf(f, p[(size_t)r * hd + lane + 32 * i], o[i]);
-        }
-        const int row = mg.row0 + r;
-        const size_t tok = (size_t)sq.tok0 + row / a.G, qh = (size_t)mg.kvh * a.G + row % a.G;
-        TV *y = (TV *)a.y + (tok * a.H + qh) * hd;
-#pragma unroll
-        for (int i = 0; i < kMaxHeadDim / 32; ++i)
-            if (lane + 32 * i < hd) store_value(y, lane + 32 * i, __fdiv_rn(o[i], l));
-    }
+void launch_merge(const Args &a, int rows, cudaStream_t st) {
+    const dim3 grid(a.merges, rows);
+    if (a.hd <= 64)
+        merge_rows<TV, 2><<<grid, kMergeWarps * 32, 0, st>>>(a);
+    else if (a.hd <= 128)
+        merge_rows<TV, 4><<<grid, kMergeWarps * 32, 0, st>>>(a);
+    else
+        merge_rows<TV, 8><<<grid, kMergeWarps * 32, 0, st>>>(a);
 }
 
 template <typename TV>
@@ -137,9 +163,9 @@ uint32_t qb_paged_attention(const void *q, size_t q_len, size_t q_stride, const 
     }
     if (plan->merges) {
         if (wide)
-            merge_rows<float><<<a.merges, kMergeWarps * 32, 0, st>>>(a);
+            launch_merge<float>(a, (int)plan->merge_rows, st);
         else
-            merge_rows<uint16_t><<<a.merges, kMergeWarps * 32, 0, st>>>(a);
+            launch_merge<uint16_t>(a, (int)plan->merge_rows, st);
         QB_CUDA(cudaGetLastError());
     }
     return QB_OK;

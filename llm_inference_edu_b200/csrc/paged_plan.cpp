@@ -226,6 +226,7 @@ uint32_t build(const qb_paged_step &s, int32_t *words, size_t capacity, qb_paged
     p.small_items = (uint32_t)si.size();
     p.tile_items = (uint32_t)ti.size();
     p.merges = (uint32_t)merges.size();
+    for (const Merge &m : merges) p.merge_rows = std::max(p.merge_rows, (uint32_t)m.rows);
     // Records of 4 words and more start on 16 bytes.
     size_t at = 0;
     auto take = [&](size_t words_) {

@@ -68,7 +68,7 @@ struct StepShape {
 };
 
 template <typename TV, typename TC, int HD, int NT>
-__global__ void __launch_bounds__(kStepWarps * 32, 2) attend_step(const Args a) {
+__global__ void __launch_bounds__(kStepWarps * 32, 2) attend_step(const __grid_constant__ Args a) {
     using S = StepShape<TV, TC, HD, NT>;
     constexpr int NQ = S::NQ, NPV = S::NPV, KS = S::KS, MT = S::MT, PG = S::PG, KL = S::KL, VP = S::VP, VW = S::VW;
     __shared__ __align__(16) uint8_t s_raw[S::q_bytes > S::o_bytes ? S::q_bytes : S::o_bytes];
@@ -76,7 +76,8 @@ __global__ void __launch_bounds__(kStepWarps * 32, 2) attend_step(const Args a) 
     uint2 *s_q = (uint2 *)s_raw;  // [plane][n tile][k-step][lane]
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-    const Item it = *(const Item *)(a.words + a.off_items + (size_t)blockIdx.x * 12);
+    const Item *item = (const Item *)(a.words + a.off_items + (size_t)blockIdx.x * 12);
+    const Item it = *item;
     const SeqRec sq = *(const SeqRec *)(a.words + a.off_seqs + it.seq * 4);
     const int32_t *table = a.words + sq.table;
     const int p_lo = sq.start + it.row0 / a.G, p_hi = it.hi - 1;
@@ -355,7 +356,7 @@ __global__ void __launch_bounds__(kStepWarps * 32, 2) attend_step(const Args a) 
 #pragma unroll
             for (int e = 0; e < 4; ++e) bad |= !isfinite(o[nt][t][e]);
     if (__syncthreads_or(bad)) {
-        for (int r = warp; r < it.rows; r += kStepWarps) attend_row<TV, TC>(a, it, r, kPage, lane);
+        for (int r = warp; r < it.rows; r += kStepWarps) attend_row<TV, TC>(a, item, r, kPage, lane);
         return;
     }
 

@@ -15,7 +15,7 @@
 // O is rarely rescaled), writes the weights back over S as the bf16 A
 // operand of O += P V, and keeps the row's sum in FP32.
 // FP32 values: Q and the weights are three bf16 planes (exact to 2^-24) and
-// a key tile has 64 keys, so that three planes fit where S was.
+// a key tile has 64 keys, so that three planes fit beside S.
 // BF16 values: one plane each; the weights' single rounding (2^-9 of each at
 // most) is of the size of the result's own.
 // K tiles are K-major operands as TMA leaves them (128-byte swizzle, a box a
@@ -53,7 +53,22 @@ struct Tile {
     static constexpr int kPiece = 64 * HD;
     static constexpr int RS = kInt8 ? (HD == 128 ? 3 : 4) : 0;
     static constexpr int D = kInt8 ? 4 : 0;
-    static constexpr int kThreads = kInt8 ? 512 : 384;
+    // Warps: 8 softmax, producer, MMA issuer, V fixer or scale producer, TMEM,
+    // and the INT8 converters.
+    static constexpr int CW = kInt8 ? 4 : 0;
+    static constexpr int kThreads = 384 + CW * 32;
+    // FP32 values keep O in the softmax threads' registers: a split of the
+    // launch's registers between them and the other warps.
+    static constexpr int kLaunchRegs = 65536 / kThreads / 8 * 8;
+    static constexpr int kSoftRegs = kInt8 ? 200 : 216, kOtherRegs = kInt8 ? 56 : 72;
+    static_assert(256 * kSoftRegs + (kThreads - 256) * kOtherRegs <= kThreads * kLaunchRegs, "register split");
+    // Columns of a stream: scores from 0 (KT of them), plane 0 of the weights
+    // over the scores that were read already, planes 1 and 2 behind them
+    // (FP32 values only: 64 scores), O from 128.
+    static __host__ __device__ constexpr int plane_col(int pl) { return pl == 0 ? 0 : 32 + 32 * pl; }
+    // Scores held between the maximum and the weights, where they fit.
+    static constexpr bool kHold = NP == 1 ? !kInt8 : HD == 64;
+    static constexpr int CH = NP == 3 && HD == 128 ? 16 : 32;  // scores a step of the softmax
     static constexpr size_t kv_off = kQBytes, raw_off = kv_off + (size_t)2 * NS * kTileBytes,
                             scl_off = raw_off + (size_t)RS * kPiece, ctl_off = scl_off + (size_t)D * 2 * KT * 4;
     static constexpr size_t bytes = ctl_off + 1024 + 1024;
@@ -72,7 +87,7 @@ struct Ctl {
 };
 static_assert(sizeof(Ctl) <= 1024, "control block");
 
-__device__ __noinline__ bool wait_slow(uint64_t *bar, uint32_t parity, volatile int *abort_) {
+__device__ __forceinline__ bool wait_slow(uint64_t *bar, uint32_t parity, volatile int *abort_) {
     const uint64_t t0 = globaltimer_ns();
 #pragma unroll 1
     for (unsigned it = 1;; ++it) {
@@ -87,7 +102,7 @@ __device__ __forceinline__ bool wait(uint64_t *bar, uint32_t parity, Ctl *ctl) {
     return mbar_try_wait(bar, parity) || wait_slow(bar, parity, &ctl->abort_);
 }
 // Copies and MMAs already issued: bounded by time alone.
-__device__ __noinline__ bool wait_issued(uint64_t *bar, uint32_t parity) {
+__device__ __forceinline__ bool wait_issued(uint64_t *bar, uint32_t parity) {
     const uint64_t t0 = globaltimer_ns();
 #pragma unroll 1
     while (!mbar_try_wait_suspend(bar, parity, 1000))
@@ -133,6 +148,14 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&v)[32]) {
         : QB_R8(v, 0), QB_R8(v, 8), QB_R8(v, 16), QB_R8(v, 24)
         : "r"(taddr));
 }
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&v)[32]) { tmem_ld32(taddr, v); }
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&v)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
+        "[%16];"
+        : QB_R8(v, 0), QB_R8(v, 8)
+        : "r"(taddr));
+}
 #undef QB_R8
 #define QB_R8(v, o) "r"(v[o]), "r"(v[o + 1]), "r"(v[o + 2]), "r"(v[o + 3]), "r"(v[o + 4]), "r"(v[o + 5]), "r"(v[o + 6]), "r"(v[o + 7])
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32]) {
@@ -148,6 +171,11 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16
         "%16};" ::"r"(taddr),
         QB_R8(v, 0), QB_R8(v, 8)
         : "memory");
+}
+__device__ __forceinline__ void tmem_st(uint32_t taddr, const uint32_t (&v)[16]) { tmem_st16(taddr, v); }
+__device__ __forceinline__ void tmem_st(uint32_t taddr, const uint32_t (&v)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), QB_R8(v, 0)
+                 : "memory");
 }
 #undef QB_R8
 __device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
@@ -212,9 +240,9 @@ __device__ __forceinline__ void nth(int x, int n, bool &is_k, int &tile) {
 
 template <typename TV, typename TC, int HD>
 __global__ void __launch_bounds__(Tile<TV, TC, HD>::kThreads, 1)
-    attend_tile(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv, const Args a) {
+    attend_tile(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv, const __grid_constant__ Args a) {
     using T = Tile<TV, TC, HD>;
-    constexpr int NP = T::NP, KT = T::KT, NS = T::NS, PN = T::PN, RS = T::RS, D = T::D;
+    constexpr int NP = T::NP, KT = T::KT, NS = T::NS, PN = T::PN, RS = T::RS, D = T::D, CH = T::CH;
     constexpr int kPages = KT / kPage;
     extern __shared__ uint8_t raw_[];
     uint8_t *sm = (uint8_t *)(((uintptr_t)raw_ + 1023) & ~(uintptr_t)1023);
@@ -224,7 +252,8 @@ __global__ void __launch_bounds__(Tile<TV, TC, HD>::kThreads, 1)
     Ctl *ctl = (Ctl *)(sm + T::ctl_off);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const Item it = *(const Item *)(a.words + a.off_items + (size_t)blockIdx.x * 12);
+    const Item *item = (const Item *)(a.words + a.off_items + (size_t)blockIdx.x * 12);
+    const Item it = *item;
     const SeqRec sq = *(const SeqRec *)(a.words + a.off_seqs + it.seq * 4);
     const int32_t *table = a.words + sq.table;
     const int nk = it.i1 - it.i0;
@@ -246,13 +275,13 @@ __global__ void __launch_bounds__(Tile<TV, TC, HD>::kThreads, 1)
             mbar_init(&ctl->p_full[i], 128);
         }
         for (int i = 0; i < 4; ++i) {
-            mbar_init(&ctl->k_full[i], T::kInt8 ? 4 : 1);
-            mbar_init(&ctl->v_full[i], T::kInt8 ? 4 : 1);
+            mbar_init(&ctl->k_full[i], T::kInt8 ? T::CW : 1);
+            mbar_init(&ctl->v_full[i], T::kInt8 ? T::CW : 1);
             mbar_init(&ctl->k_empty[i], 1);
             mbar_init(&ctl->v_empty[i], 1);
             mbar_init(&ctl->v_land[i], 1);
             mbar_init(&ctl->raw_full[i], 1);
-            mbar_init(&ctl->raw_empty[i], 4);
+            mbar_init(&ctl->raw_empty[i], T::kInt8 ? T::CW : 1);
             mbar_init(&ctl->scl_full[i], 1);
             mbar_init(&ctl->scl_empty[i], shared ? 8 : 4);
         }
@@ -270,205 +299,8 @@ __global__ void __launch_bounds__(Tile<TV, TC, HD>::kThreads, 1)
     fence_after();
     const uint32_t tmem = ctl->tmem;
 
-    if (warp == 8) {
-        // Producer: BF16 boxes straight into the operand stages (one lane a
-        // page), INT8 pages raw into the pieces.
-        if constexpr (!T::kInt8) {
-            int x = 0;
-#pragma unroll 1
-            for (; x < 2 * nk; ++x) {
-                bool is_k;
-                int i;
-                nth(x, nk, is_k, i);
-                const int st = i % NS;
-                if (i >= NS && !__all_sync(0xffffffffu, wait(is_k ? &ctl->k_empty[st] : &ctl->v_empty[st], (uint32_t)((i / NS - 1) & 1), ctl)))
-                    break;
-                const int pj = key0(i) / kPage + lane;
-                const bool on = lane < kPages && page_seen(pj);
-                const int pages = __popc(__ballot_sync(0xffffffffu, on));
-                uint64_t *bar = is_k ? &ctl->k_full[st] : &ctl->v_land[st];
-                if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)pages * (kPage * HD * 2));
-                __syncwarp();
-                if (on) {
-                    const int row = (table[pj] * a.KV + it.kvh) * kPage;
-                    uint8_t *dst = (is_k ? s_k : s_v) + (size_t)st * T::kTileBytes + lane * (kPage * 128);
-#pragma unroll
-                    for (int p = 0; p < PN; ++p) tma_2d(dst + (size_t)p * KT * 128, is_k ? &mk : &mv, p * 64, row, bar);
-                }
-                __syncwarp();
-            }
-            // Every copy issued must land before the CTA can exit.
-            for (int y = x - 1; y >= 0 && y >= x - 2 * NS - 1; --y) {
-                bool is_k;
-                int i;
-                nth(y, nk, is_k, i);
-                // Later phases of the stage cannot exist: only its last use is waited for.
-                const int last = ([&] {
-                    for (int z = x - 1; z > y; --z) {
-                        bool k2;
-                        int i2;
-                        nth(z, nk, k2, i2);
-                        if (k2 == is_k && i2 % NS == i % NS) return false;
-                    }
-                    return true;
-                })();
-                if (last) wait_issued(is_k ? &ctl->k_full[i % NS] : &ctl->v_land[i % NS], (uint32_t)((i / NS) & 1));
-            }
-        } else {
-            constexpr int per = KT / 64;
-            int z = 0;  // pieces issued
-#pragma unroll 1
-            for (; z < 2 * nk * per; ++z) {
-                bool is_k;
-                int i;
-                nth(z / per, nk, is_k, i);
-                const int st = z % RS;
-                if (z >= RS && !__all_sync(0xffffffffu, wait(&ctl->raw_empty[st], (uint32_t)((z / RS - 1) & 1), ctl))) break;
-                const int pj = key0(i) / kPage + z % per * 4 + lane;
-                const bool on = lane < 4 && page_seen(pj);
-                const int pages = __popc(__ballot_sync(0xffffffffu, on));
-                if (lane == 0) mbar_arrive_expect_tx(&ctl->raw_full[st], (uint32_t)pages * (kPage * HD));
-                __syncwarp();
-                if (on)
-                    bulk_copy_g2s(s_raw + (size_t)st * T::kPiece + lane * (kPage * HD),
-                                  (is_k ? a.k : a.v) + ((size_t)table[pj] * a.KV + it.kvh) * (kPage * HD), kPage * HD,
-                                  &ctl->raw_full[st]);
-                __syncwarp();
-            }
-            for (int y = z > RS ? z - RS : 0; y < z; ++y) wait_issued(&ctl->raw_full[y % RS], (uint32_t)((y / RS) & 1));
-        }
-    } else if (warp == 9) {
-        if (lane == 0) {
-            constexpr uint32_t is = idesc(KT, false), io = idesc(HD, true);
-            auto tile_of = [&](int t) { return shared ? t >> 1 : t; };
-            auto first = [&](int t) { return !shared || !(t & 1); };
-            auto last = [&](int t) { return !shared || (t & 1); };
-            auto scores = [&](int t) {
-                const int i = tile_of(t), st = i % NS, s = t & 1;
-                if (first(t) && !wait(&ctl->k_full[st], (uint32_t)((i / NS) & 1), ctl)) return false;
-                fence_after();
-                const uint32_t q = smem_addr(s_q) + (shared ? s : 0) * (PN * 16384);
-                const uint32_t k = smem_addr(s_k) + st * T::kTileBytes;
-#pragma unroll
-                for (int pl = 0; pl < NP; ++pl)
-#pragma unroll
-                    for (int ks = 0; ks < HD / 16; ++ks)
-                        mma_ss(tmem + s * 256, desc_k(q + (pl * PN + ks / 4) * 16384) + 2 * (ks % 4),
-                               desc_k(k + ks / 4 * (KT * 128)) + 2 * (ks % 4), is, (pl | ks) != 0);
-                commit(&ctl->s_full[s]);
-                if (last(t)) commit(&ctl->k_empty[st]);
-                return true;
-            };
-            bool ok = wait(&ctl->q_full, 0u, ctl);
-            if (ok) ok = scores(0);
-            if (ok && steps > 1) ok = scores(1);
-#pragma unroll 1
-            for (int t = 0; ok && t < steps; ++t) {
-                const int i = tile_of(t), st = i % NS, s = t & 1;
-                if (!wait(&ctl->p_full[s], (uint32_t)((t >> 1) & 1), ctl)) break;
-                if (first(t) && !wait(&ctl->v_full[st], (uint32_t)((i / NS) & 1), ctl)) break;
-                fence_after();
-                const uint32_t v = smem_addr(s_v) + st * T::kTileBytes;
-#pragma unroll
-                for (int pl = 0; pl < NP; ++pl)
-#pragma unroll
-                    for (int kb = 0; kb < KT / 16; ++kb)
-                        mma_ts(tmem + s * 256 + 128, tmem + s * 256 + pl * (KT / 2) + kb * 8,
-                               desc_mn(v + kb * 2048, KT * 128), io, t > 1 || (pl | kb) != 0);
-                if (last(t)) commit(&ctl->v_empty[st]);
-                if (t + 2 < steps) ok = scores(t + 2);
-            }
-            commit(&ctl->done);
-        }
-        __syncwarp();
-    } else if (warp == 10) {
-        if constexpr (!T::kInt8) {
-            // V rows that no row sees may hold anything (0 * inf is not 0).
-#pragma unroll 1
-            for (int i = 0; i < nk; ++i) {
-                const int st = i % NS, j0 = key0(i);
-                if (!__all_sync(0xffffffffu, wait(&ctl->v_land[st], (uint32_t)((i / NS) & 1), ctl))) break;
-                bool fix = false;
-                for (int j = j0 + lane; j < j0 + KT; j += 32) fix |= none(j);
-                if (__any_sync(0xffffffffu, fix)) {
-                    uint32_t *v = (uint32_t *)(s_v + (size_t)st * T::kTileBytes);
-                    for (int r = 0; r < KT; ++r)
-                        if (none(j0 + r))
-#pragma unroll
-                            for (int p = 0; p < PN; ++p) v[p * (KT * 32) + r * 32 + lane] = 0u;
-                    fence_proxy_async_smem();
-                    __syncwarp();
-                }
-                if (lane == 0) mbar_arrive(&ctl->v_full[st]);
-            }
-        } else {
-            // The scales of every tile's keys, a 64-byte copy a page and pool.
-            int i = 0;
-#pragma unroll 1
-            for (; i < nk; ++i) {
-                const int st = i % D;
-                if (i >= D && !__all_sync(0xffffffffu, wait(&ctl->scl_empty[st], (uint32_t)((i / D - 1) & 1), ctl))) break;
-                const int pj = key0(i) / kPage + lane;
-                const bool on = lane < kPages && page_seen(pj);
-                const int pages = __popc(__ballot_sync(0xffffffffu, on));
-                if (lane == 0) mbar_arrive_expect_tx(&ctl->scl_full[st], (uint32_t)pages * 128u);
-                __syncwarp();
-                if (on) {
-                    const size_t at = ((size_t)table[pj] * a.KV + it.kvh) * kPage;
-                    bulk_copy_g2s(s_scl + (st * 2) * KT + lane * kPage, a.ks + at, 64, &ctl->scl_full[st]);
-                    bulk_copy_g2s(s_scl + (st * 2 + 1) * KT + lane * kPage, a.vs + at, 64, &ctl->scl_full[st]);
-                }
-                __syncwarp();
-            }
-            for (int y = i > D ? i - D : 0; y < i; ++y) wait_issued(&ctl->scl_full[y % D], (uint32_t)((y / D) & 1));
-        }
-    } else if (warp >= 12) {
-        if constexpr (T::kInt8) {
-            // INT8 -> bf16 (exact), 64 keys a piece, into the operand layout.
-            constexpr int per = KT / 64, units = T::kPiece / 16 / 128;
-            const int ct = threadIdx.x - 384;
-            bool ok = true;
-#pragma unroll 1
-            for (int z = 0; ok && z < 2 * nk * per; ++z) {
-                bool is_k;
-                int i;
-                nth(z / per, nk, is_k, i);
-                const int rs = z % RS, st = i % NS, half = z % per;
-                ok = half != 0 || i < NS ||
-                     wait(is_k ? &ctl->k_empty[st] : &ctl->v_empty[st], (uint32_t)((i / NS - 1) & 1), ctl);
-                ok = __all_sync(0xffffffffu, ok && wait(&ctl->raw_full[rs], (uint32_t)((z / RS) & 1), ctl));
-                if (!ok) break;
-                const uint8_t *src = s_raw + (size_t)rs * T::kPiece;
-                uint8_t *dst = (is_k ? s_k : s_v) + (size_t)st * T::kTileBytes + half * (64 * 128);
-                uint4 w[units];
-#pragma unroll
-                for (int u = 0; u < units; ++u) w[u] = *(const uint4 *)(src + (u * 128 + ct) * 16);
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&ctl->raw_empty[rs]);
-#pragma unroll
-                for (int u = 0; u < units; ++u) {
-                    const int e = u * 128 + ct, key = e / (HD / 16), q = e % (HD / 16);
-                    uint4 o0, o1;
-                    o0.x = s8x2_to_bf16x2(__byte_perm(w[u].x, 0u, 0x4140u));
-                    o0.y = s8x2_to_bf16x2(__byte_perm(w[u].x, 0u, 0x4342u));
-                    o0.z = s8x2_to_bf16x2(__byte_perm(w[u].y, 0u, 0x4140u));
-                    o0.w = s8x2_to_bf16x2(__byte_perm(w[u].y, 0u, 0x4342u));
-                    o1.x = s8x2_to_bf16x2(__byte_perm(w[u].z, 0u, 0x4140u));
-                    o1.y = s8x2_to_bf16x2(__byte_perm(w[u].z, 0u, 0x4342u));
-                    o1.z = s8x2_to_bf16x2(__byte_perm(w[u].w, 0u, 0x4140u));
-                    o1.w = s8x2_to_bf16x2(__byte_perm(w[u].w, 0u, 0x4342u));
-                    uint8_t *r = dst + (q / 4) * (KT * 128) + key * 128;
-                    *(uint4 *)(r + ((((q % 4) * 2) ^ (key & 7)) << 4)) = o0;
-                    *(uint4 *)(r + ((((q % 4) * 2 + 1) ^ (key & 7)) << 4)) = o1;
-                }
-                fence_proxy_async_smem();
-                if (half == per - 1) {
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(is_k ? &ctl->k_full[st] : &ctl->v_full[st]);
-                }
-            }
-        }
-    } else if (warp < 8) {
+    if (warp < 8) {
+        if constexpr (NP == 3) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(T::kSoftRegs));
         // ---- Q into its planes, then this stream's softmax ----
         const int s = warp >> 2;
         {
@@ -526,12 +358,37 @@ __global__ void __launch_bounds__(Tile<TV, TC, HD>::kThreads, 1)
         const int n_steps = shared ? nk : (nk - s + 1) / 2;
         const float c = a.c;
         float m = -INFINITY;   // in units of log2
-        float2 l2 = make_float2(0.0f, 0.0f);
+        float2 l2[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+        // FP32 values: each tile's product starts from zero and is added to
+        // O here.  The tensor cores cut their sums instead of rounding them,
+        // and over a long row that adds up (4e-6 of the result at 2,000 keys).
+        float o[NP == 3 ? HD : 1];
+        if constexpr (NP == 3)
+#pragma unroll
+            for (int d = 0; d < HD; ++d) o[d] = 0.0f;
+        auto gather = [&]() {
+            if constexpr (NP == 3) {
+#pragma unroll
+                for (int d = 0; d < HD; d += CH) {
+                    uint32_t x[CH];
+                    tmem_ld(to + d, x);
+                    wait_ld();
+#pragma unroll
+                    for (int e = 0; e < CH; e += 2) {
+                        const float2 w = add2(make_float2(o[d + e], o[d + e + 1]),
+                                              make_float2(__uint_as_float(x[e]), __uint_as_float(x[e + 1])));
+                        o[d + e] = w.x;
+                        o[d + e + 1] = w.y;
+                    }
+                }
+            }
+        };
         bool ok = true;
 #pragma unroll 1
         for (int n = 0; n < n_steps; ++n) {
             const int i = shared ? n : 2 * n + s, j0 = key0(i);
             const bool whole = j0 + KT - 1 <= p_lo && (a.window == 0 || j0 > p_hi - a.window || j0 + KT <= a.sinks);
+            // The products issued before these scores are then done too.
             if (!(ok = __all_sync(0xffffffffu, wait(&ctl->s_full[s], (uint32_t)(n & 1), ctl)))) break;
             fence_after();
             const float *ks = nullptr, *vs = nullptr;
@@ -540,12 +397,14 @@ __global__ void __launch_bounds__(Tile<TV, TC, HD>::kThreads, 1)
                 ks = s_scl + (i % D * 2) * KT;
                 vs = ks + KT;
             }
-            // A chunk of 32 scores: scaled by the keys' scales, hidden ones -inf.
-            auto finish = [&](uint32_t (&x)[32], int ch) {
+            // Key e of the tile is visible up to e_hi, and then above e_lo or below e_sk.
+            const int e_hi = pos - j0, e_lo = a.window ? pos - a.window - j0 : -1, e_sk = a.window ? a.sinks - j0 : 0;
+            // A chunk of scores: scaled by the keys' scales, hidden ones -inf.
+            auto finish = [&](uint32_t (&x)[CH], int ch) {
                 if constexpr (T::kInt8) {
 #pragma unroll
-                    for (int e = 0; e < 32; e += 4) {
-                        const float4 f = *(const float4 *)(ks + ch * 32 + e);
+                    for (int e = 0; e < CH; e += 4) {
+                        const float4 f = *(const float4 *)(ks + ch * CH + e);
                         float2 u = mul2(make_float2(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), make_float2(f.x, f.y));
                         float2 w = mul2(make_float2(__uint_as_float(x[e + 2]), __uint_as_float(x[e + 3])), make_float2(f.z, f.w));
                         x[e] = __float_as_uint(u.x);
@@ -555,36 +414,47 @@ __global__ void __launch_bounds__(Tile<TV, TC, HD>::kThreads, 1)
                     }
                 }
                 if (!whole) {
+                    const int hi = e_hi - ch * CH, lo = e_lo - ch * CH, sk = e_sk - ch * CH;
 #pragma unroll
-                    for (int e = 0; e < 32; ++e)
-                        if (!sees(pos, j0 + ch * 32 + e, a.window, a.sinks)) x[e] = 0xff800000u;
+                    for (int e = 0; e < CH; ++e) x[e] = (e <= hi) & ((e > lo) | (e < sk)) ? x[e] : 0xff800000u;
                 }
             };
+            auto largest = [&](const uint32_t (&x)[CH]) {
+                float q[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) q[e] = __uint_as_float(x[e]);
+#pragma unroll
+                for (int e = 4; e < CH; ++e) q[e & 3] = fmaxf(q[e & 3], __uint_as_float(x[e]));
+                return fmaxf(fmaxf(q[0], q[1]), fmaxf(q[2], q[3]));
+            };
             float bm = -INFINITY;
-            uint32_t hold[KT == 64 ? 2 : 1][32];
+            uint32_t hold[T::kHold ? KT / CH : 1][CH];
+            if constexpr (T::kHold) {
 #pragma unroll
-            for (int ch = 0; ch < KT / 32; ++ch) {
-                uint32_t(&x)[32] = hold[KT == 64 ? ch : 0];
-                tmem_ld32(ts + ch * 32, x);
+                for (int ch = 0; ch < KT / CH; ++ch) tmem_ld(ts + ch * CH, hold[ch]);
                 wait_ld();
-                finish(x, ch);
-                float m0 = __uint_as_float(x[0]), m1 = __uint_as_float(x[1]);
+            }
 #pragma unroll
-                for (int e = 2; e < 32; e += 2) {
-                    m0 = fmaxf(m0, __uint_as_float(x[e]));
-                    m1 = fmaxf(m1, __uint_as_float(x[e + 1]));
+            for (int ch = 0; ch < KT / CH; ++ch) {
+                uint32_t(&x)[CH] = hold[T::kHold ? ch : 0];
+                if constexpr (!T::kHold) {
+                    tmem_ld(ts + ch * CH, x);
+                    wait_ld();
                 }
-                bm = fmaxf(bm, fmaxf(m0, m1));
+                finish(x, ch);
+                bm = fmaxf(bm, largest(x));
             }
             bm *= c;
-            const bool grow = bm > m + 8.0f;
-            if (__any_sync(0xffffffffu, grow)) {
+            if (n > 0) gather();
+            if (__any_sync(0xffffffffu, bm > m + 8.0f)) {
                 const float mn = fmaxf(m, bm), f = m == mn ? 1.0f : ex2(m - mn);
                 m = mn;
-                l2.x *= f;
-                l2.y *= f;
-                if (n > 0) {
-                    // The products that were issued before these scores are done.
+#pragma unroll
+                for (int e = 0; e < 2; ++e) l2[e] = mul2(l2[e], make_float2(f, f));
+                if constexpr (NP == 3) {
+#pragma unroll
+                    for (int d = 0; d < HD; ++d) o[d] *= f;
+                } else if (n > 0) {
 #pragma unroll 1
                     for (int d = 0; d < HD; d += 32) {
                         uint32_t x[32];
@@ -599,25 +469,25 @@ __global__ void __launch_bounds__(Tile<TV, TC, HD>::kThreads, 1)
             const float base = m == -INFINITY ? 0.0f : m;
             const float2 c2 = make_float2(c, c), b2 = make_float2(-base, -base);
 #pragma unroll
-            for (int ch = 0; ch < KT / 32; ++ch) {
-                uint32_t(&x)[32] = hold[KT == 64 ? ch : 0];
-                if constexpr (KT != 64) {
-                    tmem_ld32(ts + ch * 32, x);
+            for (int ch = 0; ch < KT / CH; ++ch) {
+                uint32_t(&x)[CH] = hold[T::kHold ? ch : 0];
+                if constexpr (!T::kHold) {
+                    tmem_ld(ts + ch * CH, x);
                     wait_ld();
                     finish(x, ch);
                 }
-                float2 p[16];
+                float2 p[CH / 2];
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
+                for (int e = 0; e < CH / 2; ++e) {
                     p[e] = fma2(make_float2(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1])), c2, b2);
                     p[e].x = ex2(p[e].x);
                     p[e].y = ex2(p[e].y);
-                    l2 = add2(l2, p[e]);
+                    l2[e & 1] = add2(l2[e & 1], p[e]);
                 }
                 if constexpr (T::kInt8) {
 #pragma unroll
-                    for (int e = 0; e < 16; e += 2) {
-                        const float4 f = *(const float4 *)(vs + ch * 32 + 2 * e);
+                    for (int e = 0; e < CH / 2; e += 2) {
+                        const float4 f = *(const float4 *)(vs + ch * CH + 2 * e);
                         const float2 u = mul2(p[e], make_float2(f.x, f.y)), w = mul2(p[e + 1], make_float2(f.z, f.w));
                         if (whole) {
                             p[e] = u;
@@ -633,16 +503,16 @@ __global__ void __launch_bounds__(Tile<TV, TC, HD>::kThreads, 1)
                 }
 #pragma unroll
                 for (int pl = 0; pl < NP; ++pl) {
-                    uint32_t w[16];
+                    uint32_t w[CH / 2];
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) {
+                    for (int e = 0; e < CH / 2; ++e) {
                         w[e] = pack_bf16(p[e].x, p[e].y);
                         if (pl + 1 < NP) {
                             p[e].x -= bf16_lo(w[e]);
                             p[e].y -= bf16_hi(w[e]);
                         }
                     }
-                    tmem_st16(ts + pl * (KT / 2) + ch * 16, w);
+                    tmem_st(ts + T::plane_col(pl) + ch * (CH / 2), w);
                 }
             }
             wait_st();
@@ -653,10 +523,22 @@ __global__ void __launch_bounds__(Tile<TV, TC, HD>::kThreads, 1)
                 if (lane == 0) mbar_arrive(&ctl->scl_empty[i % D]);
             }
         }
-        float l = l2.x + l2.y;
+        const float2 lsum = add2(l2[0], l2[1]);
+        float l = lsum.x + lsum.y;
         const bool fin = __all_sync(0xffffffffu, wait_issued(&ctl->done, 0u) && ok && !ctl->abort_);
         fence_after();
+        if (n_steps > 0) gather();
         // ---- the rows' results ----
+        constexpr int EC = NP == 3 && HD == 128 ? 16 : 32, kUnroll = NP == 3 ? HD / EC : 1;
+        auto result = [&](int d, uint32_t (&x)[EC]) {
+            if constexpr (NP == 3) {
+#pragma unroll
+                for (int e = 0; e < EC; ++e) x[e] = __float_as_uint(o[d + e]);
+            } else {
+                tmem_ld(to + d, x);
+                wait_ld();
+            }
+        };
         bool write = r < it.rows;
         float f0 = 1.0f;
         float *s_o = (float *)s_k;  // stream 1's part where both had the same rows
@@ -666,13 +548,12 @@ __global__ void __launch_bounds__(Tile<TV, TC, HD>::kThreads, 1)
             if (s == 1) {
                 s_ml[r_in] = m;
                 s_ml[128 + r_in] = l;
-#pragma unroll 1
-                for (int d = 0; d < HD; d += 32) {
-                    uint32_t x[32];
-                    tmem_ld32(to + d, x);
-                    wait_ld();
+#pragma unroll(kUnroll)
+                for (int d = 0; d < HD; d += EC) {
+                    uint32_t x[EC];
+                    result(d, x);
 #pragma unroll
-                    for (int e = 0; e < 32; e += 4)
+                    for (int e = 0; e < EC; e += 4)
                         *(uint4 *)(s_o + r_in * OS + d + e) = make_uint4(x[e], x[e + 1], x[e + 2], x[e + 3]);
                 }
             }
@@ -695,44 +576,44 @@ __global__ void __launch_bounds__(Tile<TV, TC, HD>::kThreads, 1)
             const bool vec = ((uintptr_t)a.y & 15) == 0;
             const float nan = __uint_as_float(0x7fffffffu);
             bool bad = false;
-#pragma unroll 1
-            for (int d = 0; d < HD; d += 32) {
-                uint32_t x[32];
-                tmem_ld32(to + d, x);
-                wait_ld();
-                float o[32];
+            const float inv = __fdiv_rn(1.0f, l);
+#pragma unroll(kUnroll)
+            for (int d = 0; d < HD; d += EC) {
+                uint32_t x[EC];
+                result(d, x);
+                float v[EC];
 #pragma unroll
-                for (int e = 0; e < 32; ++e) {
-                    o[e] = __uint_as_float(x[e]) * f0;
-                    if (f1 != 0.0f) o[e] = fmaf(f1, s_o[r_in * OS + d + e], o[e]);
-                    bad |= !isfinite(o[e]);
-                    if (!fin) o[e] = nan;
-                    if (it.slot < 0) o[e] = __fdiv_rn(o[e], l);
+                for (int e = 0; e < EC; ++e) {
+                    v[e] = __uint_as_float(x[e]) * f0;
+                    if (f1 != 0.0f) v[e] = fmaf(f1, s_o[r_in * OS + d + e], v[e]);
+                    bad |= !isfinite(v[e]);
+                    if (!fin) v[e] = nan;
+                    if (it.slot < 0) v[e] *= inv;
                 }
-                if (!write) continue;
-                if (it.slot >= 0) {
+                if (!write) {
+                } else if (it.slot >= 0) {
                     float *w = a.ws + it.slot + (size_t)r * HD + d;
 #pragma unroll
-                    for (int e = 0; e < 32; e += 2) *(float2 *)(w + e) = make_float2(o[e], o[e + 1]);
+                    for (int e = 0; e < EC; e += 2) *(float2 *)(w + e) = make_float2(v[e], v[e + 1]);
                 } else if constexpr (NP == 3) {
                     float *y = (float *)a.y + at + d;
                     if (vec) {
 #pragma unroll
-                        for (int e = 0; e < 32; e += 4) *(float4 *)(y + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                        for (int e = 0; e < EC; e += 4) *(float4 *)(y + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
                     } else {
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) y[e] = o[e];
+                        for (int e = 0; e < EC; ++e) y[e] = v[e];
                     }
                 } else {
                     uint16_t *y = (uint16_t *)a.y + at + d;
                     if (vec) {
 #pragma unroll
-                        for (int e = 0; e < 32; e += 8)
-                            *(uint4 *)(y + e) = make_uint4(pack_bf16(o[e], o[e + 1]), pack_bf16(o[e + 2], o[e + 3]),
-                                                           pack_bf16(o[e + 4], o[e + 5]), pack_bf16(o[e + 6], o[e + 7]));
+                        for (int e = 0; e < EC; e += 8)
+                            *(uint4 *)(y + e) = make_uint4(pack_bf16(v[e], v[e + 1]), pack_bf16(v[e + 2], v[e + 3]),
+                                                           pack_bf16(v[e + 4], v[e + 5]), pack_bf16(v[e + 6], v[e + 7]));
                     } else {
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) y[e] = bf16_bits(o[e]);
+                        for (int e = 0; e < EC; ++e) y[e] = bf16_bits(v[e]);
                     }
                 }
             }
@@ -745,15 +626,216 @@ __global__ void __launch_bounds__(Tile<TV, TC, HD>::kThreads, 1)
             // times planes of both signs): such rows are done again below.
             if (write && bad && fin) ctl->bad[r] = 1;
         }
+    } else {
+        if constexpr (NP == 3) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(T::kOtherRegs));
+        if (warp == 8) {
+            // Producer: BF16 boxes straight into the operand stages (one lane a
+            // page), INT8 pages raw into the pieces.
+            if constexpr (!T::kInt8) {
+                int x = 0;
+#pragma unroll 1
+                for (; x < 2 * nk; ++x) {
+                    bool is_k;
+                    int i;
+                    nth(x, nk, is_k, i);
+                    const int st = i % NS;
+                    if (i >= NS && !__all_sync(0xffffffffu, wait(is_k ? &ctl->k_empty[st] : &ctl->v_empty[st], (uint32_t)((i / NS - 1) & 1), ctl)))
+                        break;
+                    const int pj = key0(i) / kPage + lane;
+                    const bool on = lane < kPages && page_seen(pj);
+                    const int pages = __popc(__ballot_sync(0xffffffffu, on));
+                    uint64_t *bar = is_k ? &ctl->k_full[st] : &ctl->v_land[st];
+                    if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)pages * (kPage * HD * 2));
+                    __syncwarp();
+                    if (on) {
+                        const int row = (table[pj] * a.KV + it.kvh) * kPage;
+                        uint8_t *dst = (is_k ? s_k : s_v) + (size_t)st * T::kTileBytes + lane * (kPage * 128);
+#pragma unroll
+                        for (int p = 0; p < PN; ++p) tma_2d(dst + (size_t)p * KT * 128, is_k ? &mk : &mv, p * 64, row, bar);
+                    }
+                    __syncwarp();
+                }
+                // Every copy issued must land before the CTA can exit.
+                for (int y = x - 1; y >= 0 && y >= x - 2 * NS - 1; --y) {
+                    bool is_k;
+                    int i;
+                    nth(y, nk, is_k, i);
+                    // Later phases of the stage cannot exist: only its last use is waited for.
+                    const int last = ([&] {
+                        for (int z = x - 1; z > y; --z) {
+                            bool k2;
+                            int i2;
+                            nth(z, nk, k2, i2);
+                            if (k2 == is_k && i2 % NS == i % NS) return false;
+                        }
+                        return true;
+                    })();
+                    if (last) wait_issued(is_k ? &ctl->k_full[i % NS] : &ctl->v_land[i % NS], (uint32_t)((i / NS) & 1));
+                }
+            } else {
+                constexpr int per = KT / 64;
+                int z = 0;  // pieces issued
+#pragma unroll 1
+                for (; z < 2 * nk * per; ++z) {
+                    bool is_k;
+                    int i;
+                    nth(z / per, nk, is_k, i);
+                    const int st = z % RS;
+                    if (z >= RS && !__all_sync(0xffffffffu, wait(&ctl->raw_empty[st], (uint32_t)((z / RS - 1) & 1), ctl))) break;
+                    const int pj = key0(i) / kPage + z % per * 4 + lane;
+                    const bool on = lane < 4 && page_seen(pj);
+                    const int pages = __popc(__ballot_sync(0xffffffffu, on));
+                    if (lane == 0) mbar_arrive_expect_tx(&ctl->raw_full[st], (uint32_t)pages * (kPage * HD));
+                    __syncwarp();
+                    if (on)
+                        bulk_copy_g2s(s_raw + (size_t)st * T::kPiece + lane * (kPage * HD),
+                                      (is_k ? a.k : a.v) + ((size_t)table[pj] * a.KV + it.kvh) * (kPage * HD), kPage * HD,
+                                      &ctl->raw_full[st]);
+                    __syncwarp();
+                }
+                for (int y = z > RS ? z - RS : 0; y < z; ++y) wait_issued(&ctl->raw_full[y % RS], (uint32_t)((y / RS) & 1));
+            }
+        } else if (warp == 9) {
+            if (lane == 0) {
+                constexpr uint32_t is = idesc(KT, false), io = idesc(HD, true);
+                auto tile_of = [&](int t) { return shared ? t >> 1 : t; };
+                auto first = [&](int t) { return !shared || !(t & 1); };
+                auto last = [&](int t) { return !shared || (t & 1); };
+                auto scores = [&](int t) {
+                    const int i = tile_of(t), st = i % NS, s = t & 1;
+                    if (first(t) && !wait(&ctl->k_full[st], (uint32_t)((i / NS) & 1), ctl)) return false;
+                    fence_after();
+                    const uint32_t q = smem_addr(s_q) + (shared ? s : 0) * (PN * 16384);
+                    const uint32_t k = smem_addr(s_k) + st * T::kTileBytes;
+#pragma unroll 1
+                    for (int pl = NP - 1; pl >= 0; --pl)
+#pragma unroll
+                        for (int ks = 0; ks < HD / 16; ++ks)
+                            mma_ss(tmem + s * 256, desc_k(q + (pl * PN + ks / 4) * 16384) + 2 * (ks % 4),
+                                   desc_k(k + ks / 4 * (KT * 128)) + 2 * (ks % 4), is, pl != NP - 1 || ks != 0);
+                    commit(&ctl->s_full[s]);
+                    if (last(t)) commit(&ctl->k_empty[st]);
+                    return true;
+                };
+                bool ok = wait(&ctl->q_full, 0u, ctl);
+                if (ok) ok = scores(0);
+                if (ok && steps > 1) ok = scores(1);
+#pragma unroll 1
+                for (int t = 0; ok && t < steps; ++t) {
+                    const int i = tile_of(t), st = i % NS, s = t & 1;
+                    if (!wait(&ctl->p_full[s], (uint32_t)((t >> 1) & 1), ctl)) break;
+                    if (first(t) && !wait(&ctl->v_full[st], (uint32_t)((i / NS) & 1), ctl)) break;
+                    fence_after();
+                    const uint32_t v = smem_addr(s_v) + st * T::kTileBytes;
+#pragma unroll 1
+                    for (int pl = NP - 1; pl >= 0; --pl)
+#pragma unroll
+                        for (int kb = 0; kb < KT / 16; ++kb)
+                            mma_ts(tmem + s * 256 + 128, tmem + s * 256 + T::plane_col(pl) + kb * 8,
+                                   desc_mn(v + kb * 2048, KT * 128), io, (NP == 1 && t > 1) || pl != NP - 1 || kb != 0);
+                    if (last(t)) commit(&ctl->v_empty[st]);
+                    if (t + 2 < steps) ok = scores(t + 2);
+                }
+                commit(&ctl->done);
+            }
+            __syncwarp();
+        } else if (warp == 10) {
+            if constexpr (!T::kInt8) {
+                // V rows that no row sees may hold anything (0 * inf is not 0).
+#pragma unroll 1
+                for (int i = 0; i < nk; ++i) {
+                    const int st = i % NS, j0 = key0(i);
+                    if (!__all_sync(0xffffffffu, wait(&ctl->v_land[st], (uint32_t)((i / NS) & 1), ctl))) break;
+                    bool fix = false;
+                    for (int j = j0 + lane; j < j0 + KT; j += 32) fix |= none(j);
+                    if (__any_sync(0xffffffffu, fix)) {
+                        uint32_t *v = (uint32_t *)(s_v + (size_t)st * T::kTileBytes);
+                        for (int r = 0; r < KT; ++r)
+                            if (none(j0 + r))
+#pragma unroll
+                                for (int p = 0; p < PN; ++p) v[p * (KT * 32) + r * 32 + lane] = 0u;
+                        fence_proxy_async_smem();
+                        __syncwarp();
+                    }
+                    if (lane == 0) mbar_arrive(&ctl->v_full[st]);
+                }
+            } else {
+                // The scales of every tile's keys, a 64-byte copy a page and pool.
+                int i = 0;
+#pragma unroll 1
+                for (; i < nk; ++i) {
+                    const int st = i % D;
+                    if (i >= D && !__all_sync(0xffffffffu, wait(&ctl->scl_empty[st], (uint32_t)((i / D - 1) & 1), ctl))) break;
+                    const int pj = key0(i) / kPage + lane;
+                    const bool on = lane < kPages && page_seen(pj);
+                    const int pages = __popc(__ballot_sync(0xffffffffu, on));
+                    if (lane == 0) mbar_arrive_expect_tx(&ctl->scl_full[st], (uint32_t)pages * 128u);
+                    __syncwarp();
+                    if (on) {
+                        const size_t at = ((size_t)table[pj] * a.KV + it.kvh) * kPage;
+                        bulk_copy_g2s(s_scl + (st * 2) * KT + lane * kPage, a.ks + at, 64, &ctl->scl_full[st]);
+                        bulk_copy_g2s(s_scl + (st * 2 + 1) * KT + lane * kPage, a.vs + at, 64, &ctl->scl_full[st]);
+                    }
+                    __syncwarp();
+                }
+                for (int y = i > D ? i - D : 0; y < i; ++y) wait_issued(&ctl->scl_full[y % D], (uint32_t)((y / D) & 1));
+            }
+        } else if (warp >= 12) {
+            if constexpr (T::kInt8) {
+                // INT8 -> bf16 (exact), 64 keys a piece, into the operand layout.
+                constexpr int per = KT / 64, units = T::kPiece / 16 / (T::CW * 32);
+                const int ct = threadIdx.x - 384;
+                bool ok = true;
+#pragma unroll 1
+                for (int z = 0; ok && z < 2 * nk * per; ++z) {
+                    bool is_k;
+                    int i;
+                    nth(z / per, nk, is_k, i);
+                    const int rs = z % RS, st = i % NS, half = z % per;
+                    ok = half != 0 || i < NS ||
+                         wait(is_k ? &ctl->k_empty[st] : &ctl->v_empty[st], (uint32_t)((i / NS - 1) & 1), ctl);
+                    ok = __all_sync(0xffffffffu, ok && wait(&ctl->raw_full[rs], (uint32_t)((z / RS) & 1), ctl));
+                    if (!ok) break;
+                    const uint8_t *src = s_raw + (size_t)rs * T::kPiece;
+                    uint8_t *dst = (is_k ? s_k : s_v) + (size_t)st * T::kTileBytes + half * (64 * 128);
+                    uint4 w[units];
+#pragma unroll
+                    for (int u = 0; u < units; ++u) w[u] = *(const uint4 *)(src + (u * T::CW * 32 + ct) * 16);
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&ctl->raw_empty[rs]);
+#pragma unroll
+                    for (int u = 0; u < units; ++u) {
+                        const int e = u * T::CW * 32 + ct, key = e / (HD / 16), q = e % (HD / 16);
+                        uint4 o0, o1;
+                        o0.x = s8x2_to_bf16x2(__byte_perm(w[u].x, 0u, 0x4140u));
+                        o0.y = s8x2_to_bf16x2(__byte_perm(w[u].x, 0u, 0x4342u));
+                        o0.z = s8x2_to_bf16x2(__byte_perm(w[u].y, 0u, 0x4140u));
+                        o0.w = s8x2_to_bf16x2(__byte_perm(w[u].y, 0u, 0x4342u));
+                        o1.x = s8x2_to_bf16x2(__byte_perm(w[u].z, 0u, 0x4140u));
+                        o1.y = s8x2_to_bf16x2(__byte_perm(w[u].z, 0u, 0x4342u));
+                        o1.z = s8x2_to_bf16x2(__byte_perm(w[u].w, 0u, 0x4140u));
+                        o1.w = s8x2_to_bf16x2(__byte_perm(w[u].w, 0u, 0x4342u));
+                        uint8_t *r = dst + (q / 4) * (KT * 128) + key * 128;
+                        *(uint4 *)(r + ((((q % 4) * 2) ^ (key & 7)) << 4)) = o0;
+                        *(uint4 *)(r + ((((q % 4) * 2 + 1) ^ (key & 7)) << 4)) = o1;
+                    }
+                    fence_proxy_async_smem();
+                    if (half == per - 1) {
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(is_k ? &ctl->k_full[st] : &ctl->v_full[st]);
+                    }
+                }
+            }
+        }
     }
     fence_before();
     const int redo = __syncthreads_or(warp < 8 && ctl->bad[threadIdx.x & 255]);
     fence_after();
     if (warp == 11)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
-    if (redo)
-        for (int r = warp; r < it.rows; r += T::kThreads / 32)
-            if (ctl->bad[r]) attend_row<TV, TC>(a, it, r, KT, lane);
+    if (redo && warp < 8)
+        for (int r = warp; r < it.rows; r += 8)
+            if (ctl->bad[r]) attend_row<TV, TC>(a, item, r, KT, lane);
 }
 
 // ------------------------------------------------------------------ host ----
@@ -795,6 +877,11 @@ cudaError_t launch(const Args &a, size_t pool_rows, cudaStream_t st) {
     if (!configured[dev].load()) {
         e = cudaFuncSetAttribute(attend_tile<TV, TC, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
         if (e != cudaSuccess) return e;
+        // The split of the registers counts on what the launch allots.
+        cudaFuncAttributes fa;
+        e = cudaFuncGetAttributes(&fa, attend_tile<TV, TC, HD>);
+        if (e != cudaSuccess) return e;
+        if (T::NP == 3 && fa.numRegs != T::kLaunchRegs) return cudaErrorInvalidConfiguration;
         configured[dev].store(true);
     }
     alignas(64) CUtensorMap mk = {}, mv = {};
