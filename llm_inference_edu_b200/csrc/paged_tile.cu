@@ -112,23 +112,35 @@ __device__ __forceinline__ bool wait_issued(uint64_t *bar, uint32_t parity) {
 
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void commit(uint64_t *bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar))
-                 : "memory");
-}
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
+// Issued by the elected lane of a converged warp: the whole warp walks the
+// issue loop, so that the operands stay in uniform registers (in a one-lane
+// branch each MMA cost 100 cycles to issue, twice its execution).
+__device__ __forceinline__ uint32_t elect_one() {
+    uint32_t r;
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc)
+        "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void commit(uint64_t *bar, uint32_t leader) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_addr(bar)),
+        "r"(leader)
+        : "memory");
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc, uint32_t leader) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc), "r"(leader)
         : "memory");
 }
 // A from tensor memory (bf16 pairs along the columns).
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool acc) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool acc, uint32_t leader) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-        "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc)
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc), "r"(leader)
         : "memory");
 }
 __device__ __forceinline__ void tma_2d(void *dst, const CUtensorMap *m, int x, int y, uint64_t *bar) {
@@ -696,48 +708,57 @@ __global__ void __launch_bounds__(Tile<TV, TC, HD>::kThreads, 1)
                 for (int y = z > RS ? z - RS : 0; y < z; ++y) wait_issued(&ctl->raw_full[y % RS], (uint32_t)((y / RS) & 1));
             }
         } else if (warp == 9) {
-            if (lane == 0) {
-                constexpr uint32_t is = idesc(KT, false), io = idesc(HD, true);
-                auto tile_of = [&](int t) { return shared ? t >> 1 : t; };
-                auto first = [&](int t) { return !shared || !(t & 1); };
-                auto last = [&](int t) { return !shared || (t & 1); };
-                auto scores = [&](int t) {
-                    const int i = tile_of(t), st = i % NS, s = t & 1;
-                    if (first(t) && !wait(&ctl->k_full[st], (uint32_t)((i / NS) & 1), ctl)) return false;
-                    fence_after();
-                    const uint32_t q = smem_addr(s_q) + (shared ? s : 0) * (PN * 16384);
-                    const uint32_t k = smem_addr(s_k) + st * T::kTileBytes;
-#pragma unroll 1
-                    for (int pl = NP - 1; pl >= 0; --pl)
+            constexpr uint32_t is = idesc(KT, false), io = idesc(HD, true);
+            const uint32_t leader = elect_one();
+            const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+            const bool two = __shfl_sync(0xffffffffu, it.rows, 0) > 128;
+            const int total = __shfl_sync(0xffffffffu, steps, 0);
+            const uint32_t q_at = __shfl_sync(0xffffffffu, smem_addr(s_q), 0), k_at = q_at + (uint32_t)T::kv_off,
+                           v_at = k_at + (uint32_t)(NS * T::kTileBytes);
+            auto await = [&](uint64_t *bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity, ctl)); };
+            auto k_ready = [&](int t) {
+                const int i = two ? t >> 1 : t;
+                return (two && (t & 1)) || await(&ctl->k_full[i % NS], (uint32_t)((i / NS) & 1));
+            };
+            auto scores = [&](int t) {
+                const int i = two ? t >> 1 : t, st = i % NS, s = t & 1;
+                const uint32_t q = q_at + (two ? s : 0) * (PN * 16384), k = k_at + st * T::kTileBytes;
 #pragma unroll
-                        for (int ks = 0; ks < HD / 16; ++ks)
-                            mma_ss(tmem + s * 256, desc_k(q + (pl * PN + ks / 4) * 16384) + 2 * (ks % 4),
-                                   desc_k(k + ks / 4 * (KT * 128)) + 2 * (ks % 4), is, pl != NP - 1 || ks != 0);
-                    commit(&ctl->s_full[s]);
-                    if (last(t)) commit(&ctl->k_empty[st]);
-                    return true;
-                };
-                bool ok = wait(&ctl->q_full, 0u, ctl);
-                if (ok) ok = scores(0);
-                if (ok && steps > 1) ok = scores(1);
-#pragma unroll 1
-                for (int t = 0; ok && t < steps; ++t) {
-                    const int i = tile_of(t), st = i % NS, s = t & 1;
-                    if (!wait(&ctl->p_full[s], (uint32_t)((t >> 1) & 1), ctl)) break;
-                    if (first(t) && !wait(&ctl->v_full[st], (uint32_t)((i / NS) & 1), ctl)) break;
-                    fence_after();
-                    const uint32_t v = smem_addr(s_v) + st * T::kTileBytes;
-#pragma unroll 1
-                    for (int pl = NP - 1; pl >= 0; --pl)
+                for (int pl = NP - 1; pl >= 0; --pl)
 #pragma unroll
-                        for (int kb = 0; kb < KT / 16; ++kb)
-                            mma_ts(tmem + s * 256 + 128, tmem + s * 256 + T::plane_col(pl) + kb * 8,
-                                   desc_mn(v + kb * 2048, KT * 128), io, (NP == 1 && t > 1) || pl != NP - 1 || kb != 0);
-                    if (last(t)) commit(&ctl->v_empty[st]);
-                    if (t + 2 < steps) ok = scores(t + 2);
-                }
-                commit(&ctl->done);
+                    for (int ks = 0; ks < HD / 16; ++ks)
+                        mma_ss(tm + s * 256, desc_k(q + (pl * PN + ks / 4) * 16384) + 2 * (ks % 4),
+                               desc_k(k + ks / 4 * (KT * 128)) + 2 * (ks % 4), is, pl != NP - 1 || ks != 0, leader);
+                commit(&ctl->s_full[s], leader);
+                if (!two || s == 1) commit(&ctl->k_empty[st], leader);
+            };
+            bool ok = await(&ctl->q_full, 0u);
+#pragma unroll 1
+            for (int t = 0; t < 2 && t < total && (ok = ok && k_ready(t)); ++t) {
+                fence_after();
+                scores(t);
             }
+#pragma unroll 1
+            for (int t = 0; ok && t < total; ++t) {
+                const int i = two ? t >> 1 : t, st = i % NS, s = t & 1;
+                // The tiles of these products and of the next scores are there
+                // long before the weights: looked at first.
+                if ((!two || s == 0) && !await(&ctl->v_full[st], (uint32_t)((i / NS) & 1))) break;
+                if (t + 2 < total && !k_ready(t + 2)) break;
+                if (!await(&ctl->p_full[s], (uint32_t)((t >> 1) & 1))) break;
+                fence_after();
+                const uint32_t v = v_at + st * T::kTileBytes;
+#pragma unroll
+                for (int pl = NP - 1; pl >= 0; --pl)
+#pragma unroll
+                    for (int kb = 0; kb < KT / 16; ++kb)
+                        mma_ts(tm + s * 256 + 128, tm + s * 256 + T::plane_col(pl) + kb * 8,
+                               desc_mn(v + kb * 2048, KT * 128), io, (NP == 1 && t > 1) || pl != NP - 1 || kb != 0,
+                               leader);
+                if (!two || s == 1) commit(&ctl->v_empty[st], leader);
+                if (t + 2 < total) scores(t + 2);
+            }
+            commit(&ctl->done, leader);
             __syncwarp();
         } else if (warp == 10) {
             if constexpr (!T::kInt8) {
