@@ -49,28 +49,29 @@ struct Tile {
     static constexpr int kTileBytes = KT * HD * 2;
     static constexpr int kQBytes = QT * NP * PN * 128 * 128;
     // Operand stages of each ring, raw INT8 pieces of 64 keys, scale slots.
-    static constexpr int NS = kTileBytes == 32768 ? 2 : kInt8 && HD == 128 ? 3 : 4;
+    static constexpr int NS = kTileBytes == 32768 ? 2 : NP == 3 && HD == 128 ? 3 : 4;
     static constexpr int kPiece = 64 * HD;
     static constexpr int RS = kInt8 ? (HD == 128 ? 3 : 4) : 0;
     static constexpr int D = kInt8 ? 4 : 0;
-    // Warps: 8 softmax, producer, MMA issuer, V fixer or scale producer, TMEM,
-    // and the INT8 converters.
-    static constexpr int CW = kInt8 ? 4 : 0;
-    static constexpr int kThreads = 384 + CW * 32;
-    // FP32 values keep O in the softmax threads' registers: a split of the
-    // launch's registers between them and the other warps.
+    // Warps: 8 softmax, producer, MMA issuer, V fixer or scale producer, TMEM;
+    // 4 that gather O (FP32 values); 4 INT8 converters.
+    static constexpr int kGather = 12, kConvert = NP == 3 ? 16 : 12;
+    static constexpr int kThreads = 384 + (NP == 3 ? 128 : 0) + (kInt8 ? 128 : 0);
+    // O is in registers where it is gathered: a split of the launch's
+    // registers (FP32 values only).
     static constexpr int kLaunchRegs = 65536 / kThreads / 8 * 8;
-    static constexpr int kSoftRegs = kInt8 ? 200 : 216, kOtherRegs = kInt8 ? 56 : 72;
-    static_assert(256 * kSoftRegs + (kThreads - 256) * kOtherRegs <= kThreads * kLaunchRegs, "register split");
+    static constexpr int kSoftRegs = kInt8 ? 112 : 120, kGatherRegs = kInt8 ? 168 : 176, kOtherRegs = kInt8 ? 40 : 88;
+    static_assert(NP == 1 || 256 * kSoftRegs + 128 * kGatherRegs + (kThreads - 384) * kOtherRegs <= kThreads * kLaunchRegs,
+                  "register split");
     // Columns of a stream: scores from 0 (KT of them), plane 0 of the weights
     // over the scores that were read already, planes 1 and 2 behind them
     // (FP32 values only: 64 scores), O from 128.
     static __host__ __device__ constexpr int plane_col(int pl) { return pl == 0 ? 0 : 32 + 32 * pl; }
     // Scores held between the maximum and the weights, where they fit.
-    static constexpr bool kHold = NP == 1 ? !kInt8 : HD == 64;
-    static constexpr int CH = NP == 3 && HD == 128 ? 16 : 32;  // scores a step of the softmax
+    static constexpr bool kHold = NP == 3 || !kInt8;
     static constexpr size_t kv_off = kQBytes, raw_off = kv_off + (size_t)2 * NS * kTileBytes,
-                            scl_off = raw_off + (size_t)RS * kPiece, ctl_off = scl_off + (size_t)D * 2 * KT * 4;
+                            scl_off = raw_off + (size_t)RS * kPiece, max_off = scl_off + (size_t)D * 2 * KT * 4,
+                            ctl_off = max_off + (NP == 3 ? 2048 : 0);
     static constexpr size_t bytes = ctl_off + 1024 + 1024;
     static_assert(bytes <= 232448, "shared memory of a CTA");
 };
@@ -78,7 +79,7 @@ struct Tile {
 // Barriers and flags, after the tiles.
 struct Ctl {
     uint64_t q_full, done;
-    uint64_t s_full[2], p_full[2];
+    uint64_t s_full[2], p_full[2][2], o_full[2], o_empty[2];
     uint64_t k_full[4], k_empty[4], v_land[4], v_full[4], v_empty[4];
     uint64_t raw_full[4], raw_empty[4], scl_full[4], scl_empty[4];
     uint32_t tmem;
@@ -143,11 +144,13 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
         "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc), "r"(leader)
         : "memory");
 }
-__device__ __forceinline__ void tma_2d(void *dst, const CUtensorMap *m, int x, int y, uint64_t *bar) {
+// By the elected lane of a converged warp, as the MMAs.
+__device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap *m, int x, int y, uint32_t bar, uint32_t leader) {
     asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
-            smem_addr(dst)),
-        "l"((uint64_t)m), "r"(x), "r"(y), "r"(smem_addr(bar))
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+        "\n\t}" ::"r"(dst),
+        "l"((uint64_t)m), "r"(x), "r"(y), "r"(bar), "r"(leader)
         : "memory");
 }
 
@@ -160,8 +163,7 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&v)[32]) {
         : QB_R8(v, 0), QB_R8(v, 8), QB_R8(v, 16), QB_R8(v, 24)
         : "r"(taddr));
 }
-__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&v)[32]) { tmem_ld32(taddr, v); }
-__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&v)[16]) {
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&v)[16]) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
         "[%16];"
@@ -170,24 +172,12 @@ __device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&v)[16]) {
 }
 #undef QB_R8
 #define QB_R8(v, o) "r"(v[o]), "r"(v[o + 1]), "r"(v[o + 2]), "r"(v[o + 3]), "r"(v[o + 4]), "r"(v[o + 5]), "r"(v[o + 6]), "r"(v[o + 7])
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32]) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
-        QB_R8(v, 0), QB_R8(v, 8), QB_R8(v, 16), QB_R8(v, 24)
-        : "memory");
-}
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
         "%16};" ::"r"(taddr),
         QB_R8(v, 0), QB_R8(v, 8)
         : "memory");
-}
-__device__ __forceinline__ void tmem_st(uint32_t taddr, const uint32_t (&v)[16]) { tmem_st16(taddr, v); }
-__device__ __forceinline__ void tmem_st(uint32_t taddr, const uint32_t (&v)[8]) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), QB_R8(v, 0)
-                 : "memory");
 }
 #undef QB_R8
 __device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
@@ -235,6 +225,84 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
     return d;
 }
 
+// The largest of three, NaN if one is.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
+// 2^x on the FMA pipe, x <= 8: x = n + f with n the nearest integer (added
+// to and taken from 1.5 * 2^23, whose low bits it then is) and 2^f, |f| <=
+// 1/2, by the polynomial of degree 4 through 1 with the least largest
+// relative error (3e-6, a fraction of a bf16 weight's rounding); n goes into
+// the exponent.  -127 and below (a hidden key's -inf) give 0 exactly: f is 0
+// and the exponent of 1 is 127.  (A NaN is lost here: the row's sum has it.)
+__device__ __forceinline__ float2 ex2_poly(float2 x) {
+    x.x = fmaxf(x.x, -127.0f);
+    x.y = fmaxf(x.y, -127.0f);
+    const float big = 12582912.0f;
+    const float2 n = add2(x, make_float2(big, big));
+    const float2 f = fma2(add2(n, make_float2(-big, -big)), make_float2(-1.0f, -1.0f), x);
+    float2 y = make_float2(0.00958104711f, 0.00958104711f);
+    y = fma2(y, f, make_float2(0.0559059717f, 0.0559059717f));
+    y = fma2(y, f, make_float2(0.240241453f, 0.240241453f));
+    y = fma2(y, f, make_float2(0.693124354f, 0.693124354f));
+    y = fma2(y, f, make_float2(1.0f, 1.0f));
+    y.x = __uint_as_float(__float_as_uint(y.x) + (__float_as_uint(n.x) << 23));
+    y.y = __uint_as_float(__float_as_uint(y.y) + (__float_as_uint(n.y) << 23));
+    return y;
+}
+
+// Two parts of a row's softmax: maximum, sum, and the parts' factors.
+struct Join {
+    float m, l, f0, f1;
+};
+__device__ __forceinline__ Join join(float m0, float l0, float m1, float l1) {
+    Join j;
+    j.m = fmaxf(m0, m1);
+    const float base = j.m == -INFINITY ? 0.0f : j.m;
+    j.f0 = m0 == base ? 1.0f : ex2(m0 - base);
+    j.f1 = m1 == base ? 1.0f : ex2(m1 - base);
+    j.l = j.f0 * l0 + j.f1 * l1;
+    return j;
+}
+
+// Dimensions d .. d + 31 of a row's result: divided by the sum, or as the
+// item's part with its maximum and sum.
+template <typename TV, int HD>
+__device__ __forceinline__ void put_row(const Args &a, const Item &it, const SeqRec &sq, int r, int d, float (&v)[32],
+                                        float m, float l) {
+    if (it.slot >= 0) {
+        float *w = a.ws + it.slot + (size_t)r * HD + d;
+#pragma unroll
+        for (int e = 0; e < 32; e += 2) *(float2 *)(w + e) = make_float2(v[e], v[e + 1]);
+        if (d == 0) {
+            a.ws[it.slot + (size_t)it.rows * HD + r] = m;
+            a.ws[it.slot + (size_t)it.rows * (HD + 1) + r] = l;
+        }
+        return;
+    }
+    const int row = it.row0 + r;
+    const size_t at = ((size_t)(sq.tok0 + row / a.G) * a.H + it.kvh * a.G + row % a.G) * HD + d;
+    const float inv = __fdiv_rn(1.0f, l);
+#pragma unroll
+    for (int e = 0; e < 32; ++e) v[e] *= inv;
+    TV *y = (TV *)a.y + at;
+    if ((uintptr_t)a.y & 15) {
+#pragma unroll
+        for (int e = 0; e < 32; ++e) store_value(y, e, v[e]);
+    } else if constexpr (sizeof(TV) == 4) {
+#pragma unroll
+        for (int e = 0; e < 32; e += 4) *(float4 *)(y + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 32; e += 8)
+            *(uint4 *)(y + e) = make_uint4(pack_bf16(v[e], v[e + 1]), pack_bf16(v[e + 2], v[e + 3]),
+                                           pack_bf16(v[e + 4], v[e + 5]), pack_bf16(v[e + 6], v[e + 7]));
+    }
+}
+
 // The order in which the tiles of both operands are produced: K one tile
 // ahead of V.  Position x: K 0, K 1, V 0, K 2, V 1, ..., V n-1.
 __device__ __forceinline__ void nth(int x, int n, bool &is_k, int &tile) {
@@ -254,13 +322,14 @@ template <typename TV, typename TC, int HD>
 __global__ void __launch_bounds__(Tile<TV, TC, HD>::kThreads, 1)
     attend_tile(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv, const __grid_constant__ Args a) {
     using T = Tile<TV, TC, HD>;
-    constexpr int NP = T::NP, KT = T::KT, NS = T::NS, PN = T::PN, RS = T::RS, D = T::D, CH = T::CH;
+    constexpr int NP = T::NP, KT = T::KT, NS = T::NS, PN = T::PN, RS = T::RS, D = T::D, CH = 32;
     constexpr int kPages = KT / kPage;
     extern __shared__ uint8_t raw_[];
     uint8_t *sm = (uint8_t *)(((uintptr_t)raw_ + 1023) & ~(uintptr_t)1023);
     uint8_t *s_q = sm, *s_k = sm + T::kv_off, *s_v = s_k + (size_t)NS * T::kTileBytes;
     uint8_t *s_raw = sm + T::raw_off;
     float *s_scl = (float *)(sm + T::scl_off);  // [D][k, v][KT]
+    float *s_max = (float *)(sm + T::max_off);  // [stream][step & 1][row]
     Ctl *ctl = (Ctl *)(sm + T::ctl_off);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -284,16 +353,19 @@ __global__ void __launch_bounds__(Tile<TV, TC, HD>::kThreads, 1)
         mbar_init(&ctl->done, 1);
         for (int i = 0; i < 2; ++i) {
             mbar_init(&ctl->s_full[i], 1);
-            mbar_init(&ctl->p_full[i], 128);
+            mbar_init(&ctl->p_full[i][0], 128);
+            mbar_init(&ctl->p_full[i][1], 128);
+            mbar_init(&ctl->o_full[i], 1);
+            mbar_init(&ctl->o_empty[i], 128);
         }
         for (int i = 0; i < 4; ++i) {
-            mbar_init(&ctl->k_full[i], T::kInt8 ? T::CW : 1);
-            mbar_init(&ctl->v_full[i], T::kInt8 ? T::CW : 1);
+            mbar_init(&ctl->k_full[i], T::kInt8 ? 4 : 1);
+            mbar_init(&ctl->v_full[i], T::kInt8 ? 4 : 1);
             mbar_init(&ctl->k_empty[i], 1);
             mbar_init(&ctl->v_empty[i], 1);
             mbar_init(&ctl->v_land[i], 1);
             mbar_init(&ctl->raw_full[i], 1);
-            mbar_init(&ctl->raw_empty[i], T::kInt8 ? T::CW : 1);
+            mbar_init(&ctl->raw_empty[i], T::kInt8 ? 4 : 1);
             mbar_init(&ctl->scl_full[i], 1);
             mbar_init(&ctl->scl_empty[i], shared ? 8 : 4);
         }
@@ -312,7 +384,8 @@ __global__ void __launch_bounds__(Tile<TV, TC, HD>::kThreads, 1)
     const uint32_t tmem = ctl->tmem;
 
     if (warp < 8) {
-        if constexpr (NP == 3) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(T::kSoftRegs));
+        if constexpr (NP == 3 && T::kSoftRegs > T::kLaunchRegs) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(T::kSoftRegs));
+        if constexpr (NP == 3 && T::kSoftRegs < T::kLaunchRegs) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(T::kSoftRegs));
         // ---- Q into its planes, then this stream's softmax ----
         const int s = warp >> 2;
         {
@@ -371,30 +444,6 @@ __global__ void __launch_bounds__(Tile<TV, TC, HD>::kThreads, 1)
         const float c = a.c;
         float m = -INFINITY;   // in units of log2
         float2 l2[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
-        // FP32 values: each tile's product starts from zero and is added to
-        // O here.  The tensor cores cut their sums instead of rounding them,
-        // and over a long row that adds up (4e-6 of the result at 2,000 keys).
-        float o[NP == 3 ? HD : 1];
-        if constexpr (NP == 3)
-#pragma unroll
-            for (int d = 0; d < HD; ++d) o[d] = 0.0f;
-        auto gather = [&]() {
-            if constexpr (NP == 3) {
-#pragma unroll
-                for (int d = 0; d < HD; d += CH) {
-                    uint32_t x[CH];
-                    tmem_ld(to + d, x);
-                    wait_ld();
-#pragma unroll
-                    for (int e = 0; e < CH; e += 2) {
-                        const float2 w = add2(make_float2(o[d + e], o[d + e + 1]),
-                                              make_float2(__uint_as_float(x[e]), __uint_as_float(x[e + 1])));
-                        o[d + e] = w.x;
-                        o[d + e + 1] = w.y;
-                    }
-                }
-            }
-        };
         bool ok = true;
 #pragma unroll 1
         for (int n = 0; n < n_steps; ++n) {
@@ -436,55 +485,57 @@ __global__ void __launch_bounds__(Tile<TV, TC, HD>::kThreads, 1)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) q[e] = __uint_as_float(x[e]);
 #pragma unroll
-                for (int e = 4; e < CH; ++e) q[e & 3] = fmaxf(q[e & 3], __uint_as_float(x[e]));
-                return fmaxf(fmaxf(q[0], q[1]), fmaxf(q[2], q[3]));
+                for (int e = 4; e < CH; e += 8)
+#pragma unroll
+                    for (int y = 0; y < 4; ++y)
+                        q[y] = max3(q[y], __uint_as_float(x[e + y]), __uint_as_float(x[(e + 4 + y) % CH]));
+                return max3(max3(q[0], q[1], q[2]), q[3], q[3]);
             };
             float bm = -INFINITY;
             uint32_t hold[T::kHold ? KT / CH : 1][CH];
             if constexpr (T::kHold) {
 #pragma unroll
-                for (int ch = 0; ch < KT / CH; ++ch) tmem_ld(ts + ch * CH, hold[ch]);
+                for (int ch = 0; ch < KT / CH; ++ch) tmem_ld32(ts + ch * CH, hold[ch]);
                 wait_ld();
             }
 #pragma unroll
             for (int ch = 0; ch < KT / CH; ++ch) {
                 uint32_t(&x)[CH] = hold[T::kHold ? ch : 0];
                 if constexpr (!T::kHold) {
-                    tmem_ld(ts + ch * CH, x);
+                    tmem_ld32(ts + ch * CH, x);
                     wait_ld();
                 }
                 finish(x, ch);
-                bm = fmaxf(bm, largest(x));
+                bm = max3(bm, largest(x), bm);
             }
             bm *= c;
-            if (n > 0) gather();
+            // A NaN among the visible scores is the row's result.
+            if (bm != bm) l2[0].x = bm;
             if (__any_sync(0xffffffffu, bm > m + 8.0f)) {
                 const float mn = fmaxf(m, bm), f = m == mn ? 1.0f : ex2(m - mn);
                 m = mn;
 #pragma unroll
                 for (int e = 0; e < 2; ++e) l2[e] = mul2(l2[e], make_float2(f, f));
-                if constexpr (NP == 3) {
-#pragma unroll
-                    for (int d = 0; d < HD; ++d) o[d] *= f;
-                } else if (n > 0) {
+                if (NP == 1 && n > 0) {
 #pragma unroll 1
-                    for (int d = 0; d < HD; d += 32) {
-                        uint32_t x[32];
-                        tmem_ld32(to + d, x);
+                    for (int d = 0; d < HD; d += 16) {
+                        uint32_t x[16];
+                        tmem_ld16(to + d, x);
                         wait_ld();
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * f);
-                        tmem_st32(to + d, x);
+                        for (int e = 0; e < 16; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * f);
+                        tmem_st16(to + d, x);
                     }
                 }
             }
+            if constexpr (NP == 3) s_max[(s * 2 + (n & 1)) * 128 + r_in] = m;
             const float base = m == -INFINITY ? 0.0f : m;
             const float2 c2 = make_float2(c, c), b2 = make_float2(-base, -base);
 #pragma unroll
             for (int ch = 0; ch < KT / CH; ++ch) {
                 uint32_t(&x)[CH] = hold[T::kHold ? ch : 0];
                 if constexpr (!T::kHold) {
-                    tmem_ld(ts + ch * CH, x);
+                    tmem_ld32(ts + ch * CH, x);
                     wait_ld();
                     finish(x, ch);
                 }
@@ -492,8 +543,15 @@ __global__ void __launch_bounds__(Tile<TV, TC, HD>::kThreads, 1)
 #pragma unroll
                 for (int e = 0; e < CH / 2; ++e) {
                     p[e] = fma2(make_float2(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1])), c2, b2);
-                    p[e].x = ex2(p[e].x);
-                    p[e].y = ex2(p[e].y);
+                    // One weight in four by polynomial on the FMA pipe: the
+                    // special-function unit alone (16 a cycle) would take
+                    // longer than the tensor cores.
+                    if (NP == 1 && (e & 3) == 3) {
+                        p[e] = ex2_poly(p[e]);
+                    } else {
+                        p[e].x = ex2(p[e].x);
+                        p[e].y = ex2(p[e].y);
+                    }
                     l2[e & 1] = add2(l2[e & 1], p[e]);
                 }
                 if constexpr (T::kInt8) {
@@ -519,124 +577,121 @@ __global__ void __launch_bounds__(Tile<TV, TC, HD>::kThreads, 1)
 #pragma unroll
                     for (int e = 0; e < CH / 2; ++e) {
                         w[e] = pack_bf16(p[e].x, p[e].y);
-                        if (pl + 1 < NP) {
-                            p[e].x -= bf16_lo(w[e]);
-                            p[e].y -= bf16_hi(w[e]);
-                        }
+                        if (pl + 1 < NP) p[e] = add2(p[e], make_float2(-bf16_lo(w[e]), -bf16_hi(w[e])));
                     }
-                    tmem_st(ts + T::plane_col(pl) + ch * (CH / 2), w);
+                    tmem_st16(ts + T::plane_col(pl) + ch * (CH / 2), w);
+                }
+                if (ch == KT / CH / 2 - 1 || ch == KT / CH - 1) {
+                    wait_st();
+                    fence_before();
+                    mbar_arrive(&ctl->p_full[s][ch == KT / CH - 1]);
                 }
             }
-            wait_st();
-            fence_before();
-            mbar_arrive(&ctl->p_full[s]);
             if constexpr (T::kInt8) {
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&ctl->scl_empty[i % D]);
             }
         }
         const float2 lsum = add2(l2[0], l2[1]);
-        float l = lsum.x + lsum.y;
+        const float l = lsum.x + lsum.y;
         const bool fin = __all_sync(0xffffffffu, wait_issued(&ctl->done, 0u) && ok && !ctl->abort_);
         fence_after();
-        if (n_steps > 0) gather();
-        // ---- the rows' results ----
-        constexpr int EC = NP == 3 && HD == 128 ? 16 : 32, kUnroll = NP == 3 ? HD / EC : 1;
-        auto result = [&](int d, uint32_t (&x)[EC]) {
-            if constexpr (NP == 3) {
-#pragma unroll
-                for (int e = 0; e < EC; ++e) x[e] = __float_as_uint(o[d + e]);
-            } else {
-                tmem_ld(to + d, x);
-                wait_ld();
-            }
-        };
-        bool write = r < it.rows;
-        float f0 = 1.0f;
-        float *s_o = (float *)s_k;  // stream 1's part where both had the same rows
-        constexpr int OS = HD + 4;
-        float *s_ml = s_o + 128 * OS;
-        if (!shared && nk > 1) {
-            if (s == 1) {
-                s_ml[r_in] = m;
-                s_ml[128 + r_in] = l;
-#pragma unroll(kUnroll)
-                for (int d = 0; d < HD; d += EC) {
-                    uint32_t x[EC];
-                    result(d, x);
-#pragma unroll
-                    for (int e = 0; e < EC; e += 4)
-                        *(uint4 *)(s_o + r_in * OS + d + e) = make_uint4(x[e], x[e + 1], x[e + 2], x[e + 3]);
-                }
-            }
-            asm volatile("bar.sync 1, 256;" ::: "memory");
-        }
-        float f1 = 0.0f;
+        // Every copy and product has ended: stream 1's sums (and, where O is
+        // not gathered, its O) for whoever writes the rows both streams had.
+        float *s_o = (float *)s_k, *s_ml = s_o + 128 * (HD + 4);  // [stream][maximum, sum][row]
         if (!shared) {
-            write = write && s == 0;
-            if (nk > 1 && s == 0) {
-                const float m1 = s_ml[r_in], l1 = s_ml[128 + r_in], mn = fmaxf(m, m1), base = mn == -INFINITY ? 0.0f : mn;
-                f0 = m == base ? 1.0f : ex2(m - base);
-                f1 = m1 == base ? 1.0f : ex2(m1 - base);
-                l = f0 * l + f1 * l1;
-                m = mn;
+            s_ml[s * 256 + r_in] = m;
+            s_ml[s * 256 + 128 + r_in] = fin ? l : __uint_as_float(0x7fffffffu);
+            if (NP == 1 && s == 1 && nk > 1) {
+#pragma unroll 1
+                for (int d = 0; d < HD; d += 32) {
+                    uint32_t x[32];
+                    tmem_ld32(to + d, x);
+                    wait_ld();
+#pragma unroll
+                    for (int e = 0; e < 32; e += 4)
+                        *(uint4 *)(s_o + r_in * (HD + 4) + d + e) = make_uint4(x[e], x[e + 1], x[e + 2], x[e + 3]);
+                }
             }
+            asm volatile("bar.sync 1, %0;" ::"n"(NP == 3 ? 384 : 256) : "memory");
         }
-        if (shared || s == 0) {
-            const int row = it.row0 + r;
-            const size_t at = ((size_t)(sq.tok0 + row / a.G) * a.H + it.kvh * a.G + row % a.G) * HD;
-            const bool vec = ((uintptr_t)a.y & 15) == 0;
-            const float nan = __uint_as_float(0x7fffffffu);
+        if (NP == 1 && (shared || s == 0)) {
+            Join j = {m, l, 1.0f, 0.0f};
+            if (!shared && nk > 1) j = join(m, l, s_ml[256 + r_in], s_ml[384 + r_in]);
             bool bad = false;
-            const float inv = __fdiv_rn(1.0f, l);
-#pragma unroll(kUnroll)
-            for (int d = 0; d < HD; d += EC) {
-                uint32_t x[EC];
-                result(d, x);
-                float v[EC];
+#pragma unroll 1
+            for (int d = 0; d < HD; d += 32) {
+                uint32_t x[32];
+                tmem_ld32(to + d, x);
+                wait_ld();
+                float v[32];
 #pragma unroll
-                for (int e = 0; e < EC; ++e) {
-                    v[e] = __uint_as_float(x[e]) * f0;
-                    if (f1 != 0.0f) v[e] = fmaf(f1, s_o[r_in * OS + d + e], v[e]);
+                for (int e = 0; e < 32; ++e) {
+                    v[e] = __uint_as_float(x[e]) * j.f0;
+                    if (j.f1 != 0.0f) v[e] = fmaf(j.f1, s_o[r_in * (HD + 4) + d + e], v[e]);
                     bad |= !isfinite(v[e]);
-                    if (!fin) v[e] = nan;
-                    if (it.slot < 0) v[e] *= inv;
                 }
-                if (!write) {
-                } else if (it.slot >= 0) {
-                    float *w = a.ws + it.slot + (size_t)r * HD + d;
+                if (r < it.rows) put_row<TV, HD>(a, it, sq, r, d, v, j.m, fin ? j.l : __uint_as_float(0x7fffffffu));
+            }
+            if (bad && fin && r < it.rows) ctl->bad[r] = 1;
+        }
+    } else if (NP == 3 && warp >= T::kGather && warp < T::kGather + 4) {
+        // O of both streams, in registers.  Each tile's product starts from
+        // zero and is added here: the tensor cores cut their sums instead of
+        // rounding them, and over a long row that adds up (5e-6 of the result
+        // at 3,000 keys).
+        if constexpr (NP == 3) {
+            asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(T::kGatherRegs));
+            const int r = (warp & 3) * 32 + lane;
+            const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+            float2 o[HD / 2];
 #pragma unroll
-                    for (int e = 0; e < EC; e += 2) *(float2 *)(w + e) = make_float2(v[e], v[e + 1]);
-                } else if constexpr (NP == 3) {
-                    float *y = (float *)a.y + at + d;
-                    if (vec) {
+            for (int d = 0; d < HD / 2; ++d) o[d] = make_float2(0.0f, 0.0f);
+            float m = -INFINITY;
+            bool ok = true;
+#pragma unroll 1
+            for (int t = 0; t < steps; ++t) {
+                const int s = t & 1;
+                if (!(ok = __all_sync(0xffffffffu, wait(&ctl->o_full[s], (uint32_t)((t >> 1) & 1), ctl)))) break;
+                fence_after();
+                const float mt = s_max[(s * 2 + ((t >> 1) & 1)) * 128 + r];
+                if (__any_sync(0xffffffffu, mt > m)) {
+                    const float mn = fmaxf(m, mt), f = m == mn ? 1.0f : ex2(m - mn);
+                    m = mn;
 #pragma unroll
-                        for (int e = 0; e < EC; e += 4) *(float4 *)(y + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < EC; ++e) y[e] = v[e];
-                    }
-                } else {
-                    uint16_t *y = (uint16_t *)a.y + at + d;
-                    if (vec) {
-#pragma unroll
-                        for (int e = 0; e < EC; e += 8)
-                            *(uint4 *)(y + e) = make_uint4(pack_bf16(v[e], v[e + 1]), pack_bf16(v[e + 2], v[e + 3]),
-                                                           pack_bf16(v[e + 4], v[e + 5]), pack_bf16(v[e + 6], v[e + 7]));
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < EC; ++e) y[e] = bf16_bits(v[e]);
-                    }
+                    for (int d = 0; d < HD / 2; ++d) o[d] = mul2(o[d], make_float2(f, f));
                 }
+                const float w = mt == m ? 1.0f : ex2(mt - m);
+#pragma unroll
+                for (int d = 0; d < HD; d += 16) {
+                    uint32_t x[16];
+                    tmem_ld16(tmem + s * 256 + 128 + lanes + d, x);
+                    wait_ld();
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        o[d / 2 + e] = fma2(make_float2(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1])),
+                                            make_float2(w, w), o[d / 2 + e]);
+                }
+                fence_before();
+                mbar_arrive(&ctl->o_empty[s]);
             }
-            if (write && it.slot >= 0) {
-                a.ws[it.slot + (size_t)it.rows * HD + r] = fin ? m : nan;
-                a.ws[it.slot + (size_t)it.rows * (HD + 1) + r] = l;
+            const bool fin = __all_sync(0xffffffffu, ok);
+            asm volatile("bar.sync 1, 384;" ::: "memory");
+            const float *s_ml = (const float *)s_k + 128 * (HD + 4);
+            const Join j = join(s_ml[r], s_ml[128 + r], s_ml[256 + r], s_ml[384 + r]);
+            bool bad = false;
+#pragma unroll
+            for (int d = 0; d < HD; d += 32) {
+                float v[32];
+#pragma unroll
+                for (int e = 0; e < 32; e += 2) {
+                    v[e] = o[(d + e) / 2].x;
+                    v[e + 1] = o[(d + e) / 2].y;
+                    bad |= !isfinite(v[e]) | !isfinite(v[e + 1]);
+                }
+                if (r < it.rows) put_row<TV, HD>(a, it, sq, r, d, v, j.m, fin ? j.l : __uint_as_float(0x7fffffffu));
             }
-            // A result that is not finite may be a hidden value's doing (a key
-            // that only some of the rows see) or the planes' (an infinity
-            // times planes of both signs): such rows are done again below.
-            if (write && bad && fin) ctl->bad[r] = 1;
+            if (bad && fin && r < it.rows) ctl->bad[r] = 1;
         }
     } else {
         if constexpr (NP == 3) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(T::kOtherRegs));
@@ -644,26 +699,39 @@ __global__ void __launch_bounds__(Tile<TV, TC, HD>::kThreads, 1)
             // Producer: BF16 boxes straight into the operand stages (one lane a
             // page), INT8 pages raw into the pieces.
             if constexpr (!T::kInt8) {
-                int x = 0;
+                // A tile's page is looked up one tile ahead: the table's latency
+                // would otherwise come on top of the copy's.
+                auto page = [&](int x) {
+                    bool is_k;
+                    int i;
+                    nth(x, nk, is_k, i);
+                    const int pj = key0(i) / kPage + lane;
+                    return x < 2 * nk && lane < kPages && page_seen(pj) ? table[pj] : -1;
+                };
+                const uint32_t leader = elect_one();
+                int x = 0, next = page(0);
 #pragma unroll 1
                 for (; x < 2 * nk; ++x) {
                     bool is_k;
                     int i;
                     nth(x, nk, is_k, i);
-                    const int st = i % NS;
+                    const int st = i % NS, pid = next;
+                    next = page(x + 1);
                     if (i >= NS && !__all_sync(0xffffffffu, wait(is_k ? &ctl->k_empty[st] : &ctl->v_empty[st], (uint32_t)((i / NS - 1) & 1), ctl)))
                         break;
-                    const int pj = key0(i) / kPage + lane;
-                    const bool on = lane < kPages && page_seen(pj);
+                    const bool on = pid >= 0;
                     const int pages = __popc(__ballot_sync(0xffffffffu, on));
                     uint64_t *bar = is_k ? &ctl->k_full[st] : &ctl->v_land[st];
                     if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)pages * (kPage * HD * 2));
                     __syncwarp();
-                    if (on) {
-                        const int row = (table[pj] * a.KV + it.kvh) * kPage;
-                        uint8_t *dst = (is_k ? s_k : s_v) + (size_t)st * T::kTileBytes + lane * (kPage * 128);
+                    const uint32_t dst = smem_addr((is_k ? s_k : s_v) + (size_t)st * T::kTileBytes);
+                    const CUtensorMap *map = is_k ? &mk : &mv;
 #pragma unroll
-                        for (int p = 0; p < PN; ++p) tma_2d(dst + (size_t)p * KT * 128, is_k ? &mk : &mv, p * 64, row, bar);
+                    for (int g = 0; g < kPages; ++g) {
+                        const int id = __shfl_sync(0xffffffffu, pid, g), row = (id * a.KV + it.kvh) * kPage;
+#pragma unroll
+                        for (int p = 0; p < PN; ++p)
+                            if (id >= 0) tma_2d(dst + p * (KT * 128) + g * (kPage * 128), map, p * 64, row, smem_addr(bar), leader);
                     }
                     __syncwarp();
                 }
@@ -686,22 +754,29 @@ __global__ void __launch_bounds__(Tile<TV, TC, HD>::kThreads, 1)
                 }
             } else {
                 constexpr int per = KT / 64;
-                int z = 0;  // pieces issued
+                auto page = [&](int z) {
+                    bool is_k;
+                    int i;
+                    nth(z / per, nk, is_k, i);
+                    const int pj = key0(i) / kPage + z % per * 4 + lane;
+                    return z < 2 * nk * per && lane < 4 && page_seen(pj) ? table[pj] : -1;
+                };
+                int z = 0, next = page(0);  // pieces issued
 #pragma unroll 1
                 for (; z < 2 * nk * per; ++z) {
                     bool is_k;
                     int i;
                     nth(z / per, nk, is_k, i);
-                    const int st = z % RS;
+                    const int st = z % RS, pid = next;
+                    next = page(z + 1);
                     if (z >= RS && !__all_sync(0xffffffffu, wait(&ctl->raw_empty[st], (uint32_t)((z / RS - 1) & 1), ctl))) break;
-                    const int pj = key0(i) / kPage + z % per * 4 + lane;
-                    const bool on = lane < 4 && page_seen(pj);
+                    const bool on = pid >= 0;
                     const int pages = __popc(__ballot_sync(0xffffffffu, on));
                     if (lane == 0) mbar_arrive_expect_tx(&ctl->raw_full[st], (uint32_t)pages * (kPage * HD));
                     __syncwarp();
                     if (on)
                         bulk_copy_g2s(s_raw + (size_t)st * T::kPiece + lane * (kPage * HD),
-                                      (is_k ? a.k : a.v) + ((size_t)table[pj] * a.KV + it.kvh) * (kPage * HD), kPage * HD,
+                                      (is_k ? a.k : a.v) + ((size_t)pid * a.KV + it.kvh) * (kPage * HD), kPage * HD,
                                       &ctl->raw_full[st]);
                     __syncwarp();
                 }
@@ -745,16 +820,24 @@ __global__ void __launch_bounds__(Tile<TV, TC, HD>::kThreads, 1)
                 // long before the weights: looked at first.
                 if ((!two || s == 0) && !await(&ctl->v_full[st], (uint32_t)((i / NS) & 1))) break;
                 if (t + 2 < total && !k_ready(t + 2)) break;
-                if (!await(&ctl->p_full[s], (uint32_t)((t >> 1) & 1))) break;
-                fence_after();
+                if (NP == 3 && t > 1 && !await(&ctl->o_empty[s], (uint32_t)(((t >> 1) - 1) & 1))) break;
                 const uint32_t v = v_at + st * T::kTileBytes;
+                // The first half of the keys while the second's weights are
+                // still being computed.
 #pragma unroll
-                for (int pl = NP - 1; pl >= 0; --pl)
+                for (int h = 0; h < 2; ++h) {
+                    if (!(ok = await(&ctl->p_full[s][h], (uint32_t)((t >> 1) & 1)))) break;
+                    fence_after();
 #pragma unroll
-                    for (int kb = 0; kb < KT / 16; ++kb)
-                        mma_ts(tm + s * 256 + 128, tm + s * 256 + T::plane_col(pl) + kb * 8,
-                               desc_mn(v + kb * 2048, KT * 128), io, (NP == 1 && t > 1) || pl != NP - 1 || kb != 0,
-                               leader);
+                    for (int pl = NP - 1; pl >= 0; --pl)
+#pragma unroll
+                        for (int kb = h * (KT / 32); kb < (h + 1) * (KT / 32); ++kb)
+                            mma_ts(tm + s * 256 + 128, tm + s * 256 + T::plane_col(pl) + kb * 8,
+                                   desc_mn(v + kb * 2048, KT * 128), io,
+                                   (NP == 1 && t > 1) || h || pl != NP - 1 || kb != 0, leader);
+                }
+                if (!ok) break;
+                if (NP == 3) commit(&ctl->o_full[s], leader);
                 if (!two || s == 1) commit(&ctl->v_empty[st], leader);
                 if (t + 2 < total) scores(t + 2);
             }
@@ -782,18 +865,23 @@ __global__ void __launch_bounds__(Tile<TV, TC, HD>::kThreads, 1)
                 }
             } else {
                 // The scales of every tile's keys, a 64-byte copy a page and pool.
-                int i = 0;
+                auto page = [&](int i) {
+                    if (i >= nk) return -1;
+                    const int pj = key0(i) / kPage + lane;
+                    return lane < kPages && page_seen(pj) ? table[pj] : -1;
+                };
+                int i = 0, next = page(0);
 #pragma unroll 1
                 for (; i < nk; ++i) {
-                    const int st = i % D;
+                    const int st = i % D, pid = next;
+                    next = page(i + 1);
                     if (i >= D && !__all_sync(0xffffffffu, wait(&ctl->scl_empty[st], (uint32_t)((i / D - 1) & 1), ctl))) break;
-                    const int pj = key0(i) / kPage + lane;
-                    const bool on = lane < kPages && page_seen(pj);
+                    const bool on = pid >= 0;
                     const int pages = __popc(__ballot_sync(0xffffffffu, on));
                     if (lane == 0) mbar_arrive_expect_tx(&ctl->scl_full[st], (uint32_t)pages * 128u);
                     __syncwarp();
                     if (on) {
-                        const size_t at = ((size_t)table[pj] * a.KV + it.kvh) * kPage;
+                        const size_t at = ((size_t)pid * a.KV + it.kvh) * kPage;
                         bulk_copy_g2s(s_scl + (st * 2) * KT + lane * kPage, a.ks + at, 64, &ctl->scl_full[st]);
                         bulk_copy_g2s(s_scl + (st * 2 + 1) * KT + lane * kPage, a.vs + at, 64, &ctl->scl_full[st]);
                     }
@@ -801,11 +889,11 @@ __global__ void __launch_bounds__(Tile<TV, TC, HD>::kThreads, 1)
                 }
                 for (int y = i > D ? i - D : 0; y < i; ++y) wait_issued(&ctl->scl_full[y % D], (uint32_t)((y / D) & 1));
             }
-        } else if (warp >= 12) {
+        } else if (warp >= T::kConvert) {
             if constexpr (T::kInt8) {
                 // INT8 -> bf16 (exact), 64 keys a piece, into the operand layout.
-                constexpr int per = KT / 64, units = T::kPiece / 16 / (T::CW * 32);
-                const int ct = threadIdx.x - 384;
+                constexpr int per = KT / 64, units = T::kPiece / 16 / 128;
+                const int ct = threadIdx.x - T::kConvert * 32;
                 bool ok = true;
 #pragma unroll 1
                 for (int z = 0; ok && z < 2 * nk * per; ++z) {
@@ -821,12 +909,12 @@ __global__ void __launch_bounds__(Tile<TV, TC, HD>::kThreads, 1)
                     uint8_t *dst = (is_k ? s_k : s_v) + (size_t)st * T::kTileBytes + half * (64 * 128);
                     uint4 w[units];
 #pragma unroll
-                    for (int u = 0; u < units; ++u) w[u] = *(const uint4 *)(src + (u * T::CW * 32 + ct) * 16);
+                    for (int u = 0; u < units; ++u) w[u] = *(const uint4 *)(src + (u * 128 + ct) * 16);
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&ctl->raw_empty[rs]);
 #pragma unroll
                     for (int u = 0; u < units; ++u) {
-                        const int e = u * T::CW * 32 + ct, key = e / (HD / 16), q = e % (HD / 16);
+                        const int e = u * 128 + ct, key = e / (HD / 16), q = e % (HD / 16);
                         uint4 o0, o1;
                         o0.x = s8x2_to_bf16x2(__byte_perm(w[u].x, 0u, 0x4140u));
                         o0.y = s8x2_to_bf16x2(__byte_perm(w[u].x, 0u, 0x4342u));
@@ -850,6 +938,7 @@ __global__ void __launch_bounds__(Tile<TV, TC, HD>::kThreads, 1)
         }
     }
     fence_before();
+    __syncthreads();
     const int redo = __syncthreads_or(warp < 8 && ctl->bad[threadIdx.x & 255]);
     fence_after();
     if (warp == 11)
