@@ -53,15 +53,17 @@ struct Tile {
     static constexpr int kPiece = 64 * HD;
     static constexpr int RS = kInt8 ? (HD == 128 ? 3 : 4) : 0;
     static constexpr int D = kInt8 ? 4 : 0;
-    // Warps: 8 softmax, producer, MMA issuer, V fixer or scale producer, TMEM;
+    // Warps: 8 softmax, K producer, MMA issuer, scale producer, TMEM and V producer;
     // 4 that gather O (FP32 values); 4 INT8 converters.
     static constexpr int kGather = 12, kConvert = NP == 3 ? 16 : 12;
     static constexpr int kThreads = 384 + (NP == 3 ? 128 : 0) + (kInt8 ? 128 : 0);
-    // O is in registers where it is gathered: a split of the launch's
-    // registers (FP32 values only).
+    // The launch's registers, split among the roles: the softmax holds its
+    // scores (BF16 caches) and the gathering warps O.
     static constexpr int kLaunchRegs = 65536 / kThreads / 8 * 8;
-    static constexpr int kSoftRegs = kInt8 ? 112 : 120, kGatherRegs = kInt8 ? 168 : 176, kOtherRegs = kInt8 ? 40 : 88;
-    static_assert(NP == 1 || 256 * kSoftRegs + 128 * kGatherRegs + (kThreads - 384) * kOtherRegs <= kThreads * kLaunchRegs,
+    static constexpr int kSoftRegs = NP == 3 ? (kInt8 ? 112 : 120) : kInt8 ? 168 : 216, kGatherRegs = kInt8 ? 168 : 176,
+                         kOtherRegs = NP == 3 ? (kInt8 ? 40 : 88) : kInt8 ? 88 : 72;
+    static_assert(256 * kSoftRegs + (NP == 3 ? 128 * kGatherRegs : 0) + (kThreads - (NP == 3 ? 384 : 256)) * kOtherRegs <=
+                      kThreads * kLaunchRegs,
                   "register split");
     // Columns of a stream: scores from 0 (KT of them), plane 0 of the weights
     // over the scores that were read already, planes 1 and 2 behind them
@@ -80,7 +82,7 @@ struct Tile {
 struct Ctl {
     uint64_t q_full, done;
     uint64_t s_full[2], p_full[2][2], o_full[2], o_empty[2];
-    uint64_t k_full[4], k_empty[4], v_land[4], v_full[4], v_empty[4];
+    uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4];
     uint64_t raw_full[4], raw_empty[4], scl_full[4], scl_empty[4];
     uint32_t tmem;
     int abort_;
@@ -154,6 +156,16 @@ __device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap *m, int x
         : "memory");
 }
 
+// All panels of a page at once (V).
+__device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap *m, int y, uint32_t bar, uint32_t leader) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %4, 0;\n\t"
+        "@q cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%5, %2, %5}], [%3];"
+        "\n\t}" ::"r"(dst),
+        "l"((uint64_t)m), "r"(y), "r"(bar), "r"(leader), "r"(0)
+        : "memory");
+}
+
 #define QB_R8(v, o) "=r"(v[o]), "=r"(v[o + 1]), "=r"(v[o + 2]), "=r"(v[o + 3]), "=r"(v[o + 4]), "=r"(v[o + 5]), "=r"(v[o + 6]), "=r"(v[o + 7])
 // 32 columns of this warp's 32 lanes; valid after wait_ld.
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&v)[32]) {
@@ -185,7 +197,7 @@ __device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.
 
 // Shared-memory operand descriptors, 128-byte swizzle.  K-major: 8-row
 // groups 1024 bytes apart.  MN-major: 64-element panels `panel` bytes apart,
-// groups of 8 reduction rows 1024 bytes apart.
+// groups of 8 reduction rows 1024 bytes apart (16 rows, a page, a step).
 __device__ __forceinline__ uint64_t desc_k(uint32_t saddr) {
     return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) |
            ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
@@ -363,7 +375,6 @@ __global__ void __launch_bounds__(Tile<TV, TC, HD>::kThreads, 1)
             mbar_init(&ctl->v_full[i], T::kInt8 ? 4 : 1);
             mbar_init(&ctl->k_empty[i], 1);
             mbar_init(&ctl->v_empty[i], 1);
-            mbar_init(&ctl->v_land[i], 1);
             mbar_init(&ctl->raw_full[i], 1);
             mbar_init(&ctl->raw_empty[i], T::kInt8 ? 4 : 1);
             mbar_init(&ctl->scl_full[i], 1);
@@ -383,9 +394,52 @@ __global__ void __launch_bounds__(Tile<TV, TC, HD>::kThreads, 1)
     fence_after();
     const uint32_t tmem = ctl->tmem;
 
+    // Loads every tile of one operand (BF16): a box a page (V) or a page's
+    // panel (K).  A copy takes its warp about 110 cycles to issue, so K and V
+    // have a warp each.  (K by two warps was slower: 421 against 402 us on
+    // 4,096 tokens behind 4,096 at the 7B shape.)
+    auto produce = [&](bool is_k) {
+        uint64_t *full = is_k ? ctl->k_full : ctl->v_full, *empty = is_k ? ctl->k_empty : ctl->v_empty;
+        const uint32_t base = smem_addr(is_k ? s_k : s_v), leader = elect_one();
+        // A tile's pages (as pool rows) are looked up one tile ahead: the
+        // table's latency would otherwise come on top of the copy's.
+        auto page = [&](int i) {
+            if (i >= nk) return -1;
+            const int pj = key0(i) / kPage + lane;
+            return lane < kPages && page_seen(pj) ? (table[pj] * a.KV + it.kvh) * kPage : -1;
+        };
+        int i = 0, next = page(0);
+#pragma unroll 1
+        for (; i < nk; ++i) {
+            const int st = i % NS;
+            int row[kPages];
+#pragma unroll
+            for (int g = 0; g < kPages; ++g) row[g] = __shfl_sync(0xffffffffu, next, g);
+            const int pages = __popc(__ballot_sync(0xffffffffu, next >= 0));
+            next = page(i + 1);
+            if (i >= NS && !__all_sync(0xffffffffu, wait(empty + st, (uint32_t)((i / NS - 1) & 1), ctl))) break;
+            if (lane == 0) mbar_arrive_expect_tx(full + st, (uint32_t)pages * (kPage * HD * 2));
+            __syncwarp();
+            const uint32_t dst = base + st * T::kTileBytes, bar = smem_addr(full + st);
+#pragma unroll
+            for (int g = 0; g < kPages; ++g) {
+                const uint32_t go = row[g] >= 0 ? leader : 0u;
+                if (is_k) {
+#pragma unroll
+                    for (int p = 0; p < PN; ++p)
+                        tma_2d(dst + p * (KT * 128) + g * (kPage * 128), &mk, p * 64, row[g], bar, go);
+                } else {
+                    tma_3d(dst + g * (PN * kPage * 128), &mv, row[g], bar, go);
+                }
+            }
+            __syncwarp();
+        }
+        // Every copy issued must land before the CTA can exit.
+        for (int y = i > NS ? i - NS : 0; y < i; ++y) wait_issued(full + y % NS, (uint32_t)((y / NS) & 1));
+    };
     if (warp < 8) {
-        if constexpr (NP == 3 && T::kSoftRegs > T::kLaunchRegs) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(T::kSoftRegs));
-        if constexpr (NP == 3 && T::kSoftRegs < T::kLaunchRegs) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(T::kSoftRegs));
+        if constexpr (T::kSoftRegs > T::kLaunchRegs) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(T::kSoftRegs));
+        if constexpr (T::kSoftRegs < T::kLaunchRegs) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(T::kSoftRegs));
         // ---- Q into its planes, then this stream's softmax ----
         const int s = warp >> 2;
         {
@@ -576,8 +630,17 @@ __global__ void __launch_bounds__(Tile<TV, TC, HD>::kThreads, 1)
                     uint32_t w[CH / 2];
 #pragma unroll
                     for (int e = 0; e < CH / 2; ++e) {
-                        w[e] = pack_bf16(p[e].x, p[e].y);
-                        if (pl + 1 < NP) p[e] = add2(p[e], make_float2(-bf16_lo(w[e]), -bf16_hi(w[e])));
+                        if constexpr (NP == 1) {
+                            w[e] = pack_bf16(p[e].x, p[e].y);
+                        } else {
+                            // Planes by truncation: 8 bits of the significand
+                            // each, exact in three.
+                            const uint32_t x0 = __float_as_uint(p[e].x), x1 = __float_as_uint(p[e].y);
+                            w[e] = __byte_perm(x0, x1, 0x7632u);
+                            if (pl + 1 < NP)
+                                p[e] = fma2(make_float2(__uint_as_float(x0 & 0xffff0000u), __uint_as_float(x1 & 0xffff0000u)),
+                                            make_float2(-1.0f, -1.0f), p[e]);
+                        }
                     }
                     tmem_st16(ts + T::plane_col(pl) + ch * (CH / 2), w);
                 }
@@ -694,64 +757,12 @@ __global__ void __launch_bounds__(Tile<TV, TC, HD>::kThreads, 1)
             if (bad && fin && r < it.rows) ctl->bad[r] = 1;
         }
     } else {
-        if constexpr (NP == 3) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(T::kOtherRegs));
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(T::kOtherRegs));
         if (warp == 8) {
-            // Producer: BF16 boxes straight into the operand stages (one lane a
-            // page), INT8 pages raw into the pieces.
+            // Producers: BF16 boxes straight into the operand stages (K by this
+            // warp and warp 10, V by warp 11), INT8 pages raw into the pieces.
             if constexpr (!T::kInt8) {
-                // A tile's page is looked up one tile ahead: the table's latency
-                // would otherwise come on top of the copy's.
-                auto page = [&](int x) {
-                    bool is_k;
-                    int i;
-                    nth(x, nk, is_k, i);
-                    const int pj = key0(i) / kPage + lane;
-                    return x < 2 * nk && lane < kPages && page_seen(pj) ? table[pj] : -1;
-                };
-                const uint32_t leader = elect_one();
-                int x = 0, next = page(0);
-#pragma unroll 1
-                for (; x < 2 * nk; ++x) {
-                    bool is_k;
-                    int i;
-                    nth(x, nk, is_k, i);
-                    const int st = i % NS, pid = next;
-                    next = page(x + 1);
-                    if (i >= NS && !__all_sync(0xffffffffu, wait(is_k ? &ctl->k_empty[st] : &ctl->v_empty[st], (uint32_t)((i / NS - 1) & 1), ctl)))
-                        break;
-                    const bool on = pid >= 0;
-                    const int pages = __popc(__ballot_sync(0xffffffffu, on));
-                    uint64_t *bar = is_k ? &ctl->k_full[st] : &ctl->v_land[st];
-                    if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)pages * (kPage * HD * 2));
-                    __syncwarp();
-                    const uint32_t dst = smem_addr((is_k ? s_k : s_v) + (size_t)st * T::kTileBytes);
-                    const CUtensorMap *map = is_k ? &mk : &mv;
-#pragma unroll
-                    for (int g = 0; g < kPages; ++g) {
-                        const int id = __shfl_sync(0xffffffffu, pid, g), row = (id * a.KV + it.kvh) * kPage;
-#pragma unroll
-                        for (int p = 0; p < PN; ++p)
-                            if (id >= 0) tma_2d(dst + p * (KT * 128) + g * (kPage * 128), map, p * 64, row, smem_addr(bar), leader);
-                    }
-                    __syncwarp();
-                }
-                // Every copy issued must land before the CTA can exit.
-                for (int y = x - 1; y >= 0 && y >= x - 2 * NS - 1; --y) {
-                    bool is_k;
-                    int i;
-                    nth(y, nk, is_k, i);
-                    // Later phases of the stage cannot exist: only its last use is waited for.
-                    const int last = ([&] {
-                        for (int z = x - 1; z > y; --z) {
-                            bool k2;
-                            int i2;
-                            nth(z, nk, k2, i2);
-                            if (k2 == is_k && i2 % NS == i % NS) return false;
-                        }
-                        return true;
-                    })();
-                    if (last) wait_issued(is_k ? &ctl->k_full[i % NS] : &ctl->v_land[i % NS], (uint32_t)((i / NS) & 1));
-                }
+                produce(true);
             } else {
                 constexpr int per = KT / 64;
                 auto page = [&](int z) {
@@ -819,6 +830,22 @@ __global__ void __launch_bounds__(Tile<TV, TC, HD>::kThreads, 1)
                 // The tiles of these products and of the next scores are there
                 // long before the weights: looked at first.
                 if ((!two || s == 0) && !await(&ctl->v_full[st], (uint32_t)((i / NS) & 1))) break;
+                if (!T::kInt8 && (!two || s == 0)) {
+                    // V rows that no row sees may hold anything (0 * inf is
+                    // not 0; INT8 values are always finite).  Here and not in
+                    // a warp of its own: one more waiting warp cost 5 %.
+                    const int j0 = key0(i);
+                    if (j0 + KT > it.hi || (j0 < it.w0 && j0 + KT > a.sinks)) {
+                        // 16 bytes a lane, in the order they lie in: page,
+                        // panel, row, piece.
+                        uint4 *v = (uint4 *)(s_v + (size_t)st * T::kTileBytes);
+#pragma unroll 4
+                        for (int e = lane; e < KT * PN * 8; e += 32)
+                            if (none(j0 + e / (PN * kPage * 8) * kPage + e / 8 % kPage)) v[e] = make_uint4(0, 0, 0, 0);
+                        fence_proxy_async_smem();
+                        __syncwarp();
+                    }
+                }
                 if (t + 2 < total && !k_ready(t + 2)) break;
                 if (NP == 3 && t > 1 && !await(&ctl->o_empty[s], (uint32_t)(((t >> 1) - 1) & 1))) break;
                 const uint32_t v = v_at + st * T::kTileBytes;
@@ -833,7 +860,7 @@ __global__ void __launch_bounds__(Tile<TV, TC, HD>::kThreads, 1)
 #pragma unroll
                         for (int kb = h * (KT / 32); kb < (h + 1) * (KT / 32); ++kb)
                             mma_ts(tm + s * 256 + 128, tm + s * 256 + T::plane_col(pl) + kb * 8,
-                                   desc_mn(v + kb * 2048, KT * 128), io,
+                                   desc_mn(v + kb * (PN * 2048), 2048), io,
                                    (NP == 1 && t > 1) || h || pl != NP - 1 || kb != 0, leader);
                 }
                 if (!ok) break;
@@ -844,26 +871,7 @@ __global__ void __launch_bounds__(Tile<TV, TC, HD>::kThreads, 1)
             commit(&ctl->done, leader);
             __syncwarp();
         } else if (warp == 10) {
-            if constexpr (!T::kInt8) {
-                // V rows that no row sees may hold anything (0 * inf is not 0).
-#pragma unroll 1
-                for (int i = 0; i < nk; ++i) {
-                    const int st = i % NS, j0 = key0(i);
-                    if (!__all_sync(0xffffffffu, wait(&ctl->v_land[st], (uint32_t)((i / NS) & 1), ctl))) break;
-                    bool fix = false;
-                    for (int j = j0 + lane; j < j0 + KT; j += 32) fix |= none(j);
-                    if (__any_sync(0xffffffffu, fix)) {
-                        uint32_t *v = (uint32_t *)(s_v + (size_t)st * T::kTileBytes);
-                        for (int r = 0; r < KT; ++r)
-                            if (none(j0 + r))
-#pragma unroll
-                                for (int p = 0; p < PN; ++p) v[p * (KT * 32) + r * 32 + lane] = 0u;
-                        fence_proxy_async_smem();
-                        __syncwarp();
-                    }
-                    if (lane == 0) mbar_arrive(&ctl->v_full[st]);
-                }
-            } else {
+            if constexpr (T::kInt8) {
                 // The scales of every tile's keys, a 64-byte copy a page and pool.
                 auto page = [&](int i) {
                     if (i >= nk) return -1;
@@ -889,11 +897,18 @@ __global__ void __launch_bounds__(Tile<TV, TC, HD>::kThreads, 1)
                 }
                 for (int y = i > D ? i - D : 0; y < i; ++y) wait_issued(&ctl->scl_full[y % D], (uint32_t)((y / D) & 1));
             }
+        } else if (warp == 11) {
+            if constexpr (!T::kInt8) produce(false);
         } else if (warp >= T::kConvert) {
             if constexpr (T::kInt8) {
                 // INT8 -> bf16 (exact), 64 keys a piece, into the operand layout.
                 constexpr int per = KT / 64, units = T::kPiece / 16 / 128;
                 const int ct = threadIdx.x - T::kConvert * 32;
+                // Unit u of this thread: 16 values of key u * step + key_t.
+                constexpr int step = 2048 / HD;
+                const int key_t = ct / (HD / 16), q = ct % (HD / 16), c0 = q % 4 * 2, sw = key_t & 7;
+                const int at_k = q / 4 * (KT * 128) + key_t * 128,
+                          at_v = (key_t / kPage * PN + q / 4) * (kPage * 128) + key_t % kPage * 128;
                 bool ok = true;
 #pragma unroll 1
                 for (int z = 0; ok && z < 2 * nk * per; ++z) {
@@ -906,7 +921,8 @@ __global__ void __launch_bounds__(Tile<TV, TC, HD>::kThreads, 1)
                     ok = __all_sync(0xffffffffu, ok && wait(&ctl->raw_full[rs], (uint32_t)((z / RS) & 1), ctl));
                     if (!ok) break;
                     const uint8_t *src = s_raw + (size_t)rs * T::kPiece;
-                    uint8_t *dst = (is_k ? s_k : s_v) + (size_t)st * T::kTileBytes + half * (64 * 128);
+                    // K: panels of all the tile's keys; V: a page's panels together.
+                    uint8_t *dst = (is_k ? s_k : s_v) + (size_t)st * T::kTileBytes + half * (is_k ? 64 * 128 : 64 * HD * 2);
                     uint4 w[units];
 #pragma unroll
                     for (int u = 0; u < units; ++u) w[u] = *(const uint4 *)(src + (u * 128 + ct) * 16);
@@ -914,7 +930,6 @@ __global__ void __launch_bounds__(Tile<TV, TC, HD>::kThreads, 1)
                     if (lane == 0) mbar_arrive(&ctl->raw_empty[rs]);
 #pragma unroll
                     for (int u = 0; u < units; ++u) {
-                        const int e = u * 128 + ct, key = e / (HD / 16), q = e % (HD / 16);
                         uint4 o0, o1;
                         o0.x = s8x2_to_bf16x2(__byte_perm(w[u].x, 0u, 0x4140u));
                         o0.y = s8x2_to_bf16x2(__byte_perm(w[u].x, 0u, 0x4342u));
@@ -924,9 +939,9 @@ __global__ void __launch_bounds__(Tile<TV, TC, HD>::kThreads, 1)
                         o1.y = s8x2_to_bf16x2(__byte_perm(w[u].z, 0u, 0x4342u));
                         o1.z = s8x2_to_bf16x2(__byte_perm(w[u].w, 0u, 0x4140u));
                         o1.w = s8x2_to_bf16x2(__byte_perm(w[u].w, 0u, 0x4342u));
-                        uint8_t *r = dst + (q / 4) * (KT * 128) + key * 128;
-                        *(uint4 *)(r + ((((q % 4) * 2) ^ (key & 7)) << 4)) = o0;
-                        *(uint4 *)(r + ((((q % 4) * 2 + 1) ^ (key & 7)) << 4)) = o1;
+                        uint8_t *r = dst + (is_k ? at_k + u * (step * 128) : at_v + u * (step / kPage * PN * kPage * 128));
+                        *(uint4 *)(r + ((c0 ^ sw) << 4)) = o0;
+                        *(uint4 *)(r + (((c0 + 1) ^ sw) << 4)) = o1;
                     }
                     fence_proxy_async_smem();
                     if (half == per - 1) {
@@ -963,13 +978,16 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
     return fn;
 }
 
-// A pool as rows of HD bf16 elements, boxes of one page's 64-element panel.
-bool encode_pool(CUtensorMap &m, const void *base, int hd, size_t rows) {
+// A pool as rows of HD bf16 elements: boxes of one page's 64-element panel
+// (K), or of all its panels, one after the other (V).
+bool encode_pool(CUtensorMap &m, const void *base, int hd, size_t rows, bool panels) {
     auto fn = encode_fn();
     if (!fn) return false;
-    cuuint64_t dims[2] = {(cuuint64_t)hd, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)hd * 2};
-    cuuint32_t box[2] = {64, kPage}, es[2] = {1, 1};
-    return fn(&m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, (void *)base, dims, strides, box, es,
+    const cuuint32_t pn = (cuuint32_t)hd / 64;
+    cuuint64_t dims[3] = {(cuuint64_t)(panels ? 64 : hd), (cuuint64_t)rows, pn};
+    cuuint64_t strides[2] = {(cuuint64_t)hd * 2, 128};
+    cuuint32_t box[3] = {64, kPage, pn}, es[3] = {1, 1, 1};
+    return fn(&m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, panels ? 3 : 2, (void *)base, dims, strides, box, es,
               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
@@ -991,11 +1009,11 @@ cudaError_t launch(const Args &a, size_t pool_rows, cudaStream_t st) {
         cudaFuncAttributes fa;
         e = cudaFuncGetAttributes(&fa, attend_tile<TV, TC, HD>);
         if (e != cudaSuccess) return e;
-        if (T::NP == 3 && fa.numRegs != T::kLaunchRegs) return cudaErrorInvalidConfiguration;
+        if (fa.numRegs != T::kLaunchRegs) return cudaErrorInvalidConfiguration;
         configured[dev].store(true);
     }
     alignas(64) CUtensorMap mk = {}, mv = {};
-    if (!T::kInt8 && (!encode_pool(mk, a.k, HD, pool_rows) || !encode_pool(mv, a.v, HD, pool_rows)))
+    if (!T::kInt8 && (!encode_pool(mk, a.k, HD, pool_rows, false) || !encode_pool(mv, a.v, HD, pool_rows, true)))
         return cudaErrorInvalidValue;
     attend_tile<TV, TC, HD><<<a.items, T::kThreads, smem, st>>>(mk, mv, a);
     return cudaGetLastError();
