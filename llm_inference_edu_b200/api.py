@@ -373,44 +373,46 @@ def _paged_rows(t, plan, heads: int, head_dim: int, name: str):
         raise ValueError(f"{name} must be on the plan's device")
     if t.dtype != plan._torch_dtype:
         raise ValueError(f"{name} must be of the plan's type")
-    shape, stride = t.shape, t.stride()
+    shape = t.shape
     if len(shape) != 3 or shape[1] != heads or shape[2] != head_dim:
         raise ValueError(f"{name} must be [tokens][{heads}][{head_dim}]")
-    if (stride[2] != 1 and head_dim > 1) or (stride[1] != head_dim and heads > 1):
+    step, head, one = t.stride()
+    if (one != 1 and head_dim > 1) or (head != head_dim and heads > 1):
         raise ValueError(f"{name}'s rows must be contiguous")
+    tokens, row = shape[0], heads * head_dim
+    if tokens > 1:
+        return t.data_ptr(), (tokens - 1) * step + row, step
     # One token has no distance to the next; its stride may be anything.
-    step = stride[0] if shape[0] > 1 else heads * head_dim
-    return t.data_ptr(), (shape[0] - 1) * step + heads * head_dim if shape[0] else 0, step
+    return t.data_ptr(), tokens * row, row
 
 
-class _PagedCall:
-    """Device and stream of one call; memory that was not allocated on that
-    stream is marked as used by it."""
+def _paged_call(call, plan, cache, stream, *tensors):
+    """Runs call(stream) on the plan's device.  Memory that was allocated on
+    another stream is marked as used by this one."""
+    import torch
+    dev = plan.device
+    if cache.device != dev:
+        raise ValueError("the cache must be on the plan's device")
+    if torch.cuda.current_device() != dev.index:
+        with torch.cuda.device(dev):
+            return _paged_call(call, plan, cache, stream, *tensors)
+    if stream is None:
+        s = torch._C._cuda_getCurrentRawStream(dev.index)
+    else:
+        s = int(stream)
+        for t in tensors + (cache.k, cache.v, cache.k_scales, cache.v_scales):
+            if t is not None:
+                t.record_stream(_paged_stream(s, dev))
+    if s != plan._stream:
+        plan.words.record_stream(_paged_stream(s, dev))
+    status = call(s)
+    if status:
+        _check(status, CacheError)
 
-    def __init__(self, plan, cache, stream, *tensors):
-        import torch
-        if cache.device != plan.device:
-            raise ValueError("the cache must be on the plan's device")
-        self.guard = None
-        if torch.cuda.current_device() != plan.device.index:
-            self.guard = torch.cuda.device(plan.device)
-            self.guard.__enter__()
-        if stream is None:
-            self.stream = torch.cuda.current_stream(plan.device).cuda_stream
-        else:
-            self.stream = int(stream)
-            ext = torch.cuda.ExternalStream(self.stream, device=plan.device) if self.stream else \
-                torch.cuda.default_stream(plan.device)
-            held = tensors + tuple(t for t in (cache.k, cache.v, cache.k_scales, cache.v_scales) if t is not None)
-            for t in held:
-                t.record_stream(ext)
-        if self.stream != plan._stream:
-            plan.words.record_stream(torch.cuda.ExternalStream(self.stream, device=plan.device) if self.stream else
-                                     torch.cuda.default_stream(plan.device))
 
-    def done(self):
-        if self.guard is not None:
-            self.guard.__exit__(None, None, None)
+def _paged_stream(s: int, dev):
+    import torch
+    return torch.cuda.ExternalStream(s, device=dev) if s else torch.cuda.default_stream(dev)
 
 
 def kv_write(k, v, cache: PagedCache, plan: PagedPlan, stream=None):
@@ -419,11 +421,8 @@ def kv_write(k, v, cache: PagedCache, plan: PagedPlan, stream=None):
     cache; all other cache rows stay as they are."""
     h, d = cache.kv_heads, cache.head_dim
     kr, vr = _paged_rows(k, plan, h, d, "k"), _paged_rows(v, plan, h, d, "v")
-    call = _PagedCall(plan, cache, stream, k, v)
-    try:
-        _check(lib().qb_kv_write(*kr, *vr, cache._ref, plan._ref, plan._words, call.stream), CacheError)
-    finally:
-        call.done()
+    _paged_call(lambda s: lib().qb_kv_write(*kr, *vr, cache._ref, plan._ref, plan._words, s), plan, cache, stream,
+                k, v)
 
 
 def kv_read(cache: PagedCache, plan: PagedPlan, k, v, stream=None):
@@ -431,11 +430,8 @@ def kv_read(cache: PagedCache, plan: PagedPlan, k, v, stream=None):
     a plan that starts at 0 reads whole sequences."""
     h, d = cache.kv_heads, cache.head_dim
     kr, vr = _paged_rows(k, plan, h, d, "k"), _paged_rows(v, plan, h, d, "v")
-    call = _PagedCall(plan, cache, stream, k, v)
-    try:
-        _check(lib().qb_kv_read(cache._ref, plan._ref, plan._words, *kr, *vr, call.stream), CacheError)
-    finally:
-        call.done()
+    _paged_call(lambda s: lib().qb_kv_read(cache._ref, plan._ref, plan._words, *kr, *vr, s), plan, cache, stream,
+                k, v)
 
 
 def paged_attention(q, cache: PagedCache, plan: PagedPlan, y, scale: Optional[float] = None, stream=None):
@@ -443,28 +439,27 @@ def paged_attention(q, cache: PagedCache, plan: PagedPlan, y, scale: Optional[fl
     sequences' pages, their own rows (``kv_write``) included: y [tokens]
     [query_heads][head_dim] = softmax(scale q.k) v over the positions each
     token sees; scale = 1 / sqrt(head_dim) by default."""
-    import torch
     h, d = plan.query_heads, cache.head_dim
     qr, yr = _paged_rows(q, plan, h, d, "q"), _paged_rows(y, plan, h, d, "y")
     if not y.is_contiguous():
         raise ValueError("y must be contiguous")
-    call = _PagedCall(plan, cache, stream, q, y)
-    try:
-        ws, need = None, plan._c.workspace_bytes
+    need = plan._c.workspace_bytes
+    scale = float(d ** -0.5 if scale is None else scale)
+
+    def call(s):
+        ws = None
         if need:
             # From the call's own stream, so that calls never share one.
+            import torch
             if stream is None:
                 ws = torch.empty(need, dtype=torch.uint8, device=plan.device)
             else:
-                ext = torch.cuda.ExternalStream(call.stream, device=plan.device) if call.stream else \
-                    torch.cuda.default_stream(plan.device)
-                with torch.cuda.stream(ext):
+                with torch.cuda.stream(_paged_stream(s, plan.device)):
                     ws = torch.empty(need, dtype=torch.uint8, device=plan.device)
-        _check(lib().qb_paged_attention(*qr, cache._ref, plan._ref, plan._words, yr[0], yr[1],
-                                        float(d ** -0.5 if scale is None else scale),
-                                        None if ws is None else ws.data_ptr(), need, call.stream), CacheError)
-    finally:
-        call.done()
+        return lib().qb_paged_attention(*qr, cache._ref, plan._ref, plan._words, yr[0], yr[1], scale,
+                                        None if ws is None else ws.data_ptr(), need, s)
+
+    _paged_call(call, plan, cache, stream, q, y)
 
 
 # ---------------------------------------------------------------- model --

@@ -24,7 +24,7 @@ constexpr int kRowWarps = 8;
 // One warp a row, in any alignment: the row sits in registers between the
 // maximum and the encode.
 template <typename TV, typename TC>
-__global__ void __launch_bounds__(kRowWarps * 32) kv_write_rows(const RowArgs a) {
+__global__ void __launch_bounds__(kRowWarps * 32) kv_write_rows(const __grid_constant__ RowArgs a) {
     const size_t row = (size_t)blockIdx.x * kRowWarps + (threadIdx.x >> 5);
     const int lane = threadIdx.x & 31, z = blockIdx.y;
     if (row >= a.rows) return;
@@ -64,7 +64,7 @@ __global__ void __launch_bounds__(kRowWarps * 32) kv_write_rows(const RowArgs a)
 }
 
 template <typename TV, typename TC>
-__global__ void __launch_bounds__(kRowWarps * 32) kv_read_rows(const RowArgs a) {
+__global__ void __launch_bounds__(kRowWarps * 32) kv_read_rows(const __grid_constant__ RowArgs a) {
     const size_t row = (size_t)blockIdx.x * kRowWarps + (threadIdx.x >> 5);
     const int lane = threadIdx.x & 31, z = blockIdx.y;
     if (row >= a.rows) return;
@@ -79,10 +79,182 @@ __global__ void __launch_bounds__(kRowWarps * 32) kv_read_rows(const RowArgs a) 
         if (lane + 32 * i < a.hd) store_value(y, lane + 32 * i, __fmul_rn(load_value(x, lane + 32 * i), scale));
 }
 
+// The same in 16-byte pieces of the values, where widths and alignment allow
+// (lanes: pieces a row, a power of two up to 32).  Bound by HBM once there
+// are rows enough to keep loads in flight: each thread has kRun rows under
+// way, a block's worth apart.
+constexpr int kRun = 4;
+
+template <typename TV>
+struct Piece {
+    static constexpr int E = 16 / (int)sizeof(TV);
+    __device__ static void unpack(const uint4 &w, float (&v)[E]) {
+        if constexpr (sizeof(TV) == 4) {
+            v[0] = __uint_as_float(w.x); v[1] = __uint_as_float(w.y);
+            v[2] = __uint_as_float(w.z); v[3] = __uint_as_float(w.w);
+        } else {
+            v[0] = bf16_lo(w.x); v[1] = bf16_hi(w.x); v[2] = bf16_lo(w.y); v[3] = bf16_hi(w.y);
+            v[4] = bf16_lo(w.z); v[5] = bf16_hi(w.z); v[6] = bf16_lo(w.w); v[7] = bf16_hi(w.w);
+        }
+    }
+};
+
+// E elements of the row: 4 E bytes (FP32), 2 E (BF16) or E (INT8).
+template <typename TC, int E>
+__device__ __forceinline__ void store_piece(TC *p, const float (&v)[E]) {
+    if constexpr (sizeof(TC) == 4) {
+#pragma unroll
+        for (int e = 0; e < E; e += 4) *(float4 *)(p + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+    } else if constexpr (sizeof(TC) == 2) {
+        uint32_t w[E / 2];
+#pragma unroll
+        for (int e = 0; e < E / 2; ++e) w[e] = bf16_bits(v[2 * e]) | (uint32_t)bf16_bits(v[2 * e + 1]) << 16;
+#pragma unroll
+        for (int e = 0; e < E / 2; e += 2) *(uint2 *)((uint32_t *)p + e) = make_uint2(w[e], w[e + 1]);
+    } else {
+        uint32_t w[E / 4];
+#pragma unroll
+        for (int e = 0; e < E / 4; ++e)
+            w[e] = ((uint32_t)(int)v[4 * e] & 255u) | ((uint32_t)(int)v[4 * e + 1] & 255u) << 8 |
+                   ((uint32_t)(int)v[4 * e + 2] & 255u) << 16 | ((uint32_t)(int)v[4 * e + 3] & 255u) << 24;
+#pragma unroll
+        for (int e = 0; e < E / 4; ++e) ((uint32_t *)p)[e] = w[e];
+    }
+}
+
+template <typename TC, int E>
+__device__ __forceinline__ void load_piece(const TC *p, float (&v)[E]) {
+    if constexpr (sizeof(TC) == 4) {
+#pragma unroll
+        for (int e = 0; e < E; e += 4) {
+            const float4 w = *(const float4 *)(p + e);
+            v[e] = w.x; v[e + 1] = w.y; v[e + 2] = w.z; v[e + 3] = w.w;
+        }
+    } else if constexpr (sizeof(TC) == 2) {
+#pragma unroll
+        for (int e = 0; e < E; e += 4) {
+            const uint2 w = *(const uint2 *)(p + e);
+            v[e] = bf16_lo(w.x); v[e + 1] = bf16_hi(w.x); v[e + 2] = bf16_lo(w.y); v[e + 3] = bf16_hi(w.y);
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < E; e += 4) {
+            const uint32_t w = *(const uint32_t *)(p + e);
+#pragma unroll
+            for (int x = 0; x < 4; ++x) v[e + x] = (float)(int8_t)(w >> (8 * x));
+        }
+    }
+}
+
+// round(x / scale), halves away from zero, in -127 .. 127, for finite x.  The
+// product with 1 / scale is within 2^-22 of the quotient (relative), so it
+// rounds alike unless it lies that close to a half; there, and where it is
+// no number, the FP32 quotient decides.
+__device__ __forceinline__ float encode(float x, float scale, float inv) {
+    const float h = fabsf(x) * inv + 0.5f, n = floorf(h), d = h - n;
+    float r = copysignf(fminf(n, 127.0f), x);
+    if (!(d > 1e-4f && d < 1.0f - 1e-4f)) r = fminf(fmaxf(roundf(__fdiv_rn(x, scale)), -127.0f), 127.0f);
+    return r;
+}
+
+template <typename TV, typename TC>
+__global__ void __launch_bounds__(256) kv_write_pieces(const __grid_constant__ RowArgs a, int lanes) {
+    constexpr int E = Piece<TV>::E;
+    const int per = 256 / lanes, lane = threadIdx.x & (lanes - 1), z = blockIdx.y;
+    const uint32_t rows = (uint32_t)a.rows, KV = (uint32_t)a.KV, row0 = blockIdx.x * per * kRun + threadIdx.x / lanes;
+    uint4 w[kRun];
+    int slot[kRun];
+#pragma unroll
+    for (int r = 0; r < kRun; ++r) {
+        const uint32_t row = row0 + r * per;
+        w[r] = make_uint4(0u, 0u, 0u, 0u);
+        slot[r] = 0;
+        if (row < rows) {
+            const uint32_t tok = row / KV;
+            slot[r] = a.slots[tok];
+            w[r] = ld_stream_u4((const TV *)a.x[z] + tok * a.stride[z] + (size_t)(row % KV) * a.hd + lane * E);
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < kRun; ++r) {
+        const uint32_t row = row0 + r * per;
+        float v[E];
+        Piece<TV>::unpack(w[r], v);
+        float scale = 1.0f;
+        bool bad = false;
+        if constexpr (sizeof(TC) == 1) {
+            float m = 0.0f;
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                m = fmaxf(m, fabsf(v[e]));
+                bad |= !isfinite(v[e]);
+            }
+            // A NaN is above every number in the maximum of bit patterns.
+            uint32_t mb = bad ? 0x7fffffffu : __float_as_uint(m);
+            for (int off = lanes >> 1; off; off >>= 1) mb = max(mb, __shfl_xor_sync(0xffffffffu, mb, off));
+            bad = mb == 0x7fffffffu;
+            scale = __fdiv_rn(__uint_as_float(mb), 127.0f);
+            if (scale == 0.0f) scale = 1.0f;
+            const float inv = __fdiv_rn(1.0f, scale);
+#pragma unroll
+            for (int e = 0; e < E; ++e) v[e] = bad ? 0.0f : encode(v[e], scale, inv);
+        }
+        if (row >= rows) continue;
+        const size_t at = ((size_t)((uint32_t)slot[r] / kPage) * KV + row % KV) * kPage + (uint32_t)slot[r] % kPage;
+        store_piece<TC, E>((TC *)a.pool[z] + at * a.hd + lane * E, v);
+        if (sizeof(TC) == 1 && lane == 0) a.scales[z][at] = bad ? __uint_as_float(0x7fffffffu) : scale;
+    }
+}
+
+template <typename TV, typename TC>
+__global__ void __launch_bounds__(256) kv_read_pieces(const __grid_constant__ RowArgs a, int lanes) {
+    constexpr int E = Piece<TV>::E;
+    const int per = 256 / lanes, lane = threadIdx.x & (lanes - 1), z = blockIdx.y;
+    const uint32_t rows = (uint32_t)a.rows, KV = (uint32_t)a.KV, row0 = blockIdx.x * per * kRun + threadIdx.x / lanes;
+    float v[kRun][E], scale[kRun];
+    int slot[kRun];
+#pragma unroll
+    for (int r = 0; r < kRun; ++r) {
+        const uint32_t row = row0 + r * per;
+        slot[r] = row < rows ? a.slots[row / KV] : 0;
+    }
+#pragma unroll
+    for (int r = 0; r < kRun; ++r) {
+        const uint32_t row = row0 + r * per;
+        if (row >= rows) continue;
+        const size_t at = ((size_t)((uint32_t)slot[r] / kPage) * KV + row % KV) * kPage + (uint32_t)slot[r] % kPage;
+        load_piece<TC, E>((const TC *)a.pool[z] + at * a.hd + lane * E, v[r]);
+        scale[r] = sizeof(TC) == 1 ? a.scales[z][at] : 1.0f;
+    }
+#pragma unroll
+    for (int r = 0; r < kRun; ++r) {
+        const uint32_t row = row0 + r * per;
+        if (row >= rows) continue;
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[r][e] = __fmul_rn(v[r][e], scale[r]);
+        store_piece<TV, E>((TV *)a.out[z] + (row / KV) * a.stride[z] + (size_t)(row % KV) * a.hd + lane * E, v[r]);
+    }
+}
+
 template <typename TV, typename TC>
 uint32_t launch_rows(const RowArgs &a, bool write, cudaStream_t st) {
-    const size_t blocks = (a.rows + kRowWarps - 1) / kRowWarps;
-    const dim3 grid((unsigned)blocks, 2);
+    constexpr int E = Piece<TV>::E;
+    const int lanes = a.hd / E;
+    uintptr_t all = 0;
+    for (int z = 0; z < 2; ++z) all |= (uintptr_t)a.x[z] | (uintptr_t)a.out[z] | a.stride[z] * sizeof(TV);
+    // 8,192 tokens of 4 heads of 128, FP32 into INT8 and back: 17 us in
+    // pieces, 65 us a row at a time.
+    if (a.hd % E == 0 && lanes <= 32 && (lanes & (lanes - 1)) == 0 && !(all & 15)) {
+        const size_t per = (size_t)(256 / lanes) * kRun;
+        const dim3 grid((unsigned)((a.rows + per - 1) / per), 2);
+        if (write)
+            kv_write_pieces<TV, TC><<<grid, 256, 0, st>>>(a, lanes);
+        else
+            kv_read_pieces<TV, TC><<<grid, 256, 0, st>>>(a, lanes);
+        QB_CUDA(cudaGetLastError());
+        return QB_OK;
+    }
+    const dim3 grid((unsigned)((a.rows + kRowWarps - 1) / kRowWarps), 2);
     if (write)
         kv_write_rows<TV, TC><<<grid, kRowWarps * 32, 0, st>>>(a);
     else
