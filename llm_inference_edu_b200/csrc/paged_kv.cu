@@ -17,6 +17,7 @@ struct RowArgs {
     size_t stride[2];
     void *pool[2];
     float *scales[2];
+    uint32_t mul, shift;  // row / KV = (mulhi(row, mul) + row) >> shift, row < 2^31
 };
 
 constexpr int kRowWarps = 8;
@@ -99,7 +100,7 @@ struct Piece {
     }
 };
 
-// E elements of the row: 4 E bytes (FP32), 2 E (BF16) or E (INT8).
+// E elements of the row as FP32 or BF16.
 template <typename TC, int E>
 __device__ __forceinline__ void store_piece(TC *p, const float (&v)[E]) {
     if constexpr (sizeof(TC) == 4) {
@@ -111,14 +112,6 @@ __device__ __forceinline__ void store_piece(TC *p, const float (&v)[E]) {
         for (int e = 0; e < E / 2; ++e) w[e] = bf16_bits(v[2 * e]) | (uint32_t)bf16_bits(v[2 * e + 1]) << 16;
 #pragma unroll
         for (int e = 0; e < E / 2; e += 2) *(uint2 *)((uint32_t *)p + e) = make_uint2(w[e], w[e + 1]);
-    } else {
-        uint32_t w[E / 4];
-#pragma unroll
-        for (int e = 0; e < E / 4; ++e)
-            w[e] = ((uint32_t)(int)v[4 * e] & 255u) | ((uint32_t)(int)v[4 * e + 1] & 255u) << 8 |
-                   ((uint32_t)(int)v[4 * e + 2] & 255u) << 16 | ((uint32_t)(int)v[4 * e + 3] & 255u) << 24;
-#pragma unroll
-        for (int e = 0; e < E / 4; ++e) ((uint32_t *)p)[e] = w[e];
     }
 }
 
@@ -146,63 +139,88 @@ __device__ __forceinline__ void load_piece(const TC *p, float (&v)[E]) {
     }
 }
 
-// round(x / scale), halves away from zero, in -127 .. 127, for finite x.  The
-// product with 1 / scale is within 2^-22 of the quotient (relative), so it
-// rounds alike unless it lies that close to a half; there, and where it is
-// no number, the FP32 quotient decides.
-__device__ __forceinline__ float encode(float x, float scale, float inv) {
-    const float h = fabsf(x) * inv + 0.5f, n = floorf(h), d = h - n;
-    float r = copysignf(fminf(n, 127.0f), x);
-    if (!(d > 1e-4f && d < 1.0f - 1e-4f)) r = fminf(fmaxf(roundf(__fdiv_rn(x, scale)), -127.0f), 127.0f);
-    return r;
+// A row of the grid: its token, KV head and cache row.
+struct RowAt {
+    uint32_t tok, g;
+    __device__ RowAt(const RowArgs &a, uint32_t row) {
+        tok = (__umulhi(row, a.mul) + row) >> a.shift;
+        g = row - tok * (uint32_t)a.KV;
+    }
+    __device__ size_t cache_row(const RowArgs &a, int slot) const {
+        return ((size_t)((uint32_t)slot / kPage) * (uint32_t)a.KV + g) * kPage + (uint32_t)slot % kPage;
+    }
+};
+
+// One row's E elements as INT8 with the row's scale (mb: the largest bit
+// pattern of the row's magnitudes).  x / scale rounded, halves away from
+// zero: added to 1.5 * 2^23 the product x * (1 / scale) rounds to the
+// integer that then lies in the low byte.  The product is within 2^-22 of
+// the FP32 quotient (relative, so 2e-5 here) and rounds alike unless it lies
+// that close to a half; there, and where it is no number, the quotient
+// itself decides.
+template <int E>
+__device__ __forceinline__ float encode_row(const float (&v)[E], uint32_t mb, uint32_t (&out)[E / 4]) {
+    const bool bad = mb >= 0x7f800000u;
+    float scale = __fdiv_rn(__uint_as_float(mb), 127.0f);
+    if (scale == 0.0f) scale = 1.0f;
+    const float inv = __fdiv_rn(1.0f, scale), big = 12582912.0f;
+    bool exact = bad;
+    uint32_t q[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const float h = fmaf(v[e], inv, big);
+        q[e] = __float_as_uint(h);
+        exact |= !(fabsf(fmaf(v[e], inv, -(h - big))) <= 0.4999f);
+    }
+    if (exact)
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+            q[e] = bad ? 0u : (uint32_t)(int)fminf(fmaxf(roundf(__fdiv_rn(v[e], scale)), -127.0f), 127.0f);
+#pragma unroll
+    for (int e = 0; e < E; e += 4)
+        out[e / 4] = __byte_perm(__byte_perm(q[e], q[e + 1], 0x0040u), __byte_perm(q[e + 2], q[e + 3], 0x0040u), 0x5410u);
+    return bad ? __uint_as_float(0x7fffffffu) : scale;
 }
 
 template <typename TV, typename TC>
 __global__ void __launch_bounds__(256) kv_write_pieces(const __grid_constant__ RowArgs a, int lanes) {
     constexpr int E = Piece<TV>::E;
     const int per = 256 / lanes, lane = threadIdx.x & (lanes - 1), z = blockIdx.y;
-    const uint32_t rows = (uint32_t)a.rows, KV = (uint32_t)a.KV, row0 = blockIdx.x * per * kRun + threadIdx.x / lanes;
+    const uint32_t rows = (uint32_t)a.rows, row0 = blockIdx.x * per * kRun + threadIdx.x / lanes;
+    const TV *x = (const TV *)a.x[z] + lane * E;
+    TC *pool = (TC *)a.pool[z] + lane * E;
     uint4 w[kRun];
-    int slot[kRun];
+    size_t at[kRun];
 #pragma unroll
     for (int r = 0; r < kRun; ++r) {
         const uint32_t row = row0 + r * per;
         w[r] = make_uint4(0u, 0u, 0u, 0u);
-        slot[r] = 0;
         if (row < rows) {
-            const uint32_t tok = row / KV;
-            slot[r] = a.slots[tok];
-            w[r] = ld_stream_u4((const TV *)a.x[z] + tok * a.stride[z] + (size_t)(row % KV) * a.hd + lane * E);
+            const RowAt p(a, row);
+            w[r] = ld_stream_u4(x + p.tok * a.stride[z] + p.g * (uint32_t)a.hd);
+            at[r] = p.cache_row(a, a.slots[p.tok]);
         }
     }
 #pragma unroll
     for (int r = 0; r < kRun; ++r) {
-        const uint32_t row = row0 + r * per;
         float v[E];
         Piece<TV>::unpack(w[r], v);
-        float scale = 1.0f;
-        bool bad = false;
         if constexpr (sizeof(TC) == 1) {
-            float m = 0.0f;
+            uint32_t mb = 0, q[E / 4];
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-                m = fmaxf(m, fabsf(v[e]));
-                bad |= !isfinite(v[e]);
-            }
-            // A NaN is above every number in the maximum of bit patterns.
-            uint32_t mb = bad ? 0x7fffffffu : __float_as_uint(m);
+            for (int e = 0; e < E; ++e) mb = max(mb, __float_as_uint(v[e]) & 0x7fffffffu);
             for (int off = lanes >> 1; off; off >>= 1) mb = max(mb, __shfl_xor_sync(0xffffffffu, mb, off));
-            bad = mb == 0x7fffffffu;
-            scale = __fdiv_rn(__uint_as_float(mb), 127.0f);
-            if (scale == 0.0f) scale = 1.0f;
-            const float inv = __fdiv_rn(1.0f, scale);
-#pragma unroll
-            for (int e = 0; e < E; ++e) v[e] = bad ? 0.0f : encode(v[e], scale, inv);
+            const float scale = encode_row<E>(v, mb, q);
+            if (row0 + r * per >= rows) continue;
+            uint32_t *y = (uint32_t *)(pool + at[r] * (uint32_t)a.hd);
+            if constexpr (E == 8)
+                *(uint2 *)y = make_uint2(q[0], q[1]);
+            else
+                *y = q[0];
+            if (lane == 0) a.scales[z][at[r]] = scale;
+        } else {
+            if (row0 + r * per < rows) store_piece<TC, E>(pool + at[r] * (uint32_t)a.hd, v);
         }
-        if (row >= rows) continue;
-        const size_t at = ((size_t)((uint32_t)slot[r] / kPage) * KV + row % KV) * kPage + (uint32_t)slot[r] % kPage;
-        store_piece<TC, E>((TC *)a.pool[z] + at * a.hd + lane * E, v);
-        if (sizeof(TC) == 1 && lane == 0) a.scales[z][at] = bad ? __uint_as_float(0x7fffffffu) : scale;
     }
 }
 
@@ -210,30 +228,29 @@ template <typename TV, typename TC>
 __global__ void __launch_bounds__(256) kv_read_pieces(const __grid_constant__ RowArgs a, int lanes) {
     constexpr int E = Piece<TV>::E;
     const int per = 256 / lanes, lane = threadIdx.x & (lanes - 1), z = blockIdx.y;
-    const uint32_t rows = (uint32_t)a.rows, KV = (uint32_t)a.KV, row0 = blockIdx.x * per * kRun + threadIdx.x / lanes;
-    float v[kRun][E], scale[kRun];
+    const uint32_t rows = (uint32_t)a.rows, row0 = blockIdx.x * per * kRun + threadIdx.x / lanes;
+    const TC *pool = (const TC *)a.pool[z] + lane * E;
+    TV *out = (TV *)a.out[z] + lane * E;
     int slot[kRun];
+    float v[kRun][E], scale[kRun];
 #pragma unroll
-    for (int r = 0; r < kRun; ++r) {
-        const uint32_t row = row0 + r * per;
-        slot[r] = row < rows ? a.slots[row / KV] : 0;
-    }
+    for (int r = 0; r < kRun; ++r)
+        slot[r] = row0 + r * per < rows ? a.slots[RowAt(a, row0 + r * per).tok] : 0;
 #pragma unroll
-    for (int r = 0; r < kRun; ++r) {
-        const uint32_t row = row0 + r * per;
-        if (row >= rows) continue;
-        const size_t at = ((size_t)((uint32_t)slot[r] / kPage) * KV + row % KV) * kPage + (uint32_t)slot[r] % kPage;
-        load_piece<TC, E>((const TC *)a.pool[z] + at * a.hd + lane * E, v[r]);
-        scale[r] = sizeof(TC) == 1 ? a.scales[z][at] : 1.0f;
-    }
+    for (int r = 0; r < kRun; ++r)
+        if (row0 + r * per < rows) {
+            const size_t at = RowAt(a, row0 + r * per).cache_row(a, slot[r]);
+            load_piece<TC, E>(pool + at * (uint32_t)a.hd, v[r]);
+            scale[r] = sizeof(TC) == 1 ? a.scales[z][at] : 1.0f;
+        }
 #pragma unroll
-    for (int r = 0; r < kRun; ++r) {
-        const uint32_t row = row0 + r * per;
-        if (row >= rows) continue;
+    for (int r = 0; r < kRun; ++r)
+        if (row0 + r * per < rows) {
+            const RowAt p(a, row0 + r * per);
 #pragma unroll
-        for (int e = 0; e < E; ++e) v[r][e] = __fmul_rn(v[r][e], scale[r]);
-        store_piece<TV, E>((TV *)a.out[z] + (row / KV) * a.stride[z] + (size_t)(row % KV) * a.hd + lane * E, v[r]);
-    }
+            for (int e = 0; e < E; ++e) v[r][e] = __fmul_rn(v[r][e], scale[r]);
+            store_piece<TV, E>(out + p.tok * a.stride[z] + p.g * (uint32_t)a.hd, v[r]);
+        }
 }
 
 template <typename TV, typename TC>
@@ -263,7 +280,15 @@ uint32_t launch_rows(const RowArgs &a, bool write, cudaStream_t st) {
     return QB_OK;
 }
 
-uint32_t run_rows(const RowArgs &a, uint32_t vt, uint32_t ct, bool write, cudaStream_t st) {
+// Multiplier and shift of RowArgs for a division by d.
+void divide_by(uint32_t d, uint32_t &mul, uint32_t &shift) {
+    shift = 0;
+    while ((1ull << shift) < d) ++shift;
+    mul = (uint32_t)(((1ull << 32) * ((1ull << shift) - d)) / d + 1);
+}
+
+uint32_t run_rows(RowArgs a, uint32_t vt, uint32_t ct, bool write, cudaStream_t st) {
+    divide_by((uint32_t)a.KV, a.mul, a.shift);
     if (vt == QB_PAGED_F32) {
         if (ct == QB_PAGED_F32) return launch_rows<float, float>(a, write, st);
         if (ct == QB_PAGED_BF16) return launch_rows<float, uint16_t>(a, write, st);
