@@ -31,7 +31,7 @@ struct Grid {
 
 // The plain form of every variant: 8 rows and 64 keys a unit, one warp a row.
 Grid rows_grid() { return Grid{64, 8, 148 * 4, 1, 1, 2}; }
-Grid step_grid(int, int, bool) { return Grid{kPage, 8, 148 * 2, 16, 8, 32}; }
+Grid step_grid(int, int, bool) { return Grid{kPage, 8, 148 * 3, 16, 8, 32}; }
 Grid tile_grid(int, int, bool wide) { return Grid{wide ? 64 : 128, wide ? 128 : 256, 148, wide ? 4 : 3, 2, wide ? 4 : 2}; }
 
 Block block_of(const qb_paged_step &s, const Grid &g, int seq, int kvh, int row0, int rows, int G) {

@@ -12,11 +12,23 @@
 // weights cross from accumulator to operand layout by two 8x8 transposes.
 // Nothing goes through shared memory but Q (fragments) and the end result.
 //
-// FP32 values: Q is three bf16 planes (q = p0 + p1 + p2 to 2^-24) and so are
-// the weights, which keeps FP32 precision over exact bf16 or int8 operands at
-// three products each.  BF16 values: one plane of Q, two of the weights (one
-// would double the error of the result's own rounding, and the products are
-// not what this kernel waits for).
+// BF16 caches.  FP32 values: Q is three bf16 planes (q = p0 + p1 + p2 to
+// 2^-24) and so are the weights, which keeps FP32 precision over exact
+// operands at three products each.  BF16 values: one plane of Q, two of the
+// weights (one would double the error of the result's own rounding, and the
+// products are not what this kernel waits for).
+//
+// INT8 caches.  What bounds them is the widening of the bytes on the integer
+// pipe, so they are widened to f16, a byte permute or mask and an addition a
+// pair (1024 + 128 + q is the f16 with bits 0x6480 ^ q; bf16 has too few
+// bits for that), and f16 holds more of Q and the weights: FP32 values take
+// two planes (2^-22), BF16 values one.  f16 lacks range, so each row of Q
+// is scaled by a power of two to a largest element near 2^13, and the
+// weights, which carry the V rows' scales, are taken against the running
+// maximum of score + log2(scale), 2^7 above it: they stay below 2^15 and
+// what f16 drops is below 2^-31 of the largest.  (Scales below 2^-90 lose
+// precision; above 2^90 the row goes the plain way.)  64 sequences of 100 to
+// 8,191 positions at the 7B shape: 52 us widened to bf16, STEP_US us so.
 #include "paged_attn.cuh"
 
 namespace qb {
@@ -31,6 +43,37 @@ __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1
         "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ void mma16816h(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                          uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+__device__ __forceinline__ float2 unpack_f16(uint32_t w) {
+    float2 r;
+    asm("{\n\t.reg .b16 x, y;\n\tmov.b32 {x, y}, %2;\n\tcvt.f32.f16 %0, x;\n\tcvt.f32.f16 %1, y;\n\t}"
+        : "=f"(r.x), "=f"(r.y)
+        : "r"(w));
+    return r;
+}
+// Two int8 values in the low bytes of t's halves as f16, exactly.
+__device__ __forceinline__ uint32_t s8x2_to_f16x2(uint32_t t) {
+    uint32_t r;
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"((t & 0x00ff00ffu) ^ 0x64806480u), "r"(0x64806480u));
+    return r;
+}
+__device__ __forceinline__ float lg2(float x) {
+    float y;
+    asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
 }
 
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
@@ -51,8 +94,9 @@ __device__ __forceinline__ void load_piece(const uint8_t *p, uint32_t (&r)[2]) {
 template <typename TV, typename TC, int HD, int NT>
 struct StepShape {
     static constexpr bool kInt8 = sizeof(TC) == 1;
-    static constexpr int NQ = sizeof(TV) == 4 ? 3 : 1;   // planes of Q
-    static constexpr int NPV = sizeof(TV) == 4 ? 3 : 2;  // planes of the weights
+    static constexpr int NQ = sizeof(TV) == 4 ? (kInt8 ? 2 : 3) : 1;   // planes of Q
+    static constexpr int NPV = sizeof(TV) == 4 ? (kInt8 ? 2 : 3) : kInt8 ? 1 : 2;  // planes of the weights
+    static constexpr float kAbove = kInt8 ? 7.0f : 0.0f;  // of the base the weights are taken against
     static constexpr int KS = HD / 16;                   // k-steps of the scores
     static constexpr int MT = HD / 16;                   // m16 tiles of O^T
     static constexpr int PG = 8192 / (2 * 16 * HD * (int)sizeof(TC));  // pages a warp holds: 8 KB of K and V
@@ -68,11 +112,11 @@ struct StepShape {
 };
 
 template <typename TV, typename TC, int HD, int NT>
-__global__ void __launch_bounds__(kStepWarps * 32, 2) attend_step(const __grid_constant__ Args a) {
+__global__ void __launch_bounds__(kStepWarps * 32, 3) attend_step(const __grid_constant__ Args a) {
     using S = StepShape<TV, TC, HD, NT>;
     constexpr int NQ = S::NQ, NPV = S::NPV, KS = S::KS, MT = S::MT, PG = S::PG, KL = S::KL, VP = S::VP, VW = S::VW;
     __shared__ __align__(16) uint8_t s_raw[S::q_bytes > S::o_bytes ? S::q_bytes : S::o_bytes];
-    __shared__ float s_m[kStepWarps][8 * NT], s_l[kStepWarps][8 * NT];
+    __shared__ float s_m[kStepWarps][8 * NT], s_l[kStepWarps][8 * NT], s_c[8 * NT];
     uint2 *s_q = (uint2 *)s_raw;  // [plane][n tile][k-step][lane]
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
@@ -143,30 +187,58 @@ __global__ void __launch_bounds__(kStepWarps * 32, 2) attend_step(const __grid_c
     load_k();
     load_v();
 
-    // Q fragments: k-step ks of a thread is elements 4 h .. 4 h + 3 of its
-    // 8 (bf16) or 16 (int8) in the j-th stretch of 32 or 64.
-    for (int f = threadIdx.x; f < NT * KS * 32; f += kStepWarps * 32) {
-        const int fl = f & 31, ks = (f >> 5) % KS, nt = (f >> 5) / KS, r = nt * 8 + (fl >> 2);
+    // Q fragments, a row a warp and four elements a lane: k-step ks of a
+    // thread is elements 4 h .. 4 h + 3 of its 8 (bf16) or 16 (int8) in a
+    // stretch of 32 or 64.
+    for (int r = warp; r < 8 * NT; r += kStepWarps) {
         constexpr int per = S::kInt8 ? 4 : 2, run = S::kInt8 ? 16 : 8;
-        const int d = ks / per * (4 * run) + (fl & 3) * run + ks % per * 4;
+        const int d = lane * 4, ks = d / (4 * run) * per + d % run / 4, fl = (r & 7) * 4 + d % (4 * run) / run;
         float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (r < it.rows) {
+        if (r < it.rows && d < HD) {
             const int row = it.row0 + r;
             const TV *q = (const TV *)a.q + (size_t)(sq.tok0 + row / a.G) * a.q_stride +
                           (size_t)(it.kvh * a.G + row % a.G) * HD + d;
 #pragma unroll
             for (int x = 0; x < 4; ++x) v[x] = load_value(q, x);
         }
+        if constexpr (S::kInt8) {
+            // The power of two that brings the row's largest element to
+            // 2^13 .. 2^14 (none for a row without a finite one).
+            uint32_t mb = 0;
 #pragma unroll
-        for (int pl = 0; pl < NQ; ++pl) {
-            uint2 w;
-            w.x = pack_bf16(v[0], v[1]);
-            w.y = pack_bf16(v[2], v[3]);
-            s_q[((pl * NT + nt) * KS + ks) * 32 + fl] = w;
-            v[0] -= bf16_lo(w.x);
-            v[1] -= bf16_hi(w.x);
-            v[2] -= bf16_lo(w.y);
-            v[3] -= bf16_hi(w.y);
+            for (int x = 0; x < 4; ++x) mb = max(mb, __float_as_uint(v[x]) & 0x7fffffffu);
+#pragma unroll
+            for (int off = 16; off; off >>= 1) mb = max(mb, __shfl_xor_sync(0xffffffffu, mb, off));
+            const uint32_t e = min(max(mb >> 23, 27u), 250u);
+            const float up = __uint_as_float((267u - e) << 23);
+#pragma unroll
+            for (int x = 0; x < 4; ++x) v[x] *= up;
+            if (lane == 0) s_c[r] = __fdiv_rn(a.c, up);
+        } else if (lane == 0) {
+            s_c[r] = a.c;
+        }
+        if (d < HD) {
+#pragma unroll
+            for (int pl = 0; pl < NQ; ++pl) {
+                uint2 w;
+                if constexpr (S::kInt8) {
+                    w.x = pack_f16(v[0], v[1]);
+                    w.y = pack_f16(v[2], v[3]);
+                    const float2 x = unpack_f16(w.x), y = unpack_f16(w.y);
+                    v[0] -= x.x;
+                    v[1] -= x.y;
+                    v[2] -= y.x;
+                    v[3] -= y.y;
+                } else {
+                    w.x = pack_bf16(v[0], v[1]);
+                    w.y = pack_bf16(v[2], v[3]);
+                    v[0] -= bf16_lo(w.x);
+                    v[1] -= bf16_hi(w.x);
+                    v[2] -= bf16_lo(w.y);
+                    v[3] -= bf16_hi(w.y);
+                }
+                s_q[((pl * NT + (r >> 3)) * KS + ks) * 32 + fl] = w;
+            }
         }
     }
     __syncthreads();
@@ -178,10 +250,14 @@ __global__ void __launch_bounds__(kStepWarps * 32, 2) attend_step(const __grid_c
 #pragma unroll
         for (int y = 0; y < 2; ++y) pos[nt][y] = sq.start + min(it.row0 + nt * 8 + 2 * c + y, it.row0 + it.rows - 1) / a.G;
 
-    float m[NT][2], l[NT][2], o[NT][MT][4];
+    // m: what the weights are taken against, at least the running maximum
+    // less kAbove.
+    float m[NT][2], l[NT][2], o[NT][MT][4], cr[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
         m[nt][0] = m[nt][1] = -INFINITY;
+        cr[nt][0] = s_c[nt * 8 + 2 * c];
+        cr[nt][1] = s_c[nt * 8 + 2 * c + 1];
         l[nt][0] = l[nt][1] = 0.0f;
 #pragma unroll
         for (int t = 0; t < MT; ++t)
@@ -212,8 +288,8 @@ __global__ void __launch_bounds__(kStepWarps * 32, 2) attend_step(const __grid_c
                 for (int y = 0; y < 2; ++y) {
                     if constexpr (S::kInt8) {
                         const uint32_t q4 = kr[x][y][ks / 4][ks % 4];
-                        w[y][0] = s8x2_to_bf16x2(__byte_perm(q4, 0u, 0x4140u));
-                        w[y][1] = s8x2_to_bf16x2(__byte_perm(q4, 0u, 0x4342u));
+                        w[y][0] = s8x2_to_f16x2(__byte_perm(q4, 0u, 0x4140u));
+                        w[y][1] = s8x2_to_f16x2(__byte_perm(q4, 0u, 0x4342u));
                     } else {
                         w[y][0] = kr[x][y][ks / 2][ks % 2 * 2];
                         w[y][1] = kr[x][y][ks / 2][ks % 2 * 2 + 1];
@@ -223,32 +299,47 @@ __global__ void __launch_bounds__(kStepWarps * 32, 2) attend_step(const __grid_c
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int pl = 0; pl < NQ; ++pl)
-                        mma16816(s[x][nt], w[0][0], w[1][0], w[0][1], w[1][1], b[pl][nt].x, b[pl][nt].y);
+                        if constexpr (S::kInt8)
+                            mma16816h(s[x][nt], w[0][0], w[1][0], w[0][1], w[1][1], b[pl][nt].x, b[pl][nt].y);
+                        else
+                            mma16816(s[x][nt], w[0][0], w[1][0], w[0][1], w[1][1], b[pl][nt].x, b[pl][nt].y);
             }
         }
-        // t = score * log2(e), masked; this group's maximum.
+        // t = score * log2(e), masked; this group's maximum, of t + log2 of
+        // the V row's scale for INT8.
         float bm[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) bm[nt][0] = bm[nt][1] = -INFINITY;
+        bool whole[PG], all = true;
 #pragma unroll
         for (int x = 0; x < PG; ++x) {
             const int j0 = page_of(i + x) * kPage;
-            const bool whole = i + x < it.i1 && j0 + kPage - 1 <= p_lo &&
-                               (a.window == 0 || j0 > p_hi - a.window || j0 + kPage <= a.sinks);
+            whole[x] = i + x < it.i1 && j0 + kPage - 1 <= p_lo &&
+                       (a.window == 0 || j0 > p_hi - a.window || j0 + kPage <= a.sinks);
+            all &= whole[x];
+            float kc[2], lv[2];
+            if constexpr (S::kInt8) {
+#pragma unroll
+                for (int y = 0; y < 2; ++y) {
+                    kc[y] = ksc[x][y];
+                    lv[y] = fminf(fmaxf(lg2(fabsf(vsc[x][y])), -90.0f), 90.0f);
+                }
+            }
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     float t = s[x][nt][e];
-                    if constexpr (S::kInt8) t *= ksc[x][e >> 1];
-                    t *= a.c;
-                    if (!whole && !(i + x < it.i1 && sees(pos[nt][e & 1], j0 + g + (e >> 1) * 8, a.window, a.sinks)))
+                    if constexpr (S::kInt8) t *= kc[e >> 1];
+                    t *= cr[nt][e & 1];
+                    if (!whole[x] && !(i + x < it.i1 && sees(pos[nt][e & 1], j0 + g + (e >> 1) * 8, a.window, a.sinks)))
                         t = -INFINITY;
                     s[x][nt][e] = t;
-                    bm[nt][e & 1] = fmaxf(bm[nt][e & 1], t);
+                    bm[nt][e & 1] = fmaxf(bm[nt][e & 1], S::kInt8 ? t + lv[e >> 1] : t);
                 }
-            if (!whole) {
-                // V rows that no row sees may hold anything: 0 * inf is not 0.
+            if (!S::kInt8 && !whole[x]) {
+                // V rows that no row sees may hold anything: 0 * inf is not
+                // 0 (INT8 values are always finite).
                 const bool here = i + x < it.i1;
 #pragma unroll
                 for (int y = 0; y < 4; ++y) {
@@ -272,7 +363,7 @@ __global__ void __launch_bounds__(kStepWarps * 32, 2) attend_step(const __grid_c
 #pragma unroll
                 for (int off = 4; off < 32; off <<= 1)
                     bm[nt][y] = fmaxf(bm[nt][y], __shfl_xor_sync(0xffffffffu, bm[nt][y], off));
-                grow |= bm[nt][y] > m[nt][y] + 8.0f;
+                grow |= bm[nt][y] > m[nt][y] + (8.0f + S::kAbove);
             }
         // The maximum may lag by a factor 2^8 (weights up to 256 are no less
         // exact): the rescaling of O is then rare.
@@ -281,7 +372,7 @@ __global__ void __launch_bounds__(kStepWarps * 32, 2) attend_step(const __grid_c
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int y = 0; y < 2; ++y) {
-                    const float mn = fmaxf(m[nt][y], bm[nt][y]);
+                    const float mn = fmaxf(m[nt][y], bm[nt][y] - S::kAbove);
                     const float f = m[nt][y] == mn ? 1.0f : ex2(m[nt][y] - mn);
                     m[nt][y] = mn;
                     l[nt][y] *= f;
@@ -300,20 +391,42 @@ __global__ void __launch_bounds__(kStepWarps * 32, 2) attend_step(const __grid_c
                 float p[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const float t = s[x][nt][e], mm = m[nt][e & 1];
-                    p[e] = t == -INFINITY ? 0.0f : ex2(t - mm);
+                    const float t = s[x][nt][e];
+                    p[e] = ex2(t - m[nt][e & 1]);
+                    // Nothing seen so far leaves m at -inf; a hidden key's
+                    // scale may be anything.
+                    if (!all && t == -INFINITY) p[e] = 0.0f;
                     l[nt][e & 1] += p[e];
-                    if constexpr (S::kInt8) p[e] = t == -INFINITY ? 0.0f : p[e] * vsc[x][e >> 1];
+                    if constexpr (S::kInt8) {
+                        p[e] *= vsc[x][e >> 1];
+                        if (!all && t == -INFINITY) p[e] = 0.0f;
+                    }
                 }
 #pragma unroll
                 for (int pl = 0; pl < NPV; ++pl) {
-                    const uint32_t lo = pack_bf16(p[0], p[1]), hi = pack_bf16(p[2], p[3]);
+                    uint32_t lo, hi;
+                    if constexpr (S::kInt8) {
+                        lo = pack_f16(p[0], p[1]);
+                        hi = pack_f16(p[2], p[3]);
+                    } else {
+                        lo = pack_bf16(p[0], p[1]);
+                        hi = pack_bf16(p[2], p[3]);
+                    }
                     pb[nt][pl][0] = transpose8x8(lo);
                     pb[nt][pl][1] = transpose8x8(hi);
-                    p[0] -= bf16_lo(lo);
-                    p[1] -= bf16_hi(lo);
-                    p[2] -= bf16_lo(hi);
-                    p[3] -= bf16_hi(hi);
+                    if (pl + 1 == NPV) break;
+                    if constexpr (S::kInt8) {
+                        const float2 u = unpack_f16(lo), v = unpack_f16(hi);
+                        p[0] -= u.x;
+                        p[1] -= u.y;
+                        p[2] -= v.x;
+                        p[3] -= v.y;
+                    } else {
+                        p[0] -= bf16_lo(lo);
+                        p[1] -= bf16_hi(lo);
+                        p[2] -= bf16_lo(hi);
+                        p[3] -= bf16_hi(hi);
+                    }
                 }
             }
 #pragma unroll
@@ -324,10 +437,10 @@ __global__ void __launch_bounds__(kStepWarps * 32, 2) attend_step(const __grid_c
                     const int jj = 2 * t / S::EPL, z = 2 * t % S::EPL / 4, hi = t & 1;
                     const uint32_t *k0 = vr[x][0][jj], *k1 = vr[x][1][jj], *k2 = vr[x][2][jj], *k3 = vr[x][3][jj];
                     const uint32_t sel0 = hi ? 0x0602u : 0x0400u, sel1 = hi ? 0x0703u : 0x0501u;
-                    w[0] = s8x2_to_bf16x2(__byte_perm(k0[z], k1[z], sel0));
-                    w[1] = s8x2_to_bf16x2(__byte_perm(k0[z], k1[z], sel1));
-                    w[2] = s8x2_to_bf16x2(__byte_perm(k2[z], k3[z], sel0));
-                    w[3] = s8x2_to_bf16x2(__byte_perm(k2[z], k3[z], sel1));
+                    w[0] = s8x2_to_f16x2(__byte_perm(k0[z], k1[z], sel0));
+                    w[1] = s8x2_to_f16x2(__byte_perm(k0[z], k1[z], sel1));
+                    w[2] = s8x2_to_f16x2(__byte_perm(k2[z], k3[z], sel0));
+                    w[3] = s8x2_to_f16x2(__byte_perm(k2[z], k3[z], sel1));
                 } else {
                     const int jj = t / VP, z = t % VP;
                     w[0] = __byte_perm(vr[x][0][jj][z], vr[x][1][jj][z], 0x5410u);
@@ -339,7 +452,10 @@ __global__ void __launch_bounds__(kStepWarps * 32, 2) attend_step(const __grid_c
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int pl = 0; pl < NPV; ++pl)
-                        mma16816(o[nt][t], w[0], w[1], w[2], w[3], pb[nt][pl][0], pb[nt][pl][1]);
+                        if constexpr (S::kInt8)
+                            mma16816h(o[nt][t], w[0], w[1], w[2], w[3], pb[nt][pl][0], pb[nt][pl][1]);
+                        else
+                            mma16816(o[nt][t], w[0], w[1], w[2], w[3], pb[nt][pl][0], pb[nt][pl][1]);
             }
         }
         load_v();

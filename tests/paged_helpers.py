@@ -33,7 +33,8 @@ def sees(p, j, window, sinks):
     return (j <= p) & ((window == 0) | (j > p - window) | (j < sinks))
 
 
-def attention(q, k, v, tables, starts, counts, window=0, sinks=0, scale=None, bf16_weights=False, half_step=2.0**-24):
+def attention(q, k, v, tables, starts, counts, window=0, sinks=0, scale=None, bf16_weights=False, half_step=2.0**-24,
+              f16_weights=False):
     """(y, bound): attention over dequantised float64 pools [pages][kv][16][hd]
     for packed float64 queries, and how far a kernel may be from it.
 
@@ -47,7 +48,11 @@ def attention(q, k, v, tables, starts, counts, window=0, sinks=0, scale=None, bf
     denominator each carry that: w = 2 (max d + 4 u max|s - m| + 2^-21), to
     first order.  Weights kept as one bf16 number add 2^-8.  The sum over n
     keys, its rescaling (once a unit of keys) and the join of the parts add
-    (2 n + 16) u.  The result's own rounding is half_step |y|."""
+    (2 n + 16) u.  The result's own rounding is half_step |y|.
+    Over INT8 rows (`f16_weights`) a weight with its row's scale may be one
+    or two f16 numbers, taken so that the largest is at least 2^7: below
+    f16's normal numbers the spacing is 2^-24, so each is off by up to 2^-25,
+    which is 2^-32 of the largest, times up to 127 of its row."""
     T, H, hd = q.shape
     KV = k.shape[1]
     G = H // KV
@@ -72,6 +77,8 @@ def attention(q, k, v, tables, starts, counts, window=0, sinks=0, scale=None, bf
                 y[at + i, h] = w @ vv
                 rel = 2 * (d + 4 * u * np.max(m - t) + 2.0**-21) + (2 * len(seen) + 16) * u
                 rel += 2.0**-8 if bf16_weights else 0.0
-                bound[at + i, h] = 1.01 * rel * (w @ np.abs(vv)) + half_step * np.abs(y[at + i, h]) * 1.01 + 1e-37
+                if f16_weights:
+                    bound[at + i, h] += 2.0**-32 * len(seen) * np.max(w * np.abs(vv).max(-1))
+                bound[at + i, h] += 1.01 * rel * (w @ np.abs(vv)) + half_step * np.abs(y[at + i, h]) * 1.01 + 1e-37
         at += c
     return y, bound

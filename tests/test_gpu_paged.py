@@ -85,7 +85,7 @@ class Step:
     def want(self, scale=None):
         return ph.attention(self.rows[:, :self.heads].astype(np.float64), *self.host, self.tables, self.starts,
                             self.counts, self.window, self.sinks, scale, bf16_weights=self.values == "bf16",
-                            half_step=VALUES[self.values])
+                            half_step=VALUES[self.values], f16_weights=self.cache_dtype == "int8")
 
     def check(self, **kw):
         got = self.attend(**kw)
