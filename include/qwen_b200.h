@@ -278,7 +278,7 @@ typedef struct {
     size_t workspace_bytes;      /* DEVICE workspace of one attention call */
     uint32_t value_dtype, cache_dtype;
     uint32_t shared_rows;        /* nonzero: two new tokens may fall on one page, so the plan cannot write */
-    uint32_t small_kind, small_unit, tile_unit, small_items, tile_items, merges, merge_rows;
+    uint32_t small_kind, small_unit, tile_unit, small_items, tile_items, merges, merge_blocks;
     uint32_t off_seqs, off_slots, off_small, off_tile, off_merges;
 } qb_paged_plan;
 

@@ -149,7 +149,7 @@ class PagedPlanC(C.Structure):
     _fields_ = [(n, S) for n in ("sequences", "pages_per_sequence", "tokens", "pages", "query_heads",
                                  "kv_heads", "head_dim", "window", "sinks", "words", "workspace_bytes")] + \
                [(n, U32) for n in ("value_dtype", "cache_dtype", "shared_rows", "small_kind", "small_unit",
-                                   "tile_unit", "small_items", "tile_items", "merges", "merge_rows", "off_seqs", "off_slots", "off_small", "off_tile",
+                                   "tile_unit", "small_items", "tile_items", "merges", "merge_blocks", "off_seqs", "off_slots", "off_small", "off_tile",
                                    "off_merges")]
 
 

@@ -44,6 +44,8 @@ struct Merge {
 // A sequence goes to the step kernel up to kStepRows rows: with more, the
 // step kernel would read the cache more than once.
 constexpr int kStepRows = 16;
+// The merge kernel's warps a CTA, and the parts up to which one takes a row.
+constexpr int kMergeWarps = 4, kMergeFew = 8;
 
 struct Args {
     const int32_t *words;
@@ -58,6 +60,7 @@ struct Args {
     const uint8_t *k, *v;
     const float *ks, *vs;
     float *ws;
+    int dependent;        // launched behind another kernel of the same call
 };
 
 // Byte element types of values and caches.
@@ -77,6 +80,29 @@ __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+// The kernels of one call follow each other by programmatic dependent launch:
+// a kernel may start while the one before it still runs.  depend_wait waits
+// for everything before to be complete; a kernel that writes only its own
+// results calls it last, so that its own end means theirs too.
+__device__ __forceinline__ void depend_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void depend_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+template <typename... KArgs, typename... Args_>
+cudaError_t launch(void (*kernel)(KArgs...), dim3 grid, int threads, size_t smem, cudaStream_t st, bool dependent,
+                   const Args_ &...args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = dependent ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
 // Position p sees position j of its sequence.

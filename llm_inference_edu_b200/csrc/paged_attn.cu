@@ -13,26 +13,24 @@ constexpr int kRowsWarps = 4;
 // One CTA an item, its rows dealt to the warps.
 template <typename TV, typename TC>
 __global__ void __launch_bounds__(kRowsWarps * 32) attend_rows(const __grid_constant__ Args a) {
+    depend_trigger();
     const Item *it = (const Item *)(a.words + a.off_items + (size_t)blockIdx.x * 12);
     for (int r = threadIdx.x >> 5; r < it->rows; r += kRowsWarps) attend_row<TV, TC>(a, it, r, 64, threadIdx.x & 31);
 }
 
-// Joins the partial results of one row, one CTA a row: M = max m_z,
-// y = sum_z o_z 2^(m_z - M) / sum_z l_z 2^(m_z - M).  The parts are dealt to
-// the warps and the warps' sums added in order, so the result does not
-// depend on timing.  Bound by latency: every load of a warp's parts is
-// independent of the others.
-constexpr int kMergeWarps = 4;
+// Joins the partial results: M = max m_z, y = sum_z o_z 2^(m_z - M) /
+// sum_z l_z 2^(m_z - M).  Few parts: a warp a row, four rows a CTA.  Many
+// (kMergeFew): a CTA a row, the parts dealt to the warps and the warps' sums
+// added in order.  Either way the order is fixed, so the result does not
+// depend on timing.  Bound by latency (few rows) or by the parts' bytes; every load of
+// a warp's parts is independent of the others.
 
-template <typename TV, int V>  // V: dimensions a lane
-__global__ void __launch_bounds__(kMergeWarps * 32) merge_rows(const __grid_constant__ Args a) {
-    __shared__ float s_o[kMergeWarps][32 * V], s_l[kMergeWarps];
-    const Merge mg = *(const Merge *)(a.words + a.off_merges + (size_t)blockIdx.x * 8);
-    const int r = blockIdx.y;
-    if (r >= mg.rows) return;
-    const SeqRec sq = *(const SeqRec *)(a.words + a.off_seqs + mg.seq * 4);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, hd = a.hd;
-    const float *w = a.ws + mg.slot, *wm = w + (size_t)mg.rows * hd + r, *wl = wm + mg.rows;
+// Parts z0, z0 + dz, ... of row r: o (V dimensions a lane) and l against the
+// row's maximum, which is returned.
+template <int V>
+__device__ __forceinline__ void merge_parts(const float *w, const Merge &mg, int hd, int r, int z0, int dz, int lane, float (&o)[V],
+                                            float &l) {
+    const float *wm = w + (size_t)mg.rows * hd + r, *wl = wm + mg.rows;
     float m = -INFINITY;
     bool nan = false;
     for (int z = lane; z < mg.parts; z += 32) {
@@ -44,11 +42,11 @@ __global__ void __launch_bounds__(kMergeWarps * 32) merge_rows(const __grid_cons
     for (int off = 16; off; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
     if (__any_sync(0xffffffffu, nan)) m = __uint_as_float(0x7fffffffu);
     const float base = m == -INFINITY ? 0.0f : m;
-    float l = 0.0f, o[V];
+    l = 0.0f;
 #pragma unroll
     for (int i = 0; i < V; ++i) o[i] = 0.0f;
 #pragma unroll 4
-    for (int z = warp; z < mg.parts; z += kMergeWarps) {
+    for (int z = z0; z < mg.parts; z += dz) {
         const size_t at = (size_t)z * mg.stride;
         const float f = exp2f(wm[at] - base);
         l = fmaf(f, wl[at], l);
@@ -56,13 +54,40 @@ __global__ void __launch_bounds__(kMergeWarps * 32) merge_rows(const __grid_cons
         for (int i = 0; i < V; ++i)
             if (lane + 32 * i < hd) o[i] = fmaf(f, w[at + (size_t)r * hd + lane + 32 * i], o[i]);
     }
+}
+
+template <typename TV, int V>
+__global__ void __launch_bounds__(kMergeWarps * 32) merge_rows(const __grid_constant__ Args a) {
+    __shared__ float s_o[kMergeWarps][32 * V], s_l[kMergeWarps];
+    const Merge mg = *(const Merge *)(a.words + a.off_merges + (size_t)blockIdx.x * 8);
+    const bool few = mg.parts <= kMergeFew;
+    const int r0 = few ? blockIdx.y * kMergeWarps : blockIdx.y;
+    if (r0 >= mg.rows) return;  // (other CTAs of this grid wait for the parts)
+    const SeqRec sq = *(const SeqRec *)(a.words + a.off_seqs + mg.seq * 4);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, hd = a.hd;
+    depend_wait();
+    const float *w = a.ws + mg.slot;
+    auto out = [&](int r) {
+        const int row = mg.row0 + r;
+        return (TV *)a.y + (((size_t)sq.tok0 + row / a.G) * a.H + (size_t)mg.kvh * a.G + row % a.G) * hd;
+    };
+    float o[V], l;
+    if (few) {
+        const int r = r0 + warp;
+        if (r >= mg.rows) return;
+        merge_parts<V>(w, mg, hd, r, 0, 1, lane, o, l);
+        TV *y = out(r);
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (lane + 32 * i < hd) store_value(y, lane + 32 * i, __fdiv_rn(o[i], l));
+        return;
+    }
+    merge_parts<V>(w, mg, hd, r0, warp, kMergeWarps, lane, o, l);
 #pragma unroll
     for (int i = 0; i < V; ++i) s_o[warp][lane + 32 * i] = o[i];
     if (lane == 0) s_l[warp] = l;
     __syncthreads();
-    const int row = mg.row0 + r;
-    const size_t tok = (size_t)sq.tok0 + row / a.G, qh = (size_t)mg.kvh * a.G + row % a.G;
-    TV *y = (TV *)a.y + (tok * a.H + qh) * hd;
+    TV *y = out(r0);
     for (int d = threadIdx.x; d < hd; d += kMergeWarps * 32) {
         float v = 0.0f, ll = 0.0f;
 #pragma unroll
@@ -75,25 +100,15 @@ __global__ void __launch_bounds__(kMergeWarps * 32) merge_rows(const __grid_cons
 }
 
 template <typename TV>
-void launch_merge(const Args &a, int rows, cudaStream_t st) {
-    const dim3 grid(a.merges, rows);
-    if (a.hd <= 64)
-        merge_rows<TV, 2><<<grid, kMergeWarps * 32, 0, st>>>(a);
-    else if (a.hd <= 128)
-        merge_rows<TV, 4><<<grid, kMergeWarps * 32, 0, st>>>(a);
-    else
-        merge_rows<TV, 8><<<grid, kMergeWarps * 32, 0, st>>>(a);
+cudaError_t launch_merge(const Args &a, int blocks, cudaStream_t st) {
+    auto kern = a.hd <= 64 ? merge_rows<TV, 2> : a.hd <= 128 ? merge_rows<TV, 4> : merge_rows<TV, 8>;
+    return launch(kern, dim3(a.merges, blocks), kMergeWarps * 32, 0, st, true, a);
 }
 
 template <typename TV>
 uint32_t run_rows(const Args &a, uint32_t ct, cudaStream_t st) {
-    if (ct == QB_PAGED_F32)
-        attend_rows<TV, float><<<a.items, kRowsWarps * 32, 0, st>>>(a);
-    else if (ct == QB_PAGED_BF16)
-        attend_rows<TV, uint16_t><<<a.items, kRowsWarps * 32, 0, st>>>(a);
-    else
-        attend_rows<TV, int8_t><<<a.items, kRowsWarps * 32, 0, st>>>(a);
-    QB_CUDA(cudaGetLastError());
+    auto kern = ct == QB_PAGED_F32 ? attend_rows<TV, float> : ct == QB_PAGED_BF16 ? attend_rows<TV, uint16_t> : attend_rows<TV, int8_t>;
+    QB_CUDA(launch(kern, dim3(a.items), kRowsWarps * 32, 0, st, false, a));
     return QB_OK;
 }
 
@@ -147,27 +162,25 @@ uint32_t qb_paged_attention(const void *q, size_t q_len, size_t q_stride, const 
     a.ws = (float *)workspace;
     cudaStream_t st = (cudaStream_t)stream;
     const bool wide = plan->value_dtype == QB_PAGED_F32;
-    if (plan->small_items) {
-        a.off_items = plan->off_small;
-        a.items = (int)plan->small_items;
-        if (plan->small_kind)
-            s = cuda_status(step_attention(a, wide, (int)plan->cache_dtype, (int)plan->small_kind, st));
-        else
-            s = wide ? run_rows<float>(a, plan->cache_dtype, st) : run_rows<uint16_t>(a, plan->cache_dtype, st);
-        if (s) return s;
-    }
+    // The tile kernel first: the step kernel's CTAs fill the SMs as its
+    // last ones leave.  Both only read what was there before the call.
     if (plan->tile_items) {
         a.off_items = plan->off_tile;
         a.items = (int)plan->tile_items;
         QB_CUDA(tile_attention(a, wide, (int)plan->cache_dtype, plan->pages * plan->kv_heads * kPage, st));
     }
-    if (plan->merges) {
-        if (wide)
-            launch_merge<float>(a, (int)plan->merge_rows, st);
-        else
-            launch_merge<uint16_t>(a, (int)plan->merge_rows, st);
-        QB_CUDA(cudaGetLastError());
+    if (plan->small_items) {
+        a.off_items = plan->off_small;
+        a.items = (int)plan->small_items;
+        a.dependent = plan->tile_items != 0;
+        if (plan->small_kind)
+            QB_CUDA(step_attention(a, wide, (int)plan->cache_dtype, (int)plan->small_kind, st));
+        else if ((s = wide ? run_rows<float>(a, plan->cache_dtype, st) : run_rows<uint16_t>(a, plan->cache_dtype, st)))
+            return s;
     }
+    if (plan->merges)
+        QB_CUDA(wide ? launch_merge<float>(a, (int)plan->merge_blocks, st)
+                     : launch_merge<uint16_t>(a, (int)plan->merge_blocks, st));
     return QB_OK;
 }
 

@@ -27,12 +27,18 @@ struct Grid {
     int fixed;      // cost of starting an item
     int part;       // further cost of an item that leaves a partial result
     int least;      // fewest units worth an item of its own
+    int narrow, wide;  // a unit of a block of more than `narrow` rows costs `wide`
 };
 
 // The plain form of every variant: 8 rows and 64 keys a unit, one warp a row.
-Grid rows_grid() { return Grid{64, 8, 148 * 4, 1, 1, 2}; }
-Grid step_grid(int, int, bool) { return Grid{kPage, 8, 148 * 3, 16, 8, 32}; }
-Grid tile_grid(int, int, bool wide) { return Grid{wide ? 64 : 128, wide ? 128 : 256, 148, wide ? 4 : 3, 2, wide ? 4 : 2}; }
+Grid rows_grid() { return Grid{64, 8, 148 * 4, 1, 1, 2, 8, 1}; }
+// Step kernel: three CTAs an SM; a unit is a page.
+Grid step_grid() { return Grid{kPage, 8, 148 * 3, 4, 2, 32, 16, 1}; }
+// Tile kernel: one CTA an SM.  Starting an item and leaving a partial result
+// take about as long as two and one or two key tiles of 128 rows.
+Grid tile_grid(bool wide) {
+    return wide ? Grid{64, 128, 148, 4, 3, 4, 128, 1} : Grid{128, 256, 148, 4, 3, 2, 128, 2};
+}
 
 Block block_of(const qb_paged_step &s, const Grid &g, int seq, int kvh, int row0, int rows, int G) {
     Block b{seq, kvh, row0, rows, 0, 0, 0, 0, 0};
@@ -56,27 +62,60 @@ Block block_of(const qb_paged_step &s, const Grid &g, int seq, int kvh, int row0
     return b;
 }
 
-// The pieces a block of `units` falls into when none may be longer than T.
-inline int pieces_of(int units, int T) { return (units + T - 1) / T; }
+// A way to cut a list of blocks.
+enum Cut {
+    kWhole,   // not at all
+    kEven,    // each block into equal pieces of at most T units
+    kStream,  // all blocks in one row, cut every T units
+    kTail     // the last `slots` blocks (the shortest) into T pieces each
+};
+
+// The lengths of a block's pieces, appended to `out`.  `pos`: units in front
+// of the block (kStream); `tail`: one of the last blocks (kTail).
+void pieces_of(int units, const Grid &g, Cut how, int T, int64_t pos, bool tail, std::vector<int> &out) {
+    int n = 1;
+    if (how == kEven) n = (units + T - 1) / T;
+    if (how == kTail && tail) n = std::max(1, std::min(T, units / g.least));
+    if (how != kStream) {
+        for (int i = 0; i < n; ++i) out.push_back(units / n + (i < units % n));
+        return;
+    }
+    while (units > 0) {
+        int u = (int)(T - pos % T);
+        // No piece shorter than `least`: the first takes the next's share
+        // too, and a short rest goes with the last.
+        if (u < g.least) u += T;
+        if (u + g.least > units) u = units;
+        out.push_back(u);
+        units -= u;
+        pos += u;
+    }
+}
+
+inline int cost_of(const Block &b, const Grid &g, int units, bool part) {
+    const int w = b.rows > g.narrow ? g.wide : 1;
+    return units * w + g.fixed + (part ? g.part * w : 0);
+}
 
 // When every piece is done, with the longest started first on the first free
-// slot (what the hardware does with a grid in this order), in cost units.
-double makespan(const std::vector<Block> &bl, const Grid &g, int T, size_t *count) {
-    std::vector<int> cost;
-    double total = 0;
-    for (const Block &b : bl) {
-        const int n = pieces_of(b.units, T);
-        const int per = b.units / n, more = b.units % n;
-        for (int i = 0; i < n; ++i) {
-            cost.push_back(per + (i < more) + g.fixed + (n > 1 ? g.part : 0));
+// slot (what the hardware does with a grid in this order).
+double makespan(const std::vector<Block> &bl, const Grid &g, Cut how, int T) {
+    std::vector<int> cost, n;
+    int64_t total = 0, pos = 0;
+    for (size_t i = 0; i < bl.size(); ++i) {
+        n.clear();
+        pieces_of(bl[i].units, g, how, T, pos, i + g.slots >= bl.size(), n);
+        pos += bl[i].units;
+        for (int u : n) {
+            cost.push_back(cost_of(bl[i], g, u, n.size() > 1));
             total += cost.back();
         }
     }
-    *count = cost.size();
-    if (cost.empty()) return 0;
     std::sort(cost.begin(), cost.end(), std::greater<int>());
     if (cost.size() <= (size_t)g.slots) return cost[0];
-    if (cost.size() > 2048) return total / g.slots + cost[cost.size() - cost.size() / 8] ;
+    // Too many to follow one by one: the last wave is ragged by about a
+    // short piece.
+    if (cost.size() > 4096) return (double)total / g.slots + cost[cost.size() * 7 / 8];
     std::priority_queue<int64_t, std::vector<int64_t>, std::greater<int64_t>> free_at;
     int64_t last = 0;
     for (size_t i = 0; i < cost.size(); ++i) {
@@ -91,43 +130,56 @@ double makespan(const std::vector<Block> &bl, const Grid &g, int T, size_t *coun
     return (double)last;
 }
 
-// Cuts the blocks' units into items (longest first) and lists the merges.
-// Blocks stay whole unless that leaves SMs idle: the longest piece allowed
-// is the one of a few candidates whose simulated end comes first.
-void cut(const std::vector<Block> &bl, const Grid &g, int hd, int64_t &ws, std::vector<Item> &items,
+// Cuts the blocks' units into items (longest first) and lists the merges:
+// of a few candidate cuts the one whose simulated end comes first, whole
+// blocks if none is clearly better.
+void cut(std::vector<Block> &bl, const Grid &g, int hd, int64_t &ws, std::vector<Item> &items,
          std::vector<Merge> &merges) {
     if (bl.empty()) return;
+    std::stable_sort(bl.begin(), bl.end(), [&](const Block &a, const Block &b) {
+        return cost_of(a, g, a.units, false) > cost_of(b, g, b.units, false);
+    });
     int64_t total = 0;
-    int most = 1;
-    for (const Block &b : bl) {
-        total += b.units;
-        most = std::max(most, b.units);
-    }
-    size_t n;
-    int best = most;
-    double end = makespan(bl, g, most, &n);
-    // Whole blocks that fill the slots several times over end evenly anyway.
-    if (!(n >= 8 * (size_t)g.slots && (double)most < 0.25 * end)) {
-        for (double k : {1.0, 2.0, 3.0, 5.0}) {
-            const int T = std::max<int>(g.least, (int)ceil((double)total / (g.slots * k)));
-            if (T >= best) continue;
-            const double e = makespan(bl, g, T, &n);
+    for (const Block &b : bl) total += b.units;
+    Cut how = kWhole;
+    int T = 1;
+    double end = makespan(bl, g, kWhole, 1);
+    // Whole blocks that fill the slots many times over end evenly anyway.
+    if (bl.size() < 8 * (size_t)g.slots || (double)bl[0].units > 0.25 * end) {
+        auto consider = [&](Cut h, int t) {
+            const double e = makespan(bl, g, h, t);
             if (e < 0.97 * end) {
                 end = e;
-                best = T;
+                how = h;
+                T = t;
             }
+        };
+        int before = 0;
+        for (double k : {1.0, 1.25, 1.5, 2.0, 3.0, 4.0, 6.0}) {
+            const int t = std::max<int>(g.least, (int)ceil((double)total / (g.slots * k)));
+            if (t == before || t >= bl[0].units) continue;
+            before = t;
+            consider(kEven, t);
+            if (k <= 2.0) consider(kStream, t);
         }
+        if (bl.size() > (size_t)g.slots)
+            for (int t : {2, 3}) consider(kTail, t);
     }
-    for (const Block &b : bl) {
-        const int np = pieces_of(b.units, best);
-        const int per = b.units / np, more = b.units % np;
+    std::vector<int> n;
+    int64_t pos = 0;
+    for (size_t i = 0; i < bl.size(); ++i) {
+        const Block &b = bl[i];
+        n.clear();
+        pieces_of(b.units, g, how, T, pos, i + g.slots >= bl.size(), n);
+        pos += b.units;
+        const bool part = n.size() > 1;
         const int stride = b.rows * (hd + 2);
-        if (np > 1) merges.push_back(Merge{b.seq, b.kvh, b.row0, b.rows, (int32_t)ws, np, stride, 0});
-        for (int i = 0, at = 0; i < np; ++i) {
-            const int u = per + (i < more);
+        if (part) merges.push_back(Merge{b.seq, b.kvh, b.row0, b.rows, (int32_t)ws, (int32_t)n.size(), stride, 0});
+        int at = 0;
+        for (int u : n) {
             items.push_back(Item{b.seq, b.kvh, b.row0, b.rows, at, at + u, b.ns, b.u0, b.w0, b.hi,
-                                 np > 1 ? (int32_t)ws : -1, u});
-            if (np > 1) ws += stride;
+                                 part ? (int32_t)ws : -1, cost_of(b, g, u, part)});
+            if (part) ws += stride;
             at += u;
         }
     }
@@ -182,8 +234,8 @@ uint32_t build(const qb_paged_step &s, int32_t *words, size_t capacity, qb_paged
     const int G = (int)(s.query_heads / s.kv_heads), hd = (int)s.head_dim;
     const bool wide = s.value_dtype == QB_PAGED_F32;
     const bool fast = (hd == 64 || hd == 128) && s.cache_dtype != QB_PAGED_F32;
-    const Grid small = fast ? step_grid(hd, (int)s.cache_dtype, wide) : rows_grid();
-    const Grid tile = tile_grid(hd, (int)s.cache_dtype, wide);
+    const Grid small = fast ? step_grid() : rows_grid();
+    const Grid tile = tile_grid(wide);
     // Two n8 tiles a block only where some sequence of the list has use for them.
     int nt = 1;
     if (fast)
@@ -226,7 +278,8 @@ uint32_t build(const qb_paged_step &s, int32_t *words, size_t capacity, qb_paged
     p.small_items = (uint32_t)si.size();
     p.tile_items = (uint32_t)ti.size();
     p.merges = (uint32_t)merges.size();
-    for (const Merge &m : merges) p.merge_rows = std::max(p.merge_rows, (uint32_t)m.rows);
+    for (const Merge &m : merges)
+        p.merge_blocks = std::max(p.merge_blocks, (uint32_t)(m.parts > kMergeFew ? m.rows : (m.rows + kMergeWarps - 1) / kMergeWarps));
     // Records of 4 words and more start on 16 bytes.
     size_t at = 0;
     auto take = [&](size_t words_) {

@@ -119,6 +119,7 @@ __global__ void __launch_bounds__(kStepWarps * 32, 3) attend_step(const __grid_c
     __shared__ float s_m[kStepWarps][8 * NT], s_l[kStepWarps][8 * NT], s_c[8 * NT];
     uint2 *s_q = (uint2 *)s_raw;  // [plane][n tile][k-step][lane]
 
+    depend_trigger();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
     const Item *item = (const Item *)(a.words + a.off_items + (size_t)blockIdx.x * 12);
     const Item it = *item;
@@ -473,6 +474,7 @@ __global__ void __launch_bounds__(kStepWarps * 32, 3) attend_step(const __grid_c
             for (int e = 0; e < 4; ++e) bad |= !isfinite(o[nt][t][e]);
     if (__syncthreads_or(bad)) {
         for (int r = warp; r < it.rows; r += kStepWarps) attend_row<TV, TC>(a, item, r, kPage, lane);
+        if (a.dependent) depend_wait();
         return;
     }
 
@@ -528,15 +530,13 @@ __global__ void __launch_bounds__(kStepWarps * 32, 3) attend_step(const __grid_c
             a.ws[it.slot + (size_t)it.rows * (HD + 1) + r] = ll;
         }
     }
+    if (a.dependent) depend_wait();
 }
 
 template <typename TV, typename TC, int HD>
 cudaError_t launch_nt(const Args &a, int nt, cudaStream_t st) {
-    if (nt == 1)
-        attend_step<TV, TC, HD, 1><<<a.items, kStepWarps * 32, 0, st>>>(a);
-    else
-        attend_step<TV, TC, HD, 2><<<a.items, kStepWarps * 32, 0, st>>>(a);
-    return cudaGetLastError();
+    return launch(nt == 1 ? attend_step<TV, TC, HD, 1> : attend_step<TV, TC, HD, 2>, dim3(a.items), kStepWarps * 32, 0, st,
+                  a.dependent != 0, a);
 }
 
 template <typename TV>

@@ -393,6 +393,7 @@ __global__ void __launch_bounds__(Tile<TV, TC, HD>::kThreads, 1)
     __syncthreads();
     fence_after();
     const uint32_t tmem = ctl->tmem;
+    depend_trigger();
 
     // Loads every tile of one operand (BF16): a box a page (V) or a page's
     // panel (K).  A copy takes its warp about 110 cycles to issue, so K and V
@@ -993,7 +994,7 @@ bool encode_pool(CUtensorMap &m, const void *base, int hd, size_t rows, bool pan
 }
 
 template <typename TV, typename TC, int HD>
-cudaError_t launch(const Args &a, size_t pool_rows, cudaStream_t st) {
+cudaError_t launch_tile(const Args &a, size_t pool_rows, cudaStream_t st) {
     using T = Tile<TV, TC, HD>;
     // At least what keeps one CTA on an SM: an item takes all of its TMEM.
     const int smem = (int)(T::bytes > 120 * 1024 ? T::bytes : 120 * 1024);
@@ -1015,15 +1016,14 @@ cudaError_t launch(const Args &a, size_t pool_rows, cudaStream_t st) {
     alignas(64) CUtensorMap mk = {}, mv = {};
     if (!T::kInt8 && (!encode_pool(mk, a.k, HD, pool_rows, false) || !encode_pool(mv, a.v, HD, pool_rows, true)))
         return cudaErrorInvalidValue;
-    attend_tile<TV, TC, HD><<<a.items, T::kThreads, smem, st>>>(mk, mv, a);
-    return cudaGetLastError();
+    return paged::launch(attend_tile<TV, TC, HD>, dim3(a.items), T::kThreads, smem, st, false, mk, mv, a);
 }
 
 template <typename TV>
 cudaError_t launch_tv(const Args &a, int cache, size_t rows, cudaStream_t st) {
     if (cache == QB_PAGED_BF16)
-        return a.hd == 64 ? launch<TV, uint16_t, 64>(a, rows, st) : launch<TV, uint16_t, 128>(a, rows, st);
-    return a.hd == 64 ? launch<TV, int8_t, 64>(a, rows, st) : launch<TV, int8_t, 128>(a, rows, st);
+        return a.hd == 64 ? launch_tile<TV, uint16_t, 64>(a, rows, st) : launch_tile<TV, uint16_t, 128>(a, rows, st);
+    return a.hd == 64 ? launch_tile<TV, int8_t, 64>(a, rows, st) : launch_tile<TV, int8_t, 128>(a, rows, st);
 }
 
 }  // namespace
