@@ -67,15 +67,14 @@ enum Cut {
     kWhole,   // not at all
     kEven,    // each block into equal pieces of at most T units
     kStream,  // all blocks in one row, cut every T units
-    kTail     // the last `slots` blocks (the shortest) into T pieces each
+    kTail     // the last `tail` blocks (the shortest) into pieces of at most T units
 };
 
 // The lengths of a block's pieces, appended to `out`.  `pos`: units in front
 // of the block (kStream); `tail`: one of the last blocks (kTail).
 void pieces_of(int units, const Grid &g, Cut how, int T, int64_t pos, bool tail, std::vector<int> &out) {
     int n = 1;
-    if (how == kEven) n = (units + T - 1) / T;
-    if (how == kTail && tail) n = std::max(1, std::min(T, units / g.least));
+    if (how == kEven || (how == kTail && tail)) n = (units + T - 1) / T;
     if (how != kStream) {
         for (int i = 0; i < n; ++i) out.push_back(units / n + (i < units % n));
         return;
@@ -99,12 +98,12 @@ inline int cost_of(const Block &b, const Grid &g, int units, bool part) {
 
 // When every piece is done, with the longest started first on the first free
 // slot (what the hardware does with a grid in this order).
-double makespan(const std::vector<Block> &bl, const Grid &g, Cut how, int T) {
+double makespan(const std::vector<Block> &bl, const Grid &g, Cut how, int T, size_t tail) {
     std::vector<int> cost, n;
     int64_t total = 0, pos = 0;
     for (size_t i = 0; i < bl.size(); ++i) {
         n.clear();
-        pieces_of(bl[i].units, g, how, T, pos, i + g.slots >= bl.size(), n);
+        pieces_of(bl[i].units, g, how, T, pos, i + tail >= bl.size(), n);
         pos += bl[i].units;
         for (int u : n) {
             cost.push_back(cost_of(bl[i], g, u, n.size() > 1));
@@ -143,15 +142,17 @@ void cut(std::vector<Block> &bl, const Grid &g, int hd, int64_t &ws, std::vector
     for (const Block &b : bl) total += b.units;
     Cut how = kWhole;
     int T = 1;
-    double end = makespan(bl, g, kWhole, 1);
+    size_t tail = 0;
+    double end = makespan(bl, g, kWhole, 1, 0);
     // Whole blocks that fill the slots many times over end evenly anyway.
     if (bl.size() < 8 * (size_t)g.slots || (double)bl[0].units > 0.25 * end) {
-        auto consider = [&](Cut h, int t) {
-            const double e = makespan(bl, g, h, t);
-            if (e < 0.97 * end) {
+        auto consider = [&](Cut h, int t, size_t m) {
+            const double e = makespan(bl, g, h, t, m);
+            if (e < 0.98 * end) {
                 end = e;
                 how = h;
                 T = t;
+                tail = m;
             }
         };
         int before = 0;
@@ -159,18 +160,19 @@ void cut(std::vector<Block> &bl, const Grid &g, int hd, int64_t &ws, std::vector
             const int t = std::max<int>(g.least, (int)ceil((double)total / (g.slots * k)));
             if (t == before || t >= bl[0].units) continue;
             before = t;
-            consider(kEven, t);
-            if (k <= 2.0) consider(kStream, t);
+            consider(kEven, t, 0);
+            if (k <= 2.0) consider(kStream, t, 0);
         }
-        if (bl.size() > (size_t)g.slots)
-            for (int t : {2, 3}) consider(kTail, t);
+        // The blocks of the last, partly filled wave.
+        if (const size_t m = bl.size() % g.slots; m && bl.size() > (size_t)g.slots)
+            for (int t : {4, 8, 16}) consider(kTail, std::max(g.least, bl.back().units / t), m);
     }
     std::vector<int> n;
     int64_t pos = 0;
     for (size_t i = 0; i < bl.size(); ++i) {
         const Block &b = bl[i];
         n.clear();
-        pieces_of(b.units, g, how, T, pos, i + g.slots >= bl.size(), n);
+        pieces_of(b.units, g, how, T, pos, i + tail >= bl.size(), n);
         pos += b.units;
         const bool part = n.size() > 1;
         const int stride = b.rows * (hd + 2);

@@ -306,8 +306,8 @@ __global__ void __launch_bounds__(kStepWarps * 32, 3) attend_step(const __grid_c
                             mma16816(s[x][nt], w[0][0], w[1][0], w[0][1], w[1][1], b[pl][nt].x, b[pl][nt].y);
             }
         }
-        // t = score * log2(e), masked; this group's maximum, of t + log2 of
-        // the V row's scale for INT8.
+        // Scores, masked; this group's maximum of score * log2(e) (the row's
+        // factor c), with log2 of the V row's scale added for INT8.
         float bm[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) bm[nt][0] = bm[nt][1] = -INFINITY;
@@ -332,11 +332,10 @@ __global__ void __launch_bounds__(kStepWarps * 32, 3) attend_step(const __grid_c
                 for (int e = 0; e < 4; ++e) {
                     float t = s[x][nt][e];
                     if constexpr (S::kInt8) t *= kc[e >> 1];
-                    t *= cr[nt][e & 1];
                     if (!whole[x] && !(i + x < it.i1 && sees(pos[nt][e & 1], j0 + g + (e >> 1) * 8, a.window, a.sinks)))
                         t = -INFINITY;
                     s[x][nt][e] = t;
-                    bm[nt][e & 1] = fmaxf(bm[nt][e & 1], S::kInt8 ? t + lv[e >> 1] : t);
+                    bm[nt][e & 1] = fmaxf(bm[nt][e & 1], S::kInt8 ? fmaf(t, cr[nt][e & 1], lv[e >> 1]) : t * cr[nt][e & 1]);
                 }
             if (!S::kInt8 && !whole[x]) {
                 // V rows that no row sees may hold anything: 0 * inf is not
@@ -393,7 +392,9 @@ __global__ void __launch_bounds__(kStepWarps * 32, 3) attend_step(const __grid_c
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const float t = s[x][nt][e];
-                    p[e] = ex2(t - m[nt][e & 1]);
+                    // One rounding of the difference: score * c alone would
+                    // carry one of its own size.
+                    p[e] = ex2(fmaf(t, cr[nt][e & 1], -m[nt][e & 1]));
                     // Nothing seen so far leaves m at -inf; a hidden key's
                     // scale may be anything.
                     if (!all && t == -INFINITY) p[e] = 0.0f;

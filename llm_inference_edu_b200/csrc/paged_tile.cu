@@ -244,28 +244,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return d;
 }
 
-// 2^x on the FMA pipe, x <= 8: x = n + f with n the nearest integer (added
-// to and taken from 1.5 * 2^23, whose low bits it then is) and 2^f, |f| <=
-// 1/2, by the polynomial of degree 4 through 1 with the least largest
-// relative error (3e-6, a fraction of a bf16 weight's rounding); n goes into
-// the exponent.  -127 and below (a hidden key's -inf) give 0 exactly: f is 0
-// and the exponent of 1 is 127.  (A NaN is lost here: the row's sum has it.)
-__device__ __forceinline__ float2 ex2_poly(float2 x) {
-    x.x = fmaxf(x.x, -127.0f);
-    x.y = fmaxf(x.y, -127.0f);
-    const float big = 12582912.0f;
-    const float2 n = add2(x, make_float2(big, big));
-    const float2 f = fma2(add2(n, make_float2(-big, -big)), make_float2(-1.0f, -1.0f), x);
-    float2 y = make_float2(0.00958104711f, 0.00958104711f);
-    y = fma2(y, f, make_float2(0.0559059717f, 0.0559059717f));
-    y = fma2(y, f, make_float2(0.240241453f, 0.240241453f));
-    y = fma2(y, f, make_float2(0.693124354f, 0.693124354f));
-    y = fma2(y, f, make_float2(1.0f, 1.0f));
-    y.x = __uint_as_float(__float_as_uint(y.x) + (__float_as_uint(n.x) << 23));
-    y.y = __uint_as_float(__float_as_uint(y.y) + (__float_as_uint(n.y) << 23));
-    return y;
-}
-
 // Two parts of a row's softmax: maximum, sum, and the parts' factors.
 struct Join {
     float m, l, f0, f1;
@@ -598,15 +576,11 @@ __global__ void __launch_bounds__(Tile<TV, TC, HD>::kThreads, 1)
 #pragma unroll
                 for (int e = 0; e < CH / 2; ++e) {
                     p[e] = fma2(make_float2(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1])), c2, b2);
-                    // One weight in four by polynomial on the FMA pipe: the
-                    // special-function unit alone (16 a cycle) would take
-                    // longer than the tensor cores.
-                    if (NP == 1 && (e & 3) == 3) {
-                        p[e] = ex2_poly(p[e]);
-                    } else {
-                        p[e].x = ex2(p[e].x);
-                        p[e].y = ex2(p[e].y);
-                    }
+                    // (A quarter of them by polynomial on the FMA pipe made no
+                    // difference, half was slower: the special functions are
+                    // not what the tile waits for.)
+                    p[e].x = ex2(p[e].x);
+                    p[e].y = ex2(p[e].y);
                     l2[e & 1] = add2(l2[e & 1], p[e]);
                 }
                 if constexpr (T::kInt8) {
