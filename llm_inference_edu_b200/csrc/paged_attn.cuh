@@ -11,14 +11,44 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     return r;
 }
 
-// Two int8 values, in the low bytes of `t`'s halves (the high bytes are
-// ignored), as bf16, exactly: with the low 7 bits u as the mantissa of 128,
-// 128 + u - (128 or 256 by the sign bit) is the value.
-__device__ __forceinline__ uint32_t s8x2_to_bf16x2(uint32_t t) {
-    const uint32_t x = (t & 0x007f007fu) | 0x43004300u, y = (t & 0x00800080u) | 0x43004300u;
+// INT8 caches are widened to f16, which holds a byte exactly at one addition
+// a pair (1024 + 128 + q is the f16 with bits 0x6480 ^ q), and holds more of
+// Q and of the weights than bf16: two planes of an FP32 value to 2^-22, one
+// of a bf16 value exactly.  f16 lacks range.  So each row of Q is scaled by a
+// power of two to a largest element in 2^13 .. 2^14, and the weights, which
+// carry the V rows' scales, are taken against a base that keeps the largest
+// between 2^7 and 2^15: what f16 drops is below 2^-31 of it.  (V scales under
+// 2^-90 lose precision; where one over 2^90 overflows, the row is done again
+// by attend_row.)
+constexpr float kAboveBase = 7.0f, kScaleSpan = 90.0f;
+
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
     uint32_t r;
-    asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(y));
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
+}
+__device__ __forceinline__ float2 unpack_f16(uint32_t w) {
+    float2 r;
+    asm("{\n\t.reg .b16 x, y;\n\tmov.b32 {x, y}, %2;\n\tcvt.f32.f16 %0, x;\n\tcvt.f32.f16 %1, y;\n\t}"
+        : "=f"(r.x), "=f"(r.y)
+        : "r"(w));
+    return r;
+}
+// Two int8 values in the low bytes of t's halves as f16, exactly.
+__device__ __forceinline__ uint32_t s8x2_to_f16x2(uint32_t t) {
+    uint32_t r;
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"((t & 0x00ff00ffu) ^ 0x64806480u), "r"(0x64806480u));
+    return r;
+}
+__device__ __forceinline__ float lg2(float x) {
+    float y;
+    asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// The power of two for a row of Q whose largest magnitude has bits mb.
+__device__ __forceinline__ float row_scale(uint32_t mb) {
+    return __uint_as_float((267u - min(max(mb >> 23, 27u), 250u)) << 23);
 }
 
 // One CTA an item; nt: n8 tiles of an item's rows.

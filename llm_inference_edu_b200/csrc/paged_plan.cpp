@@ -36,8 +36,9 @@ Grid rows_grid() { return Grid{64, 8, 148 * 4, 1, 1, 2, 8, 1}; }
 Grid step_grid() { return Grid{kPage, 8, 148 * 3, 4, 2, 32, 16, 1}; }
 // Tile kernel: one CTA an SM.  Starting an item and leaving a partial result
 // take about as long as two and one or two key tiles of 128 rows.
-Grid tile_grid(bool wide) {
-    return wide ? Grid{64, 128, 148, 4, 3, 4, 128, 1} : Grid{128, 256, 148, 4, 3, 2, 128, 2};
+Grid tile_grid(bool wide, bool int8) {
+    if (wide && !int8) return Grid{64, 128, 148, 4, 3, 4, 128, 1};
+    return Grid{128, wide ? 128 : 256, 148, 4, 3, 2, 128, 2};
 }
 
 Block block_of(const qb_paged_step &s, const Grid &g, int seq, int kvh, int row0, int rows, int G) {
@@ -237,7 +238,7 @@ uint32_t build(const qb_paged_step &s, int32_t *words, size_t capacity, qb_paged
     const bool wide = s.value_dtype == QB_PAGED_F32;
     const bool fast = (hd == 64 || hd == 128) && s.cache_dtype != QB_PAGED_F32;
     const Grid small = fast ? step_grid() : rows_grid();
-    const Grid tile = tile_grid(wide);
+    const Grid tile = tile_grid(wide, s.cache_dtype == QB_PAGED_INT8);
     // Two n8 tiles a block only where some sequence of the list has use for them.
     int nt = 1;
     if (fast)

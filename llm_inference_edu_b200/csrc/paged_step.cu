@@ -18,17 +18,9 @@
 // weights (one would double the error of the result's own rounding, and the
 // products are not what this kernel waits for).
 //
-// INT8 caches.  What bounds them is the widening of the bytes on the integer
-// pipe, so they are widened to f16, a byte permute or mask and an addition a
-// pair (1024 + 128 + q is the f16 with bits 0x6480 ^ q; bf16 has too few
-// bits for that), and f16 holds more of Q and the weights: FP32 values take
-// two planes (2^-22), BF16 values one.  f16 lacks range, so each row of Q
-// is scaled by a power of two to a largest element near 2^13, and the
-// weights, which carry the V rows' scales, are taken against the running
-// maximum of score + log2(scale), 2^7 above it: they stay below 2^15 and
-// what f16 drops is below 2^-31 of the largest.  (Scales below 2^-90 lose
-// precision; above 2^90 the row goes the plain way.)  64 sequences of 100 to
-// 8,191 positions at the 7B shape: 52 us widened to bf16, STEP_US us so.
+// INT8 caches: what bounds them is the widening of the bytes on the integer
+// pipe, so they are widened to f16 (paged_attn.cuh).  64 sequences of 100 to
+// 8,191 positions at the 7B shape: 52 us widened to bf16, 48 us so.
 #include "paged_attn.cuh"
 
 namespace qb {
@@ -52,30 +44,6 @@ __device__ __forceinline__ void mma16816h(float (&d)[4], uint32_t a0, uint32_t a
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
-    uint32_t r;
-    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-    return r;
-}
-__device__ __forceinline__ float2 unpack_f16(uint32_t w) {
-    float2 r;
-    asm("{\n\t.reg .b16 x, y;\n\tmov.b32 {x, y}, %2;\n\tcvt.f32.f16 %0, x;\n\tcvt.f32.f16 %1, y;\n\t}"
-        : "=f"(r.x), "=f"(r.y)
-        : "r"(w));
-    return r;
-}
-// Two int8 values in the low bytes of t's halves as f16, exactly.
-__device__ __forceinline__ uint32_t s8x2_to_f16x2(uint32_t t) {
-    uint32_t r;
-    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"((t & 0x00ff00ffu) ^ 0x64806480u), "r"(0x64806480u));
-    return r;
-}
-__device__ __forceinline__ float lg2(float x) {
-    float y;
-    asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
     uint32_t y;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
@@ -96,7 +64,7 @@ struct StepShape {
     static constexpr bool kInt8 = sizeof(TC) == 1;
     static constexpr int NQ = sizeof(TV) == 4 ? (kInt8 ? 2 : 3) : 1;   // planes of Q
     static constexpr int NPV = sizeof(TV) == 4 ? (kInt8 ? 2 : 3) : kInt8 ? 1 : 2;  // planes of the weights
-    static constexpr float kAbove = kInt8 ? 7.0f : 0.0f;  // of the base the weights are taken against
+    static constexpr float kAbove = kInt8 ? kAboveBase : 0.0f;  // of the base the weights are taken against
     static constexpr int KS = HD / 16;                   // k-steps of the scores
     static constexpr int MT = HD / 16;                   // m16 tiles of O^T
     static constexpr int PG = 8192 / (2 * 16 * HD * (int)sizeof(TC));  // pages a warp holds: 8 KB of K and V
@@ -203,15 +171,12 @@ __global__ void __launch_bounds__(kStepWarps * 32, 3) attend_step(const __grid_c
             for (int x = 0; x < 4; ++x) v[x] = load_value(q, x);
         }
         if constexpr (S::kInt8) {
-            // The power of two that brings the row's largest element to
-            // 2^13 .. 2^14 (none for a row without a finite one).
             uint32_t mb = 0;
 #pragma unroll
             for (int x = 0; x < 4; ++x) mb = max(mb, __float_as_uint(v[x]) & 0x7fffffffu);
 #pragma unroll
             for (int off = 16; off; off >>= 1) mb = max(mb, __shfl_xor_sync(0xffffffffu, mb, off));
-            const uint32_t e = min(max(mb >> 23, 27u), 250u);
-            const float up = __uint_as_float((267u - e) << 23);
+            const float up = row_scale(mb);
 #pragma unroll
             for (int x = 0; x < 4; ++x) v[x] *= up;
             if (lane == 0) s_c[r] = __fdiv_rn(a.c, up);
@@ -275,37 +240,44 @@ __global__ void __launch_bounds__(kStepWarps * 32, 3) attend_step(const __grid_c
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) s[x][nt][e] = 0.0f;
+        // Small planes first: the tensor cores cut each sum to its own size,
+        // and only the last KS sums are of the score's.  (INT8 bytes are
+        // widened once for both planes.)
+        constexpr int kTurns = S::kInt8 ? 1 : NQ;
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-            uint2 b[NQ][NT];
+        for (int turn = kTurns - 1; turn >= 0; --turn)
 #pragma unroll
-            for (int pl = 0; pl < NQ; ++pl)
+            for (int ks = 0; ks < KS; ++ks) {
+                constexpr int here = NQ / kTurns;
+                uint2 b[here][NT];
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) b[pl][nt] = s_q[((pl * NT + nt) * KS + ks) * 32 + lane];
+                for (int pl = 0; pl < here; ++pl)
 #pragma unroll
-            for (int x = 0; x < PG; ++x) {
-                uint32_t w[2][2];
+                    for (int nt = 0; nt < NT; ++nt) b[pl][nt] = s_q[(((turn + pl) * NT + nt) * KS + ks) * 32 + lane];
 #pragma unroll
-                for (int y = 0; y < 2; ++y) {
-                    if constexpr (S::kInt8) {
-                        const uint32_t q4 = kr[x][y][ks / 4][ks % 4];
-                        w[y][0] = s8x2_to_f16x2(__byte_perm(q4, 0u, 0x4140u));
-                        w[y][1] = s8x2_to_f16x2(__byte_perm(q4, 0u, 0x4342u));
-                    } else {
-                        w[y][0] = kr[x][y][ks / 2][ks % 2 * 2];
-                        w[y][1] = kr[x][y][ks / 2][ks % 2 * 2 + 1];
+                for (int x = 0; x < PG; ++x) {
+                    uint32_t w[2][2];
+#pragma unroll
+                    for (int y = 0; y < 2; ++y) {
+                        if constexpr (S::kInt8) {
+                            const uint32_t q4 = kr[x][y][ks / 4][ks % 4];
+                            w[y][0] = s8x2_to_f16x2(__byte_perm(q4, 0u, 0x4140u));
+                            w[y][1] = s8x2_to_f16x2(__byte_perm(q4, 0u, 0x4342u));
+                        } else {
+                            w[y][0] = kr[x][y][ks / 2][ks % 2 * 2];
+                            w[y][1] = kr[x][y][ks / 2][ks % 2 * 2 + 1];
+                        }
                     }
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int pl = here - 1; pl >= 0; --pl)
+                            if constexpr (S::kInt8)
+                                mma16816h(s[x][nt], w[0][0], w[1][0], w[0][1], w[1][1], b[pl][nt].x, b[pl][nt].y);
+                            else
+                                mma16816(s[x][nt], w[0][0], w[1][0], w[0][1], w[1][1], b[pl][nt].x, b[pl][nt].y);
                 }
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                    for (int pl = 0; pl < NQ; ++pl)
-                        if constexpr (S::kInt8)
-                            mma16816h(s[x][nt], w[0][0], w[1][0], w[0][1], w[1][1], b[pl][nt].x, b[pl][nt].y);
-                        else
-                            mma16816(s[x][nt], w[0][0], w[1][0], w[0][1], w[1][1], b[pl][nt].x, b[pl][nt].y);
             }
-        }
         // Scores, masked; this group's maximum of score * log2(e) (the row's
         // factor c), with log2 of the V row's scale added for INT8.
         float bm[NT][2];
@@ -323,7 +295,7 @@ __global__ void __launch_bounds__(kStepWarps * 32, 3) attend_step(const __grid_c
 #pragma unroll
                 for (int y = 0; y < 2; ++y) {
                     kc[y] = ksc[x][y];
-                    lv[y] = fminf(fmaxf(lg2(fabsf(vsc[x][y])), -90.0f), 90.0f);
+                    lv[y] = fminf(fmaxf(lg2(fabsf(vsc[x][y])), -kScaleSpan), kScaleSpan);
                 }
             }
 #pragma unroll
@@ -453,7 +425,7 @@ __global__ void __launch_bounds__(kStepWarps * 32, 3) attend_step(const __grid_c
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                    for (int pl = 0; pl < NPV; ++pl)
+                    for (int pl = NPV - 1; pl >= 0; --pl)
                         if constexpr (S::kInt8)
                             mma16816h(o[nt][t], w[0], w[1], w[2], w[3], pb[nt][pl][0], pb[nt][pl][1]);
                         else

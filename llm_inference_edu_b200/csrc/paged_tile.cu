@@ -14,14 +14,16 @@
 // stream's warpgroup owns a row, finds the maximum (which may lag by 2^8, so
 // O is rarely rescaled), writes the weights back over S as the bf16 A
 // operand of O += P V, and keeps the row's sum in FP32.
-// FP32 values: Q and the weights are three bf16 planes (exact to 2^-24) and
-// a key tile has 64 keys, so that three planes fit beside S.
-// BF16 values: one plane each; the weights' single rounding (2^-9 of each at
+// BF16 caches.  FP32 values: Q and the weights are three bf16 planes (exact
+// to 2^-24) and a key tile has 64 keys, so that three planes fit beside S.
+// BF16 values: one plane each; the weights' single rounding (2^-8 of each at
 // most) is of the size of the result's own.
-// K tiles are K-major operands as TMA leaves them (128-byte swizzle, a box a
-// page); V tiles are the MN-major operand in the same layout.  INT8 pages
-// are copied raw and widened to bf16 by a warpgroup (exact); their scales
+// INT8 caches: pages are copied raw and widened to f16 by a warpgroup; two
+// planes of FP32 values, one of BF16 values (paged_attn.cuh).  Their scales
 // multiply scores and weights in the softmax.
+// FP32 values: each tile's product is gathered in FP32 by a warpgroup.
+// K tiles are K-major operands as TMA leaves them (128-byte swizzle, a box a
+// page); V tiles are the MN-major operand in the same layout.
 // Every wait is bounded: a role that gives up raises the abort flag, copies
 // and MMAs in flight are drained, TMEM is freed and the item's rows are NaN.
 #include <cuda.h>
@@ -42,39 +44,45 @@ template <typename TV, typename TC, int HD_>
 struct Tile {
     static constexpr bool kInt8 = sizeof(TC) == 1;
     static constexpr int HD = HD_;
-    static constexpr int NP = sizeof(TV) == 4 ? 3 : 1;  // planes of Q and of the weights
-    static constexpr int KT = NP == 1 ? 128 : 64;       // keys a tile
-    static constexpr int QT = NP == 1 ? 2 : 1;          // row tiles an item may have
+    static constexpr bool kWide = sizeof(TV) == 4;
+    static constexpr int NP = kWide ? (kInt8 ? 2 : 3) : 1;  // planes of Q and of the weights
+    static constexpr int KT = NP == 3 ? 64 : 128;           // keys a tile
+    static constexpr int QT = kWide ? 1 : 2;                // row tiles an item may have
     static constexpr int PN = HD / 64;                  // 64-element panels of a row
     static constexpr int kTileBytes = KT * HD * 2;
     static constexpr int kQBytes = QT * NP * PN * 128 * 128;
     // Operand stages of each ring, raw INT8 pieces of 64 keys, scale slots.
-    static constexpr int NS = kTileBytes == 32768 ? 2 : NP == 3 && HD == 128 ? 3 : 4;
+    static constexpr int NS = kTileBytes == 32768 ? 2 : kWide && HD == 128 ? 3 : 4;
     static constexpr int kPiece = 64 * HD;
     static constexpr int RS = kInt8 ? (HD == 128 ? 3 : 4) : 0;
     static constexpr int D = kInt8 ? 4 : 0;
     // Warps: 8 softmax, K producer, MMA issuer, scale producer, TMEM and V producer;
     // 4 that gather O (FP32 values); 4 INT8 converters.
-    static constexpr int kGather = 12, kConvert = NP == 3 ? 16 : 12;
-    static constexpr int kThreads = 384 + (NP == 3 ? 128 : 0) + (kInt8 ? 128 : 0);
+    static constexpr int kGather = 12, kConvert = kWide ? 16 : 12;
+    static constexpr int kThreads = 384 + (kWide ? 128 : 0) + (kInt8 ? 128 : 0);
     // The launch's registers, split among the roles: the softmax holds its
     // scores (BF16 caches) and the gathering warps O.
     static constexpr int kLaunchRegs = 65536 / kThreads / 8 * 8;
-    static constexpr int kSoftRegs = NP == 3 ? (kInt8 ? 112 : 120) : kInt8 ? 168 : 216, kGatherRegs = kInt8 ? 168 : 176,
-                         kOtherRegs = NP == 3 ? (kInt8 ? 40 : 88) : kInt8 ? 88 : 72;
-    static_assert(256 * kSoftRegs + (NP == 3 ? 128 * kGatherRegs : 0) + (kThreads - (NP == 3 ? 384 : 256)) * kOtherRegs <=
+    static constexpr int kSoftRegs = kWide ? (kInt8 ? 112 : 120) : kInt8 ? 168 : 216, kGatherRegs = kInt8 ? 168 : 176,
+                         kOtherRegs = kWide ? (kInt8 ? 40 : 88) : kInt8 ? 88 : 72;
+    static_assert(256 * kSoftRegs + (kWide ? 128 * kGatherRegs : 0) + (kThreads - (kWide ? 384 : 256)) * kOtherRegs <=
                       kThreads * kLaunchRegs,
                   "register split");
-    // Columns of a stream: scores from 0 (KT of them), plane 0 of the weights
-    // over the scores that were read already, planes 1 and 2 behind them
-    // (FP32 values only: 64 scores), O from 128.
-    static __host__ __device__ constexpr int plane_col(int pl) { return pl == 0 ? 0 : 32 + 32 * pl; }
+    // Columns of a stream: scores from 0 (KT of them), O from 128.  The
+    // weights' operand starts over the scores.  Up to two planes: chunk ch of
+    // 32 scores leaves 16 columns a plane where it was or before.  Three
+    // planes (64 scores, all read before): 1 and 2 from column 64.
+    static __host__ __device__ constexpr int chunk_col(int pl, int ch) {
+        return NP == 3 ? (pl == 0 ? 0 : 32 + 32 * pl) + 16 * ch : 16 * (NP * ch + pl);
+    }
+    static __host__ __device__ constexpr int plane_col(int pl, int kb) { return chunk_col(pl, kb / 2) + kb % 2 * 8; }
     // Scores held between the maximum and the weights, where they fit.
-    static constexpr bool kHold = NP == 3 || !kInt8;
+    static constexpr bool kHold = !kInt8;
+    static constexpr float kAbove = kInt8 ? kAboveBase : 0.0f;  // of the base the weights are taken against
     static constexpr size_t kv_off = kQBytes, raw_off = kv_off + (size_t)2 * NS * kTileBytes,
                             scl_off = raw_off + (size_t)RS * kPiece, max_off = scl_off + (size_t)D * 2 * KT * 4,
-                            ctl_off = max_off + (NP == 3 ? 2048 : 0);
-    static constexpr size_t bytes = ctl_off + 1024 + 1024;
+                            ctl_off = max_off + (kWide ? 2048 : 0);
+    static constexpr size_t bytes = ctl_off + 2048 + 1024;
     static_assert(bytes <= 232448, "shared memory of a CTA");
 };
 
@@ -87,8 +95,9 @@ struct Ctl {
     uint32_t tmem;
     int abort_;
     uint8_t bad[256];
+    float c[256];  // scale * log2(e) over the row's own scale (INT8 caches)
 };
-static_assert(sizeof(Ctl) <= 1024, "control block");
+static_assert(sizeof(Ctl) <= 2048, "control block");
 
 __device__ __forceinline__ bool wait_slow(uint64_t *bar, uint32_t parity, volatile int *abort_) {
     const uint64_t t0 = globaltimer_ns();
@@ -206,9 +215,9 @@ __device__ __forceinline__ uint64_t desc_mn(uint32_t saddr, uint32_t panel) {
     return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)(panel >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
            ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
-// BF16 operands, FP32 result, M = 128; b_mn: B is MN-major.
-__host__ __device__ constexpr uint32_t idesc(int n, bool b_mn) {
-    return (1u << 4) | (1u << 7) | (1u << 10) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | (8u << 24);
+// BF16 or f16 operands, FP32 result, M = 128; b_mn: B is MN-major.
+__host__ __device__ constexpr uint32_t idesc(int n, bool b_mn, bool f16) {
+    return (1u << 4) | (f16 ? 0u : (1u << 7) | (1u << 10)) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | (8u << 24);
 }
 
 // (a0, a1) * (b0, b1) + (c0, c1) in one instruction.
@@ -434,7 +443,7 @@ __global__ void __launch_bounds__(Tile<TV, TC, HD>::kThreads, 1)
                     const TV *q = (const TV *)a.q + (size_t)(sq.tok0 + row / a.G) * a.q_stride +
                                   (size_t)(it.kvh * a.G + row % a.G) * HD + ch * 8;
                     if (vec) {
-                        if constexpr (NP == 3) {
+                        if constexpr (T::kWide) {
                             const float4 x = *(const float4 *)q, y = *(const float4 *)(q + 4);
                             v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
                             v[4] = y.x; v[5] = y.y; v[6] = y.z; v[7] = y.w;
@@ -449,19 +458,39 @@ __global__ void __launch_bounds__(Tile<TV, TC, HD>::kThreads, 1)
                     }
                 }
                 const int rr = r & 127;
+                if constexpr (T::kInt8) {
+                    // The row's HD / 8 pieces are neighbouring lanes.
+                    uint32_t mb = 0;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) mb = max(mb, __float_as_uint(v[e]) & 0x7fffffffu);
+#pragma unroll
+                    for (int off = HD / 16; off; off >>= 1) mb = max(mb, __shfl_xor_sync(0xffffffffu, mb, off));
+                    const float up = row_scale(mb);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[e] *= up;
+                    if (ch == 0) ctl->c[r] = __fdiv_rn(a.c, up);
+                }
 #pragma unroll
                 for (int pl = 0; pl < NP; ++pl) {
                     uint32_t w[4];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        w[e] = pack_bf16(v[2 * e], v[2 * e + 1]);
-                        v[2 * e] -= bf16_lo(w[e]);
-                        v[2 * e + 1] -= bf16_hi(w[e]);
+                        if constexpr (T::kInt8) {
+                            w[e] = pack_f16(v[2 * e], v[2 * e + 1]);
+                            const float2 x = unpack_f16(w[e]);
+                            v[2 * e] -= x.x;
+                            v[2 * e + 1] -= x.y;
+                        } else {
+                            w[e] = pack_bf16(v[2 * e], v[2 * e + 1]);
+                            v[2 * e] -= bf16_lo(w[e]);
+                            v[2 * e + 1] -= bf16_hi(w[e]);
+                        }
                     }
                     uint8_t *dst = s_q + ((r >> 7) * PN + pl * PN + ch / 8) * 16384 + rr * 128 + (((ch & 7) ^ (rr & 7)) << 4);
                     *(uint4 *)dst = make_uint4(w[0], w[1], w[2], w[3]);
                 }
             }
+            if (T::kInt8) asm volatile("bar.sync 2, 256;" ::: "memory");
             fence_proxy_async_smem();
             mbar_arrive(&ctl->q_full);
         }
@@ -474,7 +503,7 @@ __global__ void __launch_bounds__(Tile<TV, TC, HD>::kThreads, 1)
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t ts = tmem + s * 256 + lanes, to = ts + 128;
         const int n_steps = shared ? nk : (nk - s + 1) / 2;
-        const float c = a.c;
+        const float c = T::kInt8 ? ctl->c[r] : a.c;
         float m = -INFINITY;   // in units of log2
         float2 l2[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
         bool ok = true;
@@ -544,12 +573,22 @@ __global__ void __launch_bounds__(Tile<TV, TC, HD>::kThreads, 1)
             bm *= c;
             // A NaN among the visible scores is the row's result.
             if (bm != bm) l2[0].x = bm;
-            if (__any_sync(0xffffffffu, bm > m + 8.0f)) {
-                const float mn = fmaxf(m, bm), f = m == mn ? 1.0f : ex2(m - mn);
+            if constexpr (T::kInt8) {
+                // The weights carry the V scales: at most the tile's largest.
+                float vm = 0.0f;
+#pragma unroll
+                for (int e = 0; e < KT; e += 32)
+                    if (!none(j0 + e + lane)) vm = fmaxf(vm, fabsf(vs[e + lane]));
+#pragma unroll
+                for (int off = 16; off; off >>= 1) vm = fmaxf(vm, __shfl_xor_sync(0xffffffffu, vm, off));
+                bm += fminf(fmaxf(lg2(vm), -kScaleSpan), kScaleSpan);
+            }
+            if (__any_sync(0xffffffffu, bm > m + (8.0f + T::kAbove))) {
+                const float mn = fmaxf(m, bm - T::kAbove), f = m == mn ? 1.0f : ex2(m - mn);
                 m = mn;
 #pragma unroll
                 for (int e = 0; e < 2; ++e) l2[e] = mul2(l2[e], make_float2(f, f));
-                if (NP == 1 && n > 0) {
+                if (!T::kWide && n > 0) {
 #pragma unroll 1
                     for (int d = 0; d < HD; d += 16) {
                         uint32_t x[16];
@@ -561,7 +600,7 @@ __global__ void __launch_bounds__(Tile<TV, TC, HD>::kThreads, 1)
                     }
                 }
             }
-            if constexpr (NP == 3) s_max[(s * 2 + (n & 1)) * 128 + r_in] = m;
+            if constexpr (T::kWide) s_max[(s * 2 + (n & 1)) * 128 + r_in] = m;
             const float base = m == -INFINITY ? 0.0f : m;
             const float2 c2 = make_float2(c, c), b2 = make_float2(-base, -base);
 #pragma unroll
@@ -605,7 +644,13 @@ __global__ void __launch_bounds__(Tile<TV, TC, HD>::kThreads, 1)
                     uint32_t w[CH / 2];
 #pragma unroll
                     for (int e = 0; e < CH / 2; ++e) {
-                        if constexpr (NP == 1) {
+                        if constexpr (T::kInt8) {
+                            w[e] = pack_f16(p[e].x, p[e].y);
+                            if (pl + 1 < NP) {
+                                const float2 x = unpack_f16(w[e]);
+                                p[e] = add2(p[e], make_float2(-x.x, -x.y));
+                            }
+                        } else if constexpr (NP == 1) {
                             w[e] = pack_bf16(p[e].x, p[e].y);
                         } else {
                             // Planes by truncation: 8 bits of the significand
@@ -617,7 +662,7 @@ __global__ void __launch_bounds__(Tile<TV, TC, HD>::kThreads, 1)
                                             make_float2(-1.0f, -1.0f), p[e]);
                         }
                     }
-                    tmem_st16(ts + T::plane_col(pl) + ch * (CH / 2), w);
+                    tmem_st16(ts + T::chunk_col(pl, ch), w);
                 }
                 if (ch == KT / CH / 2 - 1 || ch == KT / CH - 1) {
                     wait_st();
@@ -640,7 +685,7 @@ __global__ void __launch_bounds__(Tile<TV, TC, HD>::kThreads, 1)
         if (!shared) {
             s_ml[s * 256 + r_in] = m;
             s_ml[s * 256 + 128 + r_in] = fin ? l : __uint_as_float(0x7fffffffu);
-            if (NP == 1 && s == 1 && nk > 1) {
+            if (!T::kWide && s == 1 && nk > 1) {
 #pragma unroll 1
                 for (int d = 0; d < HD; d += 32) {
                     uint32_t x[32];
@@ -651,9 +696,9 @@ __global__ void __launch_bounds__(Tile<TV, TC, HD>::kThreads, 1)
                         *(uint4 *)(s_o + r_in * (HD + 4) + d + e) = make_uint4(x[e], x[e + 1], x[e + 2], x[e + 3]);
                 }
             }
-            asm volatile("bar.sync 1, %0;" ::"n"(NP == 3 ? 384 : 256) : "memory");
+            asm volatile("bar.sync 1, %0;" ::"n"(T::kWide ? 384 : 256) : "memory");
         }
-        if (NP == 1 && (shared || s == 0)) {
+        if (!T::kWide && (shared || s == 0)) {
             Join j = {m, l, 1.0f, 0.0f};
             if (!shared && nk > 1) j = join(m, l, s_ml[256 + r_in], s_ml[384 + r_in]);
             bool bad = false;
@@ -673,12 +718,12 @@ __global__ void __launch_bounds__(Tile<TV, TC, HD>::kThreads, 1)
             }
             if (bad && fin && r < it.rows) ctl->bad[r] = 1;
         }
-    } else if (NP == 3 && warp >= T::kGather && warp < T::kGather + 4) {
+    } else if (T::kWide && warp >= T::kGather && warp < T::kGather + 4) {
         // O of both streams, in registers.  Each tile's product starts from
         // zero and is added here: the tensor cores cut their sums instead of
         // rounding them, and over a long row that adds up (5e-6 of the result
         // at 3,000 keys).
-        if constexpr (NP == 3) {
+        if constexpr (T::kWide) {
             asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(T::kGatherRegs));
             const int r = (warp & 3) * 32 + lane;
             const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
@@ -769,7 +814,7 @@ __global__ void __launch_bounds__(Tile<TV, TC, HD>::kThreads, 1)
                 for (int y = z > RS ? z - RS : 0; y < z; ++y) wait_issued(&ctl->raw_full[y % RS], (uint32_t)((y / RS) & 1));
             }
         } else if (warp == 9) {
-            constexpr uint32_t is = idesc(KT, false), io = idesc(HD, true);
+            constexpr uint32_t is = idesc(KT, false, T::kInt8), io = idesc(HD, true, T::kInt8);
             const uint32_t leader = elect_one();
             const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
             const bool two = __shfl_sync(0xffffffffu, it.rows, 0) > 128;
@@ -822,7 +867,7 @@ __global__ void __launch_bounds__(Tile<TV, TC, HD>::kThreads, 1)
                     }
                 }
                 if (t + 2 < total && !k_ready(t + 2)) break;
-                if (NP == 3 && t > 1 && !await(&ctl->o_empty[s], (uint32_t)(((t >> 1) - 1) & 1))) break;
+                if (T::kWide && t > 1 && !await(&ctl->o_empty[s], (uint32_t)(((t >> 1) - 1) & 1))) break;
                 const uint32_t v = v_at + st * T::kTileBytes;
                 // The first half of the keys while the second's weights are
                 // still being computed.
@@ -834,12 +879,12 @@ __global__ void __launch_bounds__(Tile<TV, TC, HD>::kThreads, 1)
                     for (int pl = NP - 1; pl >= 0; --pl)
 #pragma unroll
                         for (int kb = h * (KT / 32); kb < (h + 1) * (KT / 32); ++kb)
-                            mma_ts(tm + s * 256 + 128, tm + s * 256 + T::plane_col(pl) + kb * 8,
+                            mma_ts(tm + s * 256 + 128, tm + s * 256 + T::plane_col(pl, kb),
                                    desc_mn(v + kb * (PN * 2048), 2048), io,
-                                   (NP == 1 && t > 1) || h || pl != NP - 1 || kb != 0, leader);
+                                   (!T::kWide && t > 1) || h || pl != NP - 1 || kb != 0, leader);
                 }
                 if (!ok) break;
-                if (NP == 3) commit(&ctl->o_full[s], leader);
+                if (T::kWide) commit(&ctl->o_full[s], leader);
                 if (!two || s == 1) commit(&ctl->v_empty[st], leader);
                 if (t + 2 < total) scores(t + 2);
             }
@@ -876,7 +921,7 @@ __global__ void __launch_bounds__(Tile<TV, TC, HD>::kThreads, 1)
             if constexpr (!T::kInt8) produce(false);
         } else if (warp >= T::kConvert) {
             if constexpr (T::kInt8) {
-                // INT8 -> bf16 (exact), 64 keys a piece, into the operand layout.
+                // INT8 -> f16 (exact), 64 keys a piece, into the operand layout.
                 constexpr int per = KT / 64, units = T::kPiece / 16 / 128;
                 const int ct = threadIdx.x - T::kConvert * 32;
                 // Unit u of this thread: 16 values of key u * step + key_t.
@@ -906,14 +951,14 @@ __global__ void __launch_bounds__(Tile<TV, TC, HD>::kThreads, 1)
 #pragma unroll
                     for (int u = 0; u < units; ++u) {
                         uint4 o0, o1;
-                        o0.x = s8x2_to_bf16x2(__byte_perm(w[u].x, 0u, 0x4140u));
-                        o0.y = s8x2_to_bf16x2(__byte_perm(w[u].x, 0u, 0x4342u));
-                        o0.z = s8x2_to_bf16x2(__byte_perm(w[u].y, 0u, 0x4140u));
-                        o0.w = s8x2_to_bf16x2(__byte_perm(w[u].y, 0u, 0x4342u));
-                        o1.x = s8x2_to_bf16x2(__byte_perm(w[u].z, 0u, 0x4140u));
-                        o1.y = s8x2_to_bf16x2(__byte_perm(w[u].z, 0u, 0x4342u));
-                        o1.z = s8x2_to_bf16x2(__byte_perm(w[u].w, 0u, 0x4140u));
-                        o1.w = s8x2_to_bf16x2(__byte_perm(w[u].w, 0u, 0x4342u));
+                        o0.x = s8x2_to_f16x2(__byte_perm(w[u].x, 0u, 0x4140u));
+                        o0.y = s8x2_to_f16x2(__byte_perm(w[u].x, 0u, 0x4342u));
+                        o0.z = s8x2_to_f16x2(__byte_perm(w[u].y, 0u, 0x4140u));
+                        o0.w = s8x2_to_f16x2(__byte_perm(w[u].y, 0u, 0x4342u));
+                        o1.x = s8x2_to_f16x2(__byte_perm(w[u].z, 0u, 0x4140u));
+                        o1.y = s8x2_to_f16x2(__byte_perm(w[u].z, 0u, 0x4342u));
+                        o1.z = s8x2_to_f16x2(__byte_perm(w[u].w, 0u, 0x4140u));
+                        o1.w = s8x2_to_f16x2(__byte_perm(w[u].w, 0u, 0x4342u));
                         uint8_t *r = dst + (is_k ? at_k + u * (step * 128) : at_v + u * (step / kPage * PN * kPage * 128));
                         *(uint4 *)(r + ((c0 ^ sw) << 4)) = o0;
                         *(uint4 *)(r + (((c0 + 1) ^ sw) << 4)) = o1;
