@@ -317,8 +317,8 @@ def _paged_plan_words(tables, starts, counts, pages, kv_heads, head_dim, query_h
     if tables.ndim != 2 or starts.shape != tables.shape[:1] or counts.shape != starts.shape:
         raise ValueError("tables must be [sequences][pages], starts and counts [sequences]")
     for name, x in (("window", window), ("sinks", sinks)):
-        if x < 0:
-            raise ValueError(f"{name} must not be negative")
+        if not 0 <= x < 2**63:
+            raise ValueError(f"{name} must be in 0 .. 2**63 - 1")
     step = _lib.PagedStepC(tables.ctypes.data, starts.ctypes.data, counts.ctypes.data, tables.shape[0],
                            tables.shape[1], pages, kv_heads, head_dim, query_heads, window, sinks,
                            PAGED_DTYPES[value_dtype], PAGED_DTYPES[cache_dtype])

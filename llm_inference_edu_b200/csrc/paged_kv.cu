@@ -329,6 +329,19 @@ uint32_t admit_rows(size_t buffer, size_t len, size_t stride, size_t width, size
     return QB_OK;
 }
 
+// Whether two sets of rows (`tokens` rows of `width` elements of `size`
+// bytes, `stride` elements apart) share memory.  Rows of one buffer with the
+// same stride may lie side by side; with other strides any overlap of the
+// whole ranges counts.
+bool rows_meet(const void *p, size_t p_stride, const void *q, size_t q_stride, size_t width, size_t tokens, size_t size) {
+    const uintptr_t a = (uintptr_t)p, b = (uintptr_t)q;
+    const uintptr_t a_end = a + ((tokens - 1) * p_stride + width) * size, b_end = b + ((tokens - 1) * q_stride + width) * size;
+    if (a >= b_end || b >= a_end) return false;
+    if (tokens == 1 || p_stride != q_stride) return true;
+    const size_t step = p_stride * size, off = (a > b ? a - b : b - a) % step, w = width * size;
+    return off < w || step - off < w;
+}
+
 }  // namespace paged
 }  // namespace qb
 
@@ -362,6 +375,8 @@ uint32_t qb_kv_read(const qb_paged_cache *cache, const qb_paged_plan *plan, cons
     if ((s = admit_rows(0, k_len, k_stride, width, plan->tokens))) return s;
     if ((s = admit_rows(1, v_len, v_stride, width, plan->tokens))) return s;
     if (!k || !v) return QB_INVALID_PARAMETERS;
+    const size_t size = plan->value_dtype == QB_PAGED_F32 ? 4 : 2;
+    if (rows_meet(k, k_stride, v, v_stride, width, plan->tokens, size)) return QB_INVALID_PARAMETERS;
     RowArgs a{words + plan->off_slots, plan->tokens * plan->kv_heads, (int)plan->kv_heads, (int)plan->head_dim,
               {nullptr, nullptr}, {k, v}, {k_stride, v_stride}, {cache->k, cache->v},
               {cache->k_scales, cache->v_scales}};

@@ -52,7 +52,9 @@ def attention(q, k, v, tables, starts, counts, window=0, sinks=0, scale=None, bf
     Over INT8 rows (`f16_weights`) a weight with its row's scale may be one
     or two f16 numbers, taken so that the largest is at least 2^7: below
     f16's normal numbers the spacing is 2^-24, so each is off by up to 2^-25,
-    which is 2^-32 of the largest, times up to 127 of its row."""
+    which is 2^-32 of the largest, times up to 127 of its row.  V scales below
+    2^-90 are not made up for: the largest is then smaller by their ratio to
+    2^-90, and the same 2^-25 is that much more of it."""
     T, H, hd = q.shape
     KV = k.shape[1]
     G = H // KV
@@ -78,7 +80,8 @@ def attention(q, k, v, tables, starts, counts, window=0, sinks=0, scale=None, bf
                 rel = 2 * (d + 4 * u * np.max(m - t) + 2.0**-21) + (2 * len(seen) + 16) * u
                 rel += 2.0**-8 if bf16_weights else 0.0
                 if f16_weights:
-                    bound[at + i, h] += 2.0**-32 * len(seen) * np.max(w * np.abs(vv).max(-1))
+                    small = max(1.0, 2.0**-90 / max(np.abs(vv).max() / 127, 1e-300))
+                    bound[at + i, h] += 2.0**-32 * small * len(seen) * np.max(w * np.abs(vv).max(-1))
                 bound[at + i, h] += 1.01 * rel * (w @ np.abs(vv)) + half_step * np.abs(y[at + i, h]) * 1.01 + 1e-37
         at += c
     return y, bound

@@ -324,6 +324,51 @@ def test_large_scores(values, cache, hd):
     s.check()
 
 
+@pytest.mark.parametrize("values,cache", [("f32", "bf16"), ("bf16", "int8"), ("f32", "int8"), ("bf16", "bf16"), ("f32", "f32")])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_queries_that_are_not_finite(values, cache, hd):
+    """A NaN or infinity in a query makes that head's row NaN and no other."""
+    s = Step([100, 5, 40], [1, 3, 60], 14, 2, hd, values, cache, seed=6)
+    want, bound = s.want()
+    spoiled = np.zeros(want.shape[:2], bool)
+    for t, h, d, x in ((0, 3, 0, np.nan), (2, 0, 5, np.inf), (30, 13, hd - 1, -np.inf), (63, 7, 1, np.nan)):
+        s.q[t, h, d] = x
+        spoiled[t, h] = True
+    got = s.attend()
+    assert np.isnan(got[spoiled]).all()
+    assert (np.abs(got - want) <= bound)[~spoiled].all()
+
+
+@pytest.mark.parametrize("values", ["f32", "bf16"])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("up", [1e-30, 1e-12, 1e12, 1e25])
+def test_sizes_of_quantised_rows(values, hd, up):
+    """Queries against keys, and values, of sizes far from 1: the powers of
+    two that the f16 operands are taken at."""
+    import torch
+    s = Step([300, 5, 40], [1, 3, 60], 14, 2, hd, values, "int8", seed=8)
+    s.cache.v_scales.mul_(up if up < 1e20 else 1e20)
+    s.cache.k_scales.mul_(1.0 / up)
+    s.q.mul_(up)
+    s.rows[:, :14] = s.q.float().cpu().numpy()
+    s.refresh()
+    s.check()
+
+
+def test_value_rows_of_very_different_sizes():
+    """V scales that vary by 2^20 within a page, and zero scales."""
+    import torch
+    for values in ("f32", "bf16"):
+        s = Step([300, 5, 40], [1, 3, 60], 14, 2, 64, values, "int8", seed=11)
+        e = torch.randint(-10, 11, s.cache.v_scales.shape, device="cuda").float()
+        s.cache.v_scales.mul_(torch.exp2(e))
+        s.cache.v_scales[::3] = 0
+        s.refresh()
+        s.check()
+    s.cache.v_scales.zero_()
+    assert (s.attend() == 0).all()
+
+
 def test_order_of_items_does_not_change_results():
     """The same call twice, and each sequence alone, bit for bit where the
     plan cuts them alike; a repeated call always."""
@@ -443,6 +488,10 @@ def test_refusals_leave_outputs_alone():
             qb.kv_write(bad, s.v, s.cache, s.plan)
     with pytest.raises(ValueError):
         qb.paged_attention(s.q, s.cache, s.plan, torch.empty(6, 14, 64, device="cuda")[::2])
+    with pytest.raises(qb.CacheError):
+        qb.paged_attention(s.y, s.cache, s.plan, s.y)
+    with pytest.raises(qb.CacheError):
+        qb.kv_read(s.cache, s.plan, s.k, s.k)
     other = qb.PagedCache(4, 2, 64, "bf16")
     with pytest.raises(qb.CacheError):
         qb.paged_attention(s.q, other, s.plan, s.y)

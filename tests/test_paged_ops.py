@@ -44,6 +44,8 @@ def test_plan_refusals():
     with pytest.raises(ValueError):
         plan(t, [0, 0], [1, 1], window=-1)
     with pytest.raises(ValueError):
+        plan(t, [0, 0], [1, 1], window=4, sinks=2**64)
+    with pytest.raises(ValueError):
         plan(t * 1.0, [0, 0], [1, 1])
     with pytest.raises(ValueError):
         plan(t, [0], [1, 1])
@@ -169,7 +171,7 @@ def test_call_refusals_need_no_device():
     def write(c=cache, pl=p, kn=n, ks=128, vn=n, vs=128, kp=x, wp=w):
         return L.qb_kv_write(kp, kn, ks, x, vn, vs, C.byref(c), C.byref(pl), wp, None)
 
-    def attend(c=cache, pl=p, qn=nq, qs=896, yn=nq, scale=0.125, ws=None, wn=None, yp=q):
+    def attend(c=cache, pl=p, qn=nq, qs=896, yn=nq, scale=0.125, ws=None, wn=None, yp=C.c_void_p(9 << 20)):
         return L.qb_paged_attention(q, qn, qs, C.byref(c), C.byref(pl), w, yp, yn, scale, ws,
                                     pl.workspace_bytes if wn is None else wn, None)
 
@@ -195,6 +197,15 @@ def test_call_refusals_need_no_device():
     for bad in (0.0, -1.0, float("nan"), float("inf")):
         assert attend(scale=bad) == 27
     assert attend(qn=1) == 3 and attend(yn=1) == 3 and attend(yp=None) == 27
+    # Y and Q share memory; rows of one buffer side by side do not.
+    assert attend(yp=C.c_void_p((3 << 20) + 4)) == 27
+    read = lambda kp, ks, vp, vs: L.qb_kv_read(C.byref(cache), C.byref(p), w, kp, 2 * ks + 128, ks, vp,  # noqa: E731
+                                               2 * vs + 128, vs, None)
+    base = 3 << 20
+    assert read(base, 128, base, 128) == 27
+    assert read(base, 256, base + 4 * 127, 256) == 27
+    assert read(base, 256, base + 4 * 129, 256) == 27
+    assert read(base, 256, base + 4 * 200, 300) == 27
     _, long = plan(np.arange(64).reshape(1, 64), [1000], [1])
     if long.workspace_bytes:
         a = 896
