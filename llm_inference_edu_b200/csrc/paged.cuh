@@ -36,8 +36,16 @@ struct Item {
 };
 
 struct Merge {
-    int32_t seq, kvh, row0, rows, slot, parts, stride, pad;
+    int32_t seq, kvh, row0, rows, slot, parts, stride, quads;
 };
+
+// Where a partial result keeps element d of row r.  The tile kernel has a
+// thread a row: in quads of four dimensions, rows side by side, its lanes
+// write 512 bytes at once (row by row they cost it 10 us an item of 256
+// rows).  The others have lanes along a row.
+__device__ __forceinline__ size_t part_at(int rows, int hd, int r, int d, bool quads) {
+    return quads ? ((size_t)(d >> 2) * rows + r) * 4 + (d & 3) : (size_t)r * hd + d;
+}
 
 // Row blocks of the step kernel (mma.sync, one block of 8 rows per n8 tile)
 // and of the tile kernel (tcgen05, 128 rows an MMA); key units of each.
@@ -118,7 +126,7 @@ __device__ __forceinline__ bool sees(int p, int j, int window, int sinks) {
 // (head widths other than 64 and 128, FP32 caches) and, by those variants,
 // for items whose partly hidden units hold values that are not finite.
 template <typename TV, typename TC>
-__device__ __noinline__ void attend_row(const Args &a, const Item *item, int r, int unit, int lane) {
+__device__ __noinline__ void attend_row(const Args &a, const Item *item, int r, int unit, int lane, bool quads = false) {
     const Item it = *item;
     const SeqRec sq = *(const SeqRec *)(a.words + a.off_seqs + it.seq * 4);
     const int32_t *table = a.words + sq.table;
@@ -178,7 +186,7 @@ __device__ __noinline__ void attend_row(const Args &a, const Item *item, int r, 
         float *w = a.ws + it.slot;
 #pragma unroll
         for (int i2 = 0; i2 < kMaxHeadDim / 32; ++i2)
-            if (lane + 32 * i2 < a.hd) w[(size_t)r * a.hd + lane + 32 * i2] = o[i2];
+            if (lane + 32 * i2 < a.hd) w[part_at(it.rows, a.hd, r, lane + 32 * i2, quads)] = o[i2];
         if (lane == 0) {
             w[(size_t)it.rows * a.hd + r] = m;
             w[(size_t)it.rows * (a.hd + 1) + r] = l;

@@ -52,7 +52,7 @@ __device__ __forceinline__ void merge_parts(const float *w, const Merge &mg, int
         l = fmaf(f, wl[at], l);
 #pragma unroll
         for (int i = 0; i < V; ++i)
-            if (lane + 32 * i < hd) o[i] = fmaf(f, w[at + (size_t)r * hd + lane + 32 * i], o[i]);
+            if (lane + 32 * i < hd) o[i] = fmaf(f, w[at + part_at(mg.rows, hd, r, lane + 32 * i, mg.quads)], o[i]);
     }
 }
 

@@ -133,7 +133,7 @@ double makespan(const std::vector<Block> &bl, const Grid &g, Cut how, int T, siz
 // Cuts the blocks' units into items (longest first) and lists the merges:
 // of a few candidate cuts the one whose simulated end comes first, whole
 // blocks if none is clearly better.
-void cut(std::vector<Block> &bl, const Grid &g, int hd, int64_t &ws, std::vector<Item> &items,
+void cut(std::vector<Block> &bl, const Grid &g, int hd, bool quads, int64_t &ws, std::vector<Item> &items,
          std::vector<Merge> &merges) {
     if (bl.empty()) return;
     std::stable_sort(bl.begin(), bl.end(), [&](const Block &a, const Block &b) {
@@ -176,8 +176,8 @@ void cut(std::vector<Block> &bl, const Grid &g, int hd, int64_t &ws, std::vector
         pieces_of(b.units, g, how, T, pos, i + tail >= bl.size(), n);
         pos += b.units;
         const bool part = n.size() > 1;
-        const int stride = b.rows * (hd + 2);
-        if (part) merges.push_back(Merge{b.seq, b.kvh, b.row0, b.rows, (int32_t)ws, (int32_t)n.size(), stride, 0});
+        const int stride = (b.rows * (hd + 2) + 3) / 4 * 4;
+        if (part) merges.push_back(Merge{b.seq, b.kvh, b.row0, b.rows, (int32_t)ws, (int32_t)n.size(), stride, quads});
         int at = 0;
         for (int u : n) {
             items.push_back(Item{b.seq, b.kvh, b.row0, b.rows, at, at + u, b.ns, b.u0, b.w0, b.hi,
@@ -257,8 +257,8 @@ uint32_t build(const qb_paged_step &s, int32_t *words, size_t capacity, qb_paged
     std::vector<Item> si, ti;
     std::vector<Merge> merges;
     int64_t ws = 0;
-    cut(bs, small, hd, ws, si, merges);
-    cut(bt, tile, hd, ws, ti, merges);
+    cut(bs, small, hd, false, ws, si, merges);
+    cut(bt, tile, hd, true, ws, ti, merges);
     if (ws > 0x7fffffff) return QB_RESOURCE_BUDGET;
 
     qb_paged_plan p = {};

@@ -273,9 +273,9 @@ template <typename TV, int HD>
 __device__ __forceinline__ void put_row(const Args &a, const Item &it, const SeqRec &sq, int r, int d, float (&v)[32],
                                         float m, float l) {
     if (it.slot >= 0) {
-        float *w = a.ws + it.slot + (size_t)r * HD + d;
 #pragma unroll
-        for (int e = 0; e < 32; e += 2) *(float2 *)(w + e) = make_float2(v[e], v[e + 1]);
+        for (int e = 0; e < 32; e += 4)
+            *(float4 *)(a.ws + it.slot + part_at(it.rows, HD, r, d + e, true)) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
         if (d == 0) {
             a.ws[it.slot + (size_t)it.rows * HD + r] = m;
             a.ws[it.slot + (size_t)it.rows * (HD + 1) + r] = l;
@@ -980,7 +980,7 @@ __global__ void __launch_bounds__(Tile<TV, TC, HD>::kThreads, 1)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
     if (redo && warp < 8)
         for (int r = warp; r < it.rows; r += 8)
-            if (ctl->bad[r]) attend_row<TV, TC>(a, item, r, KT, lane);
+            if (ctl->bad[r]) attend_row<TV, TC>(a, item, r, KT, lane, true);
 }
 
 // ------------------------------------------------------------------ host ----
