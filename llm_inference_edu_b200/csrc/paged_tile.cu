@@ -82,6 +82,9 @@ struct Tile {
     static constexpr size_t kv_off = kQBytes, raw_off = kv_off + (size_t)2 * NS * kTileBytes,
                             scl_off = raw_off + (size_t)RS * kPiece, max_off = scl_off + (size_t)D * 2 * KT * 4,
                             ctl_off = max_off + (kWide ? 2048 : 0);
+    // The results' way out, behind what the streams leave each other.
+    static constexpr int stage_off = HD == 128 ? 72 * 1024 : 40 * 1024;
+    static_assert(128 * (HD + 4) * 4 + 2048 <= stage_off && stage_off + (kWide ? 4 : 8) * 4608 <= 2 * NS * kTileBytes, "stage");
     static constexpr size_t bytes = ctl_off + 2048 + 1024;
     static_assert(bytes <= 232448, "shared memory of a CTA");
 };
@@ -267,14 +270,19 @@ __device__ __forceinline__ Join join(float m0, float l0, float m1, float l1) {
     return j;
 }
 
-// Dimensions d .. d + 31 of a row's result: divided by the sum, or as the
-// item's part with its maximum and sum.
+// 128 bytes of results (CB dimensions from d on) of this warp's 32 rows, a
+// row a lane: as the item's part with its maximum and sum, or divided by the
+// sum.  Results go through shared memory (`stage`, 32 rows 144 bytes apart),
+// so that eight lanes write a row's 128 bytes: a lane a row took the kernel
+// 2 us longer an item.
 template <typename TV, int HD>
-__device__ __forceinline__ void put_row(const Args &a, const Item &it, const SeqRec &sq, int r, int d, float (&v)[32],
-                                        float m, float l) {
+__device__ __forceinline__ void put_rows(const Args &a, const Item &it, const SeqRec &sq, int r, int d,
+                                         float (&v)[128 / sizeof(TV)], float m, float l, uint8_t *stage, int lane) {
+    constexpr int CB = 128 / (int)sizeof(TV);
     if (it.slot >= 0) {
+        if (r >= it.rows) return;
 #pragma unroll
-        for (int e = 0; e < 32; e += 4)
+        for (int e = 0; e < CB; e += 4)
             *(float4 *)(a.ws + it.slot + part_at(it.rows, HD, r, d + e, true)) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
         if (d == 0) {
             a.ws[it.slot + (size_t)it.rows * HD + r] = m;
@@ -286,19 +294,31 @@ __device__ __forceinline__ void put_row(const Args &a, const Item &it, const Seq
     const size_t at = ((size_t)(sq.tok0 + row / a.G) * a.H + it.kvh * a.G + row % a.G) * HD + d;
     const float inv = __fdiv_rn(1.0f, l);
 #pragma unroll
-    for (int e = 0; e < 32; ++e) v[e] *= inv;
-    TV *y = (TV *)a.y + at;
+    for (int e = 0; e < CB; ++e) v[e] *= inv;
     if ((uintptr_t)a.y & 15) {
+        if (r < it.rows)
 #pragma unroll
-        for (int e = 0; e < 32; ++e) store_value(y, e, v[e]);
-    } else if constexpr (sizeof(TV) == 4) {
+            for (int e = 0; e < CB; ++e) store_value((TV *)a.y, at + e, v[e]);
+        return;
+    }
+    uint4 *mine = (uint4 *)(stage + lane * 144);
+    __syncwarp();
 #pragma unroll
-        for (int e = 0; e < 32; e += 4) *(float4 *)(y + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
-    } else {
+    for (int x = 0; x < 8; ++x) {
+        if constexpr (sizeof(TV) == 4)
+            mine[x] = make_uint4(__float_as_uint(v[4 * x]), __float_as_uint(v[4 * x + 1]), __float_as_uint(v[4 * x + 2]),
+                                 __float_as_uint(v[4 * x + 3]));
+        else
+            mine[x] = make_uint4(pack_bf16(v[8 * x], v[8 * x + 1]), pack_bf16(v[8 * x + 2], v[8 * x + 3]),
+                                 pack_bf16(v[8 * x + 4], v[8 * x + 5]), pack_bf16(v[8 * x + 6], v[8 * x + 7]));
+    }
+    __syncwarp();
 #pragma unroll
-        for (int e = 0; e < 32; e += 8)
-            *(uint4 *)(y + e) = make_uint4(pack_bf16(v[e], v[e + 1]), pack_bf16(v[e + 2], v[e + 3]),
-                                           pack_bf16(v[e + 4], v[e + 5]), pack_bf16(v[e + 6], v[e + 7]));
+    for (int x = 0; x < 8; ++x) {
+        const int from = x * 4 + lane / 8;
+        const size_t to = __shfl_sync(0xffffffffu, (unsigned long long)at, from);
+        if (r - lane + from < it.rows)
+            *(uint4 *)((TV *)a.y + to + (lane & 7) * (16 / sizeof(TV))) = *(uint4 *)(stage + from * 144 + (lane & 7) * 16);
     }
 }
 
@@ -433,30 +453,34 @@ __global__ void __launch_bounds__(Tile<TV, TC, HD>::kThreads, 1)
         {
             const int nrows = shared ? 256 : 128;
             const bool vec = (((uintptr_t)a.q | (a.q_stride * sizeof(TV))) & 15) == 0;
-            for (int u = threadIdx.x; u < nrows * (HD / 8); u += 256) {
-                const int r = u / (HD / 8), ch = u % (HD / 8);
-                float v[8];
+            // Four pieces of eight elements under way at once.
+            constexpr int kRun = 4, kWords = T::kWide ? 2 : 1;
+#pragma unroll 1
+            for (int u0 = threadIdx.x; u0 < nrows * (HD / 8); u0 += 256 * kRun) {
+                uint4 raw[kRun][kWords];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = 0.0f;
-                if (r < it.rows) {
-                    const int row = it.row0 + r;
+                for (int x = 0; x < kRun; ++x) {
+                    const int u = u0 + 256 * x, r = u / (HD / 8), ch = u % (HD / 8), row = it.row0 + r;
+#pragma unroll
+                    for (int y = 0; y < kWords; ++y) raw[x][y] = make_uint4(0u, 0u, 0u, 0u);
+                    if (r >= it.rows) continue;
                     const TV *q = (const TV *)a.q + (size_t)(sq.tok0 + row / a.G) * a.q_stride +
                                   (size_t)(it.kvh * a.G + row % a.G) * HD + ch * 8;
                     if (vec) {
-                        if constexpr (T::kWide) {
-                            const float4 x = *(const float4 *)q, y = *(const float4 *)(q + 4);
-                            v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
-                            v[4] = y.x; v[5] = y.y; v[6] = y.z; v[7] = y.w;
-                        } else {
-                            const uint4 x = *(const uint4 *)q;
-                            v[0] = bf16_lo(x.x); v[1] = bf16_hi(x.x); v[2] = bf16_lo(x.y); v[3] = bf16_hi(x.y);
-                            v[4] = bf16_lo(x.z); v[5] = bf16_hi(x.z); v[6] = bf16_lo(x.w); v[7] = bf16_hi(x.w);
-                        }
-                    } else {
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) v[e] = load_value(q, e);
+                        for (int y = 0; y < kWords; ++y) raw[x][y] = ((const uint4 *)q)[y];
+                    } else {
+                        TV *e = (TV *)raw[x];
+#pragma unroll
+                        for (int y = 0; y < 8; ++y) e[y] = q[y];
                     }
                 }
+#pragma unroll
+              for (int x = 0; x < kRun; ++x) {
+                const int u = u0 + 256 * x, r = u / (HD / 8), ch = u % (HD / 8);
+                float v[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = load_value((const TV *)raw[x], e);
                 const int rr = r & 127;
                 if constexpr (T::kInt8) {
                     // The row's HD / 8 pieces are neighbouring lanes.
@@ -489,6 +513,7 @@ __global__ void __launch_bounds__(Tile<TV, TC, HD>::kThreads, 1)
                     uint8_t *dst = s_q + ((r >> 7) * PN + pl * PN + ch / 8) * 16384 + rr * 128 + (((ch & 7) ^ (rr & 7)) << 4);
                     *(uint4 *)dst = make_uint4(w[0], w[1], w[2], w[3]);
                 }
+              }
             }
             if (T::kInt8) asm volatile("bar.sync 2, 256;" ::: "memory");
             fence_proxy_async_smem();
@@ -698,23 +723,27 @@ __global__ void __launch_bounds__(Tile<TV, TC, HD>::kThreads, 1)
             }
             asm volatile("bar.sync 1, %0;" ::"n"(T::kWide ? 384 : 256) : "memory");
         }
-        if (!T::kWide && (shared || s == 0)) {
+        if constexpr (!T::kWide) if (shared || s == 0) {
             Join j = {m, l, 1.0f, 0.0f};
             if (!shared && nk > 1) j = join(m, l, s_ml[256 + r_in], s_ml[384 + r_in]);
             bool bad = false;
 #pragma unroll 1
-            for (int d = 0; d < HD; d += 32) {
-                uint32_t x[32];
-                tmem_ld32(to + d, x);
-                wait_ld();
-                float v[32];
+            for (int d = 0; d < HD; d += 64) {
+                float v[64];
 #pragma unroll
-                for (int e = 0; e < 32; ++e) {
-                    v[e] = __uint_as_float(x[e]) * j.f0;
-                    if (j.f1 != 0.0f) v[e] = fmaf(j.f1, s_o[r_in * (HD + 4) + d + e], v[e]);
-                    bad |= !isfinite(v[e]);
+                for (int h = 0; h < 64; h += 32) {
+                    uint32_t x[32];
+                    tmem_ld32(to + d + h, x);
+                    wait_ld();
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) {
+                        v[h + e] = __uint_as_float(x[e]) * j.f0;
+                        if (j.f1 != 0.0f) v[h + e] = fmaf(j.f1, s_o[r_in * (HD + 4) + d + h + e], v[h + e]);
+                        bad |= !isfinite(v[h + e]);
+                    }
                 }
-                if (r < it.rows) put_row<TV, HD>(a, it, sq, r, d, v, j.m, fin ? j.l : __uint_as_float(0x7fffffffu));
+                put_rows<uint16_t, HD>(a, it, sq, r, d, v, j.m, fin ? j.l : __uint_as_float(0x7fffffffu),
+                                       s_k + T::stage_off + warp * 4608, lane);
             }
             if (bad && fin && r < it.rows) ctl->bad[r] = 1;
         }
@@ -772,7 +801,8 @@ __global__ void __launch_bounds__(Tile<TV, TC, HD>::kThreads, 1)
                     v[e + 1] = o[(d + e) / 2].y;
                     bad |= !isfinite(v[e]) | !isfinite(v[e + 1]);
                 }
-                if (r < it.rows) put_row<TV, HD>(a, it, sq, r, d, v, j.m, fin ? j.l : __uint_as_float(0x7fffffffu));
+                put_rows<float, HD>(a, it, sq, r, d, v, j.m, fin ? j.l : __uint_as_float(0x7fffffffu),
+                                    s_k + T::stage_off + (warp - T::kGather) * 4608, lane);
             }
             if (bad && fin && r < it.rows) ctl->bad[r] = 1;
         }
