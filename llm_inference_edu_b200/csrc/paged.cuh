@@ -69,6 +69,7 @@ struct Args {
     const float *ks, *vs;
     float *ws;
     int dependent;        // launched behind another kernel of the same call
+    uint32_t g_mul, g_shift;  // row / G = (mulhi(row, g_mul) + row) >> g_shift, row < 2^31
 };
 
 // Byte element types of values and caches.
@@ -111,6 +112,23 @@ cudaError_t launch(void (*kernel)(KArgs...), dim3 grid, int threads, size_t smem
     cfg.attrs = at;
     cfg.numAttrs = dependent ? 1 : 0;
     return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+// Multiplier and shift of a division by d of numbers below 2^31.
+inline void divide_by(uint32_t d, uint32_t &mul, uint32_t &shift) {
+    shift = 0;
+    while ((1ull << shift) < d) ++shift;
+    mul = (uint32_t)(((1ull << 32) * ((1ull << shift) - d)) / d + 1);
+}
+
+// Packed row `row` of a sequence and KV head: its token and query head.
+__device__ __forceinline__ int token_of(const Args &a, int row) {
+    return (int)((__umulhi((uint32_t)row, a.g_mul) + (uint32_t)row) >> a.g_shift);
+}
+// Element offset of packed row `row` in Q (stride a token) or Y (a.H * a.hd).
+__device__ __forceinline__ size_t row_at(const Args &a, const SeqRec &sq, int kvh, int row, size_t stride) {
+    const int t = token_of(a, row);
+    return (size_t)(sq.tok0 + t) * stride + (size_t)(kvh * a.G + row - t * a.G) * a.hd;
 }
 
 // Position p sees position j of its sequence.

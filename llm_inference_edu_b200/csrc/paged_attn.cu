@@ -151,6 +151,7 @@ uint32_t qb_paged_attention(const void *q, size_t q_len, size_t q_stride, const 
     a.H = (int)plan->query_heads;
     a.KV = (int)plan->kv_heads;
     a.G = a.H / a.KV;
+    divide_by((uint32_t)a.G, a.g_mul, a.g_shift);
     a.hd = (int)plan->head_dim;
     a.window = (int)plan->window;
     a.sinks = (int)(plan->sinks < 0x7fffffffu ? plan->sinks : 0x7fffffffu);

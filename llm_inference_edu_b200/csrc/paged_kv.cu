@@ -280,13 +280,6 @@ uint32_t launch_rows(const RowArgs &a, bool write, cudaStream_t st) {
     return QB_OK;
 }
 
-// Multiplier and shift of RowArgs for a division by d.
-void divide_by(uint32_t d, uint32_t &mul, uint32_t &shift) {
-    shift = 0;
-    while ((1ull << shift) < d) ++shift;
-    mul = (uint32_t)(((1ull << 32) * ((1ull << shift) - d)) / d + 1);
-}
-
 uint32_t run_rows(RowArgs a, uint32_t vt, uint32_t ct, bool write, cudaStream_t st) {
     divide_by((uint32_t)a.KV, a.mul, a.shift);
     if (vt == QB_PAGED_F32) {

@@ -93,7 +93,7 @@ __global__ void __launch_bounds__(kStepWarps * 32, 3) attend_step(const __grid_c
     const Item it = *item;
     const SeqRec sq = *(const SeqRec *)(a.words + a.off_seqs + it.seq * 4);
     const int32_t *table = a.words + sq.table;
-    const int p_lo = sq.start + it.row0 / a.G, p_hi = it.hi - 1;
+    const int p_lo = sq.start + token_of(a, it.row0), p_hi = it.hi - 1;
     auto page_of = [&](int i) { return i < it.ns ? i : it.u0 + i - it.ns; };
 
     // The pages of this warp's next group: table entries one group ahead of
@@ -164,9 +164,7 @@ __global__ void __launch_bounds__(kStepWarps * 32, 3) attend_step(const __grid_c
         const int d = lane * 4, ks = d / (4 * run) * per + d % run / 4, fl = (r & 7) * 4 + d % (4 * run) / run;
         float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
         if (r < it.rows && d < HD) {
-            const int row = it.row0 + r;
-            const TV *q = (const TV *)a.q + (size_t)(sq.tok0 + row / a.G) * a.q_stride +
-                          (size_t)(it.kvh * a.G + row % a.G) * HD + d;
+            const TV *q = (const TV *)a.q + row_at(a, sq, it.kvh, it.row0 + r, a.q_stride) + d;
 #pragma unroll
             for (int x = 0; x < 4; ++x) v[x] = load_value(q, x);
         }
@@ -214,7 +212,7 @@ __global__ void __launch_bounds__(kStepWarps * 32, 3) attend_step(const __grid_c
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int y = 0; y < 2; ++y) pos[nt][y] = sq.start + min(it.row0 + nt * 8 + 2 * c + y, it.row0 + it.rows - 1) / a.G;
+        for (int y = 0; y < 2; ++y) pos[nt][y] = sq.start + token_of(a, min(it.row0 + nt * 8 + 2 * c + y, it.row0 + it.rows - 1));
 
     // m: what the weights are taken against, at least the running maximum
     // less kAbove.
@@ -485,8 +483,7 @@ __global__ void __launch_bounds__(kStepWarps * 32, 3) attend_step(const __grid_c
             f[w] = s_m[w][r] == base ? 1.0f : ex2(s_m[w][r] - base);
             ll = fmaf(f[w], s_l[w][r], ll);
         }
-        const int row = it.row0 + r;
-        const size_t at = ((size_t)(sq.tok0 + row / a.G) * a.H + it.kvh * a.G + row % a.G) * HD;
+        const size_t at = row_at(a, sq, it.kvh, it.row0 + r, (size_t)a.H * HD);
 #pragma unroll
         for (int d0 = 0; d0 < HD; d0 += 32) {
             const int d = d0 + lane;

@@ -290,8 +290,7 @@ __device__ __forceinline__ void put_rows(const Args &a, const Item &it, const Se
         }
         return;
     }
-    const int row = it.row0 + r;
-    const size_t at = ((size_t)(sq.tok0 + row / a.G) * a.H + it.kvh * a.G + row % a.G) * HD + d;
+    const size_t at = row_at(a, sq, it.kvh, it.row0 + r, (size_t)a.H * HD) + d;
     const float inv = __fdiv_rn(1.0f, l);
 #pragma unroll
     for (int e = 0; e < CB; ++e) v[e] *= inv;
@@ -464,8 +463,7 @@ __global__ void __launch_bounds__(Tile<TV, TC, HD>::kThreads, 1)
 #pragma unroll
                     for (int y = 0; y < kWords; ++y) raw[x][y] = make_uint4(0u, 0u, 0u, 0u);
                     if (r >= it.rows) continue;
-                    const TV *q = (const TV *)a.q + (size_t)(sq.tok0 + row / a.G) * a.q_stride +
-                                  (size_t)(it.kvh * a.G + row % a.G) * HD + ch * 8;
+                    const TV *q = (const TV *)a.q + row_at(a, sq, it.kvh, row, a.q_stride) + ch * 8;
                     if (vec) {
 #pragma unroll
                         for (int y = 0; y < kWords; ++y) raw[x][y] = ((const uint4 *)q)[y];
@@ -478,6 +476,9 @@ __global__ void __launch_bounds__(Tile<TV, TC, HD>::kThreads, 1)
 #pragma unroll
               for (int x = 0; x < kRun; ++x) {
                 const int u = u0 + 256 * x, r = u / (HD / 8), ch = u % (HD / 8);
+                if constexpr (!T::kWide && !T::kInt8) {
+                    *(uint4 *)(s_q + ((r >> 7) * PN + ch / 8) * 16384 + (r & 127) * 128 + (((ch & 7) ^ (r & 7)) << 4)) = raw[x][0];
+                } else {
                 float v[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) v[e] = load_value((const TV *)raw[x], e);
@@ -513,6 +514,7 @@ __global__ void __launch_bounds__(Tile<TV, TC, HD>::kThreads, 1)
                     uint8_t *dst = s_q + ((r >> 7) * PN + pl * PN + ch / 8) * 16384 + rr * 128 + (((ch & 7) ^ (rr & 7)) << 4);
                     *(uint4 *)dst = make_uint4(w[0], w[1], w[2], w[3]);
                 }
+                }
               }
             }
             if (T::kInt8) asm volatile("bar.sync 2, 256;" ::: "memory");
@@ -522,9 +524,9 @@ __global__ void __launch_bounds__(Tile<TV, TC, HD>::kThreads, 1)
         const int r_in = (warp & 3) * 32 + lane;               // row of the tile
         const int r = (shared ? s * 128 : 0) + r_in;           // row of the item
         const int rmax = it.row0 + it.rows - 1;
-        const int pos = sq.start + min(it.row0 + r, rmax) / a.G;
+        const int pos = sq.start + token_of(a, min(it.row0 + r, rmax));
         const int rb = it.row0 + (shared ? s * 128 : 0);
-        const int p_lo = sq.start + min(rb, rmax) / a.G, p_hi = sq.start + min(rb + 127, rmax) / a.G;
+        const int p_lo = sq.start + token_of(a, min(rb, rmax)), p_hi = sq.start + token_of(a, min(rb + 127, rmax));
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t ts = tmem + s * 256 + lanes, to = ts + 128;
         const int n_steps = shared ? nk : (nk - s + 1) / 2;
