@@ -301,9 +301,11 @@ uint32_t qb_paged_plan_build(const qb_paged_step *step, int32_t *words, size_t c
  * plan's value_dtype, *_stride elements between tokens, *_len elements from
  * the first to the last) at their positions; every other cache row is left
  * as it was.  FP32 rows are stored as they are, BF16 rounds to nearest
- * even, INT8 is qb_quantize_int8's encode with one group per row: scale =
- * max|x| / 127 (1 where that is 0), q = clamp(round(x / scale)); a row with a
- * value that is not finite stores scale NaN and zeros, so it reads back NaN.
+ * even, INT8 has one scale per row: scale = max|x| * (1 / 127) in FP32 (1
+ * where that is 0; qb_quantize_int8 divides by 127, which may differ in the
+ * last place), q = clamp(round(x / scale)) with halves away from zero; a row
+ * with a value that is not finite stores scale NaN and zeros, so it reads
+ * back NaN.
  * QB_INVALID_SHAPE: the cache is not of the plan's kind;
  * QB_INVALID_STATE: the plan's shared_rows. */
 uint32_t qb_kv_write(const void *k, size_t k_len, size_t k_stride, const void *v, size_t v_len,

@@ -1,5 +1,5 @@
-// Cache rows of the paged operators: stored (with the INT8 encode of
-// ops.cu's quant_kernel, one group a row) and read back.
+// Cache rows of the paged operators: stored (INT8: round(x / scale), halves
+// away from zero, one scale a row) and read back.
 #include <math.h>
 
 #include "paged.cuh"
@@ -21,6 +21,10 @@ struct RowArgs {
 };
 
 constexpr int kRowWarps = 8;
+
+// A row's scale is its largest magnitude times this (one rounding, so within
+// a unit in the last place of the quotient by 127).
+constexpr float kStep = 1.0f / 127.0f;
 
 // One warp a row, in any alignment: the row sits in registers between the
 // maximum and the encode.
@@ -48,7 +52,7 @@ __global__ void __launch_bounds__(kRowWarps * 32) kv_write_rows(const __grid_con
 #pragma unroll
         for (int off = 16; off; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
         bad = __any_sync(0xffffffffu, bad);
-        float scale = __fdiv_rn(m, 127.0f);
+        float scale = __fmul_rn(m, kStep);
         if (scale == 0.0f) scale = 1.0f;
         if (lane == 0) a.scales[z][at] = bad ? __uint_as_float(0x7fffffffu) : scale;
 #pragma unroll
@@ -161,7 +165,7 @@ struct RowAt {
 template <int E>
 __device__ __forceinline__ float encode_row(const float (&v)[E], uint32_t mb, uint32_t (&out)[E / 4]) {
     const bool bad = mb >= 0x7f800000u;
-    float scale = __fdiv_rn(__uint_as_float(mb), 127.0f);
+    float scale = __fmul_rn(__uint_as_float(mb), kStep);
     if (scale == 0.0f) scale = 1.0f;
     const float inv = __fdiv_rn(1.0f, scale), big = 12582912.0f;
     bool exact = bad;

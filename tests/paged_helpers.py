@@ -11,7 +11,7 @@ def quantize(x):
     x = np.asarray(x, np.float32)
     m = np.max(np.abs(x), -1)
     with np.errstate(invalid="ignore"):
-        scale = (m / np.float32(127)).astype(np.float32)
+        scale = (m * (np.float32(1) / np.float32(127))).astype(np.float32)
     scale = np.where(scale == 0, np.float32(1), scale)
     bad = ~np.isfinite(x).all(-1)
     with np.errstate(invalid="ignore"):
