@@ -24,6 +24,9 @@
 // FP32 values: each tile's product is gathered in FP32 by a warpgroup.
 // K tiles are K-major operands as TMA leaves them (128-byte swizzle, a box a
 // page); V tiles are the MN-major operand in the same layout.
+// 4,096 tokens behind 4,096, 28/4 heads of 128, BF16: 373 us, 967 TFLOP/s.
+// A stream's softmax takes 1.7 k cycles a tile and its products 1.1 k, with
+// the other stream's in between: neither pipe is full.
 // Every wait is bounded: a role that gives up raises the abort flag, copies
 // and MMAs in flight are drained, TMEM is freed and the item's rows are NaN.
 #include <cuda.h>
@@ -273,8 +276,8 @@ __device__ __forceinline__ Join join(float m0, float l0, float m1, float l1) {
 // 128 bytes of results (CB dimensions from d on) of this warp's 32 rows, a
 // row a lane: as the item's part with its maximum and sum, or divided by the
 // sum.  Results go through shared memory (`stage`, 32 rows 144 bytes apart),
-// so that eight lanes write a row's 128 bytes: a lane a row took the kernel
-// 2 us longer an item.
+// so that eight lanes write a row's 128 bytes (a lane a row: 80 against 75 us
+// on 2,001 tokens under a window of 1,001, with Q's loads four at a time).
 template <typename TV, int HD>
 __device__ __forceinline__ void put_rows(const Args &a, const Item &it, const SeqRec &sq, int r, int d,
                                          float (&v)[128 / sizeof(TV)], float m, float l, uint8_t *stage, int lane) {
