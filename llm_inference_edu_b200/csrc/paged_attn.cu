@@ -153,7 +153,8 @@ uint32_t qb_paged_attention(const void *q, size_t q_len, size_t q_stride, const 
     a.G = a.H / a.KV;
     divide_by((uint32_t)a.G, a.g_mul, a.g_shift);
     a.hd = (int)plan->head_dim;
-    a.window = (int)plan->window;
+    // A window as long as a table row hides nothing.
+    a.window = plan->window < plan->pages_per_sequence * kPage ? (int)plan->window : 0;
     a.sinks = (int)(plan->sinks < 0x7fffffffu ? plan->sinks : 0x7fffffffu);
     a.c = (float)((double)scale * 1.4426950408889634);
     a.q = q;

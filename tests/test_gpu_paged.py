@@ -240,6 +240,12 @@ def test_windows(values, cache, window, sinks, heads, kv, hd):
          seed=window + sinks).check()
 
 
+@pytest.mark.parametrize("window", [271, 288, 2**31 - 1])
+@pytest.mark.parametrize("values,cache", [("f32", "bf16"), ("bf16", "int8"), ("f32", "f32")])
+def test_windows_about_as_long_as_the_sequence(window, values, cache):
+    Step([0, 71], [1, 200], 14, 2, 64, values, cache, window, 3, seed=2).check()
+
+
 @pytest.mark.parametrize("values,cache", [("f32", "bf16"), ("bf16", "int8")])
 @pytest.mark.parametrize("scale", [1.0, 0.01, 3.5])
 def test_scales(values, cache, scale):
