@@ -34,11 +34,11 @@ struct Grid {
 Grid rows_grid() { return Grid{64, 8, 148 * 4, 1, 1, 2, 8, 1}; }
 // Step kernel: three CTAs an SM; a unit is a page.
 Grid step_grid() { return Grid{kPage, 8, 148 * 3, 4, 2, 32, 16, 1}; }
-// Tile kernel: one CTA an SM.  Starting an item and leaving a partial result
-// take about as long as two and one or two key tiles of 128 rows.
+// Tile kernel: one CTA an SM.  Starting and ending an item takes 7 to 8 us,
+// a tile of 128 keys 1 us for up to 128 rows and 2 us for 256.
 Grid tile_grid(bool wide, bool int8) {
-    if (wide && !int8) return Grid{64, 128, 148, 4, 3, 4, 128, 1};
-    return Grid{128, wide ? 128 : 256, 148, 4, 3, 2, 128, 2};
+    if (wide && !int8) return Grid{64, 128, 148, 6, 3, 4, 128, 1};
+    return Grid{128, wide ? 128 : 256, 148, 8, 3, 2, 128, 2};
 }
 
 Block block_of(const qb_paged_step &s, const Grid &g, int seq, int kvh, int row0, int rows, int G) {
@@ -157,7 +157,7 @@ void cut(std::vector<Block> &bl, const Grid &g, int hd, bool quads, int64_t &ws,
             }
         };
         int before = 0;
-        for (double k : {1.0, 1.25, 1.5, 2.0, 3.0, 4.0, 6.0}) {
+        for (double k : {0.7, 0.85, 1.0, 1.25, 1.5, 2.0, 3.0, 4.0, 6.0}) {
             const int t = std::max<int>(g.least, (int)ceil((double)total / (g.slots * k)));
             if (t == before || t >= bl[0].units) continue;
             before = t;
