@@ -307,13 +307,14 @@ uint32_t qb_paged_plan_build(const qb_paged_step *step, int32_t *words, size_t c
  * with a value that is not finite stores scale NaN and zeros, so it reads
  * back NaN.
  * QB_INVALID_SHAPE: the cache is not of the plan's kind;
- * QB_INVALID_STATE: the plan's shared_rows. */
+ * QB_INVALID_PARAMETERS: K's and V's pools share memory, or the rows lie in
+ * one of them; QB_INVALID_STATE: the plan's shared_rows. */
 uint32_t qb_kv_write(const void *k, size_t k_len, size_t k_stride, const void *v, size_t v_len,
                      size_t v_stride, const qb_paged_cache *cache, const qb_paged_plan *plan,
                      const int32_t *words, void *stream);
 /* Reads the same rows back: f32(q) * scale, rounded once to value_dtype.
- * K's and V's rows may be slices of one buffer but not share memory
- * (QB_INVALID_PARAMETERS). */
+ * K's and V's rows may be slices of one buffer but not share memory with
+ * each other or the cache (QB_INVALID_PARAMETERS). */
 uint32_t qb_kv_read(const qb_paged_cache *cache, const qb_paged_plan *plan, const int32_t *words,
                     void *k, size_t k_len, size_t k_stride, void *v, size_t v_len, size_t v_stride,
                     void *stream);
@@ -325,8 +326,9 @@ uint32_t qb_kv_read(const qb_paged_cache *cache, const qb_paged_plan *plan, cons
  * row does not see has no influence on it, whatever the cache holds there.
  * `workspace`: at least the plan's workspace_bytes, its content on entry
  * irrelevant; calls that can overlap in time need one each.
+ * K's and V's pools may be the same memory.
  * QB_INVALID_PARAMETERS: scale not finite and positive, or Y shares memory
- * with Q (rows are read again where a result is not finite). */
+ * with Q (rows are read again where a result is not finite) or the cache. */
 uint32_t qb_paged_attention(const void *q, size_t q_len, size_t q_stride, const qb_paged_cache *cache,
                             const qb_paged_plan *plan, const int32_t *words, void *y, size_t y_len,
                             float scale, void *workspace, size_t workspace_bytes, void *stream);

@@ -117,6 +117,7 @@ uint32_t run_rows(const Args &a, uint32_t ct, cudaStream_t st) {
 uint32_t admit(const qb_paged_cache *c, const qb_paged_plan *p, const int32_t *words);
 uint32_t admit_rows(size_t buffer, size_t len, size_t stride, size_t width, size_t tokens);
 bool rows_meet(const void *p, size_t p_stride, const void *q, size_t q_stride, size_t width, size_t tokens, size_t size);
+bool rows_in_cache(const void *p, size_t stride, size_t width, size_t tokens, size_t size, const qb_paged_cache *c);
 
 }  // namespace paged
 }  // namespace qb
@@ -136,7 +137,9 @@ uint32_t qb_paged_attention(const void *q, size_t q_len, size_t q_stride, const 
     if ((s = admit_rows(0, q_len, q_stride, width, plan->tokens))) return s;
     if ((s = admit_rows(2, y_len, width, width, plan->tokens))) return s;
     if (!q || !y || !(isfinite(scale) && scale > 0.0f)) return QB_INVALID_PARAMETERS;
-    if (rows_meet(q, q_stride, y, width, width, plan->tokens, plan->value_dtype == QB_PAGED_F32 ? 4 : 2))
+    const size_t size = plan->value_dtype == QB_PAGED_F32 ? 4 : 2;
+    if (rows_meet(q, q_stride, y, width, width, plan->tokens, size) ||
+        rows_in_cache(y, width, width, plan->tokens, size, cache))
         return QB_INVALID_PARAMETERS;
     if (workspace_bytes < plan->workspace_bytes) {
         set_detail(3, plan->workspace_bytes, workspace_bytes);

@@ -340,6 +340,27 @@ bool rows_meet(const void *p, size_t p_stride, const void *q, size_t q_stride, s
     return off < w || step - off < w;
 }
 
+// Whether bytes [p, p + n) and [q, q + m) share memory.
+static bool meet(const void *p, size_t n, const void *q, size_t m) {
+    return (uintptr_t)p < (uintptr_t)q + m && (uintptr_t)q < (uintptr_t)p + n;
+}
+
+// Whether the range of `tokens` rows shares memory with a pool of the cache
+// or its scales.
+bool rows_in_cache(const void *p, size_t stride, size_t width, size_t tokens, size_t size, const qb_paged_cache *c) {
+    const size_t n = ((tokens - 1) * stride + width) * size, rows = c->pages * c->kv_heads * kPage;
+    const size_t pool = rows * c->head_dim * (c->dtype == QB_PAGED_F32 ? 4 : c->dtype == QB_PAGED_BF16 ? 2 : 1);
+    if (meet(p, n, c->k, pool) || meet(p, n, c->v, pool)) return true;
+    return c->dtype == QB_PAGED_INT8 && (meet(p, n, c->k_scales, rows * 4) || meet(p, n, c->v_scales, rows * 4));
+}
+
+// Whether K's and V's rows would be stored over each other.
+static bool pools_meet(const qb_paged_cache *c) {
+    const size_t rows = c->pages * c->kv_heads * kPage;
+    const size_t pool = rows * c->head_dim * (c->dtype == QB_PAGED_F32 ? 4 : c->dtype == QB_PAGED_BF16 ? 2 : 1);
+    return meet(c->k, pool, c->v, pool) || (c->dtype == QB_PAGED_INT8 && meet(c->k_scales, rows * 4, c->v_scales, rows * 4));
+}
+
 }  // namespace paged
 }  // namespace qb
 
@@ -357,6 +378,10 @@ uint32_t qb_kv_write(const void *k, size_t k_len, size_t k_stride, const void *v
     if ((s = admit_rows(0, k_len, k_stride, width, plan->tokens))) return s;
     if ((s = admit_rows(1, v_len, v_stride, width, plan->tokens))) return s;
     if (!k || !v) return QB_INVALID_PARAMETERS;
+    const size_t size = plan->value_dtype == QB_PAGED_F32 ? 4 : 2;
+    if (pools_meet(cache) || rows_in_cache(k, k_stride, width, plan->tokens, size, cache) ||
+        rows_in_cache(v, v_stride, width, plan->tokens, size, cache))
+        return QB_INVALID_PARAMETERS;
     if (plan->shared_rows) return QB_INVALID_STATE;
     RowArgs a{words + plan->off_slots, plan->tokens * plan->kv_heads, (int)plan->kv_heads, (int)plan->head_dim,
               {k, v}, {nullptr, nullptr}, {k_stride, v_stride}, {cache->k, cache->v},
@@ -374,7 +399,10 @@ uint32_t qb_kv_read(const qb_paged_cache *cache, const qb_paged_plan *plan, cons
     if ((s = admit_rows(1, v_len, v_stride, width, plan->tokens))) return s;
     if (!k || !v) return QB_INVALID_PARAMETERS;
     const size_t size = plan->value_dtype == QB_PAGED_F32 ? 4 : 2;
-    if (rows_meet(k, k_stride, v, v_stride, width, plan->tokens, size)) return QB_INVALID_PARAMETERS;
+    if (rows_meet(k, k_stride, v, v_stride, width, plan->tokens, size) ||
+        rows_in_cache(k, k_stride, width, plan->tokens, size, cache) ||
+        rows_in_cache(v, v_stride, width, plan->tokens, size, cache))
+        return QB_INVALID_PARAMETERS;
     RowArgs a{words + plan->off_slots, plan->tokens * plan->kv_heads, (int)plan->kv_heads, (int)plan->head_dim,
               {nullptr, nullptr}, {k, v}, {k_stride, v_stride}, {cache->k, cache->v},
               {cache->k_scales, cache->v_scales}};

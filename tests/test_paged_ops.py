@@ -214,6 +214,41 @@ def test_call_refusals_need_no_device():
         assert attend(pl=long, qn=a, yn=a, ws=C.c_void_p((1 << 20) + 4)) == 27
 
 
+def test_rows_in_the_cache_are_refused():
+    # Outputs over the pools or scales that other rows are read from, inputs
+    # over those that are written, K's rows stored over V's.
+    from llm_inference_edu_b200 import _lib
+    L = _lib.lib()
+    tables, starts, counts = np.arange(8).reshape(2, 4), [0, 3], [2, 1]
+    w, mb = C.c_void_p(1 << 30), 1 << 20
+    pool, scales, n = 64 * 2 * 16 * 64, 64 * 2 * 16 * 4, 3 * 128
+    for kind, dt, size in (("f32", 0, 4), ("bf16", 1, 2), ("int8", 2, 1)):
+        _, p = plan(tables, starts, counts, cache=kind)
+        at = [mb, 2 * mb] + ([3 * mb, 4 * mb] if dt == 2 else [None, None])
+        cache = _lib.PagedCacheC(*at, 64, 2, 64, dt)
+
+        def write(kp, vp, c=cache):
+            return L.qb_kv_write(kp, n, 128, vp, n, 128, C.byref(c), C.byref(p), w, None)
+
+        def read(kp, vp):
+            return L.qb_kv_read(C.byref(cache), C.byref(p), w, kp, n, 128, vp, n, 128, None)
+
+        def attend(yp):
+            return L.qb_paged_attention(20 * mb, 3 * 896, 896, C.byref(cache), C.byref(p), w, yp, 3 * 896, 0.125, None,
+                                        p.workspace_bytes, None)
+
+        inside = [at[0], at[0] + pool * size - 4, at[1], at[1] + 1024, at[1] - n * 4 + 4]
+        inside += [at[2], at[2] + scales - 4, at[3] - n * 4 + 4] if dt == 2 else []
+        for x in inside:
+            for call in (write, read):
+                assert call(x, 10 * mb) == 27 and call(10 * mb, x) == 27, (kind, x)
+            assert attend(x) == 27, (kind, x)
+        for other in ((at[0], at[0] + pool * size - 16, at[2], at[3]), (at[0], at[0], at[2], at[3])):
+            assert write(10 * mb, 11 * mb, _lib.PagedCacheC(*other, 64, 2, 64, dt)) == 27
+        if dt == 2:
+            assert write(10 * mb, 11 * mb, _lib.PagedCacheC(at[0], at[1], at[2], at[2], 64, 2, 64, dt)) == 27
+
+
 def test_python_wrappers_refuse_host_tensors():
     import torch
     import llm_inference_edu_b200 as qb
