@@ -19,81 +19,98 @@ __global__ void __launch_bounds__(kRowsWarps * 32) attend_rows(const __grid_cons
 }
 
 // Joins the partial results: M = max m_z, y = sum_z o_z 2^(m_z - M) /
-// sum_z l_z 2^(m_z - M).  Few parts: a warp a row, four rows a CTA.  Many
-// (kMergeFew): a CTA a row, the parts dealt to the warps and the warps' sums
-// added in order.  Either way the order is fixed, so the result does not
-// depend on timing.  Bound by latency (few rows) or by the parts' bytes; every load of
-// a warp's parts is independent of the others.
+// sum_z l_z 2^(m_z - M).  Few parts: a warp a row, kMergeWarps rows a CTA.
+// Many (kMergeFew): a CTA a row, the parts dealt to the warps and the warps'
+// sums joined in order.  Either way the order is fixed, so the result does
+// not depend on timing.  Bound by the latency of the parts' loads: eight
+// parts' are under way at once, before their maximum is known (a pass for
+// the maximum first and four at a time took 2 us longer, 80 drafted tokens
+// 22.9 -> 21.0 us; CTAs of two or eight warps were slower).
 
-// Parts z0, z0 + dz, ... of row r: o (V dimensions a lane) and l against the
-// row's maximum, which is returned.
+// Parts z0, z0 + dz, ... of row r: o (V dimensions a lane) and l against
+// their maximum m.  A part that is NaN leaves l or o NaN.
 template <int V>
 __device__ __forceinline__ void merge_parts(const float *w, const Merge &mg, int hd, int r, int z0, int dz, int lane, float (&o)[V],
-                                            float &l) {
+                                            float &m, float &l) {
+    constexpr int N = kMergeFew;
     const float *wm = w + (size_t)mg.rows * hd + r, *wl = wm + mg.rows;
-    float m = -INFINITY;
-    bool nan = false;
-    for (int z = lane; z < mg.parts; z += 32) {
-        const float mz = wm[(size_t)z * mg.stride];
-        m = fmaxf(m, mz);
-        nan |= mz != mz;
-    }
-#pragma unroll
-    for (int off = 16; off; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
-    if (__any_sync(0xffffffffu, nan)) m = __uint_as_float(0x7fffffffu);
-    const float base = m == -INFINITY ? 0.0f : m;
+    m = -INFINITY;
     l = 0.0f;
 #pragma unroll
     for (int i = 0; i < V; ++i) o[i] = 0.0f;
-#pragma unroll 4
-    for (int z = z0; z < mg.parts; z += dz) {
-        const size_t at = (size_t)z * mg.stride;
-        const float f = exp2f(wm[at] - base);
-        l = fmaf(f, wl[at], l);
+#pragma unroll 1
+    for (int z = z0; z < mg.parts; z += N * dz) {
+        float mz[N], lz[N], oz[N][V], mn = m;
 #pragma unroll
-        for (int i = 0; i < V; ++i)
-            if (lane + 32 * i < hd) o[i] = fmaf(f, w[at + part_at(mg.rows, hd, r, lane + 32 * i, mg.quads)], o[i]);
+        for (int x = 0; x < N; ++x) {
+            const bool on = z + x * dz < mg.parts;
+            const size_t at = (size_t)(on ? z + x * dz : z) * mg.stride;
+            mz[x] = on ? wm[at] : -INFINITY;
+            lz[x] = on ? wl[at] : 0.0f;
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                oz[x][i] = on && lane + 32 * i < hd ? w[at + part_at(mg.rows, hd, r, lane + 32 * i, mg.quads)] : 0.0f;
+        }
+#pragma unroll
+        for (int x = 0; x < N; ++x) mn = fmaxf(mn, mz[x]);
+        const float base = mn == -INFINITY ? 0.0f : mn, f = exp2f(m - base);
+        m = mn;
+        l *= f;
+#pragma unroll
+        for (int i = 0; i < V; ++i) o[i] *= f;
+#pragma unroll
+        for (int x = 0; x < N; ++x) {
+            const float e = exp2f(mz[x] - base);
+            l = fmaf(e, lz[x], l);
+#pragma unroll
+            for (int i = 0; i < V; ++i) o[i] = fmaf(e, oz[x][i], o[i]);
+        }
     }
 }
 
 template <typename TV, int V>
 __global__ void __launch_bounds__(kMergeWarps * 32) merge_rows(const __grid_constant__ Args a) {
-    __shared__ float s_o[kMergeWarps][32 * V], s_l[kMergeWarps];
+    __shared__ float s_o[kMergeWarps][32 * V], s_m[kMergeWarps], s_l[kMergeWarps];
     const Merge mg = *(const Merge *)(a.words + a.off_merges + (size_t)blockIdx.x * 8);
     const bool few = mg.parts <= kMergeFew;
     const int r0 = few ? blockIdx.y * kMergeWarps : blockIdx.y;
     if (r0 >= mg.rows) return;  // (other CTAs of this grid wait for the parts)
     const SeqRec sq = *(const SeqRec *)(a.words + a.off_seqs + mg.seq * 4);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, hd = a.hd;
+    auto out = [&](int r) { return (TV *)a.y + row_at(a, sq, mg.kvh, mg.row0 + r, (size_t)a.H * hd); };
     depend_wait();
     const float *w = a.ws + mg.slot;
-    auto out = [&](int r) {
-        const int row = mg.row0 + r;
-        return (TV *)a.y + (((size_t)sq.tok0 + row / a.G) * a.H + (size_t)mg.kvh * a.G + row % a.G) * hd;
-    };
-    float o[V], l;
+    float o[V], m, l;
     if (few) {
         const int r = r0 + warp;
         if (r >= mg.rows) return;
-        merge_parts<V>(w, mg, hd, r, 0, 1, lane, o, l);
+        merge_parts<V>(w, mg, hd, r, 0, 1, lane, o, m, l);
         TV *y = out(r);
 #pragma unroll
         for (int i = 0; i < V; ++i)
             if (lane + 32 * i < hd) store_value(y, lane + 32 * i, __fdiv_rn(o[i], l));
         return;
     }
-    merge_parts<V>(w, mg, hd, r0, warp, kMergeWarps, lane, o, l);
+    merge_parts<V>(w, mg, hd, r0, warp, kMergeWarps, lane, o, m, l);
 #pragma unroll
     for (int i = 0; i < V; ++i) s_o[warp][lane + 32 * i] = o[i];
-    if (lane == 0) s_l[warp] = l;
+    if (lane == 0) {
+        s_m[warp] = m;
+        s_l[warp] = l;
+    }
     __syncthreads();
+    m = s_m[0];
+#pragma unroll
+    for (int x = 1; x < kMergeWarps; ++x) m = fmaxf(m, s_m[x]);
+    const float base = m == -INFINITY ? 0.0f : m;
     TV *y = out(r0);
     for (int d = threadIdx.x; d < hd; d += kMergeWarps * 32) {
         float v = 0.0f, ll = 0.0f;
 #pragma unroll
         for (int x = 0; x < kMergeWarps; ++x) {
-            v += s_o[x][d];
-            ll += s_l[x];
+            const float f = exp2f(s_m[x] - base);
+            v = fmaf(f, s_o[x][d], v);
+            ll = fmaf(f, s_l[x], ll);
         }
         store_value(y, d, __fdiv_rn(v, ll));
     }
