@@ -46,6 +46,11 @@ __device__ __forceinline__ float lg2(float x) {
     return y;
 }
 
+// log2 of a V row's scale as the base counts it: finite whatever the scale.
+__device__ __forceinline__ float scale_log2(float scale) {
+    return fminf(fmaxf(lg2(fabsf(scale)), -kScaleSpan), kScaleSpan);
+}
+
 // The power of two for a row of Q whose largest magnitude has bits mb.
 __device__ __forceinline__ float row_scale(uint32_t mb) {
     return __uint_as_float((267u - min(max(mb >> 23, 27u), 250u)) << 23);

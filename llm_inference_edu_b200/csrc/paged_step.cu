@@ -294,7 +294,7 @@ __global__ void __launch_bounds__(kStepWarps * 32, 3) attend_step(const __grid_c
 #pragma unroll
                 for (int y = 0; y < 2; ++y) {
                     kc[y] = ksc[x][y];
-                    lv[y] = fminf(fmaxf(lg2(fabsf(vsc[x][y])), -kScaleSpan), kScaleSpan);
+                    lv[y] = scale_log2(vsc[x][y]);
                 }
             }
 #pragma unroll

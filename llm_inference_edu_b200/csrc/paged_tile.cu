@@ -604,14 +604,33 @@ __global__ void __launch_bounds__(Tile<TV, TC, HD>::kThreads, 1)
             // A NaN among the visible scores is the row's result.
             if (bm != bm) l2[0].x = bm;
             if constexpr (T::kInt8) {
-                // The weights carry the V scales: at most the tile's largest.
+                // The weights carry the V scales: score and largest scale of
+                // the tile together bound every key's, so the base stays as
+                // it is unless they pass it (after a stream's first tile they
+                // seldom do).  Only then each key's own product is looked at:
+                // the largest scale may be of a key that the row does not see
+                // or hardly weighs, and f16 would drop the others' weights.
                 float vm = 0.0f;
 #pragma unroll
                 for (int e = 0; e < KT; e += 32)
                     if (!none(j0 + e + lane)) vm = fmaxf(vm, fabsf(vs[e + lane]));
 #pragma unroll
                 for (int off = 16; off; off >>= 1) vm = fmaxf(vm, __shfl_xor_sync(0xffffffffu, vm, off));
-                bm += fminf(fmaxf(lg2(vm), -kScaleSpan), kScaleSpan);
+                const bool pass = bm + scale_log2(vm) > m + (8.0f + T::kAbove);
+                bm = -INFINITY;
+                if (__any_sync(0xffffffffu, pass)) {
+#pragma unroll 1
+                    for (int ch = 0; ch < KT / CH; ++ch) {
+                        const float lv = scale_log2(vs[ch * CH + lane]);
+                        uint32_t x[CH];
+                        tmem_ld32(ts + ch * CH, x);
+                        wait_ld();
+                        finish(x, ch);
+#pragma unroll
+                        for (int e = 0; e < CH; ++e)
+                            bm = fmaxf(bm, fmaf(__uint_as_float(x[e]), c, __shfl_sync(0xffffffffu, lv, e)));
+                    }
+                }
             }
             if (__any_sync(0xffffffffu, bm > m + (8.0f + T::kAbove))) {
                 const float mn = fmaxf(m, bm - T::kAbove), f = m == mn ? 1.0f : ex2(m - mn);
