@@ -17,9 +17,11 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
 // of a bf16 value exactly.  f16 lacks range.  So each row of Q is scaled by a
 // power of two to a largest element in 2^13 .. 2^14, and the weights, which
 // carry the V rows' scales, are taken against a base that keeps the largest
-// between 2^7 and 2^15: what f16 drops is below 2^-31 of it.  (V scales under
-// 2^-90 lose precision; where one over 2^90 overflows, the row is done again
-// by attend_row.)
+// between 2^7 and 2^15: what f16 drops is below 2^-31 of it.  The largest is
+// over the keys that the row sees and whose V row has a nonzero byte: a stored
+// row of zeros has scale 1 whatever the others' are.  (Scales under 2^-90, and
+// what is that far below the weight of a row of zeros, lose precision; where
+// one over 2^90 overflows, the row is done again by attend_row.)
 constexpr float kAboveBase = 7.0f, kScaleSpan = 90.0f;
 
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {

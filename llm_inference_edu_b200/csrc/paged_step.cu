@@ -277,11 +277,7 @@ __global__ void __launch_bounds__(kStepWarps * 32, 3) attend_step(const __grid_c
                                 mma16816(s[x][nt], w[0][0], w[1][0], w[0][1], w[1][1], b[pl][nt].x, b[pl][nt].y);
                 }
             }
-        // Scores, masked; this group's maximum of score * log2(e) (the row's
-        // factor c), with log2 of the V row's scale added for INT8.
-        float bm[NT][2];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) bm[nt][0] = bm[nt][1] = -INFINITY;
+        // Scores, masked.
         bool whole[PG], all = true;
 #pragma unroll
         for (int x = 0; x < PG; ++x) {
@@ -289,24 +285,15 @@ __global__ void __launch_bounds__(kStepWarps * 32, 3) attend_step(const __grid_c
             whole[x] = i + x < it.i1 && j0 + kPage - 1 <= p_lo &&
                        (a.window == 0 || j0 > p_hi - a.window || j0 + kPage <= a.sinks);
             all &= whole[x];
-            float kc[2], lv[2];
-            if constexpr (S::kInt8) {
-#pragma unroll
-                for (int y = 0; y < 2; ++y) {
-                    kc[y] = ksc[x][y];
-                    lv[y] = scale_log2(vsc[x][y]);
-                }
-            }
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     float t = s[x][nt][e];
-                    if constexpr (S::kInt8) t *= kc[e >> 1];
+                    if constexpr (S::kInt8) t *= ksc[x][e >> 1];
                     if (!whole[x] && !(i + x < it.i1 && sees(pos[nt][e & 1], j0 + g + (e >> 1) * 8, a.window, a.sinks)))
                         t = -INFINITY;
                     s[x][nt][e] = t;
-                    bm[nt][e & 1] = fmaxf(bm[nt][e & 1], S::kInt8 ? fmaf(t, cr[nt][e & 1], lv[e >> 1]) : t * cr[nt][e & 1]);
                 }
             if (!S::kInt8 && !whole[x]) {
                 // V rows that no row sees may hold anything: 0 * inf is not
@@ -323,22 +310,75 @@ __global__ void __launch_bounds__(kStepWarps * 32, 3) attend_step(const __grid_c
                 }
             }
         }
+        // This group's maximum of score * log2(e) (the row's factor c), with
+        // log2 of the V row's scale added for INT8, and whether it passes the
+        // base.
+        float bm[NT][2];
+        auto passes = [&]() {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) bm[nt][0] = bm[nt][1] = -INFINITY;
+#pragma unroll
+            for (int x = 0; x < PG; ++x) {
+                float lv[2] = {0.0f, 0.0f};
+                if constexpr (S::kInt8) {
+                    lv[0] = scale_log2(vsc[x][0]);
+                    lv[1] = scale_log2(vsc[x][1]);
+                }
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float t = s[x][nt][e], f = cr[nt][e & 1];
+                        bm[nt][e & 1] = fmaxf(bm[nt][e & 1], S::kInt8 ? fmaf(t, f, lv[e >> 1]) : t * f);
+                    }
+            }
+            bool grow = false;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int y = 0; y < 2; ++y) {
+#pragma unroll
+                    for (int off = 4; off < 32; off <<= 1)
+                        bm[nt][y] = fmaxf(bm[nt][y], __shfl_xor_sync(0xffffffffu, bm[nt][y], off));
+                    grow |= bm[nt][y] > m[nt][y] + (8.0f + S::kAbove);
+                }
+            return (bool)__any_sync(0xffffffffu, grow);
+        };
         const int nxt = i + step;
         ids(nxt);
         load_k();
-        bool grow = false;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int y = 0; y < 2; ++y) {
-#pragma unroll
-                for (int off = 4; off < 32; off <<= 1)
-                    bm[nt][y] = fmaxf(bm[nt][y], __shfl_xor_sync(0xffffffffu, bm[nt][y], off));
-                grow |= bm[nt][y] > m[nt][y] + (8.0f + S::kAbove);
-            }
         // The maximum may lag by a factor 2^8 (weights up to 256 are no less
         // exact): the rescaling of O is then rare.
-        if (__any_sync(0xffffffffu, grow)) {
+        bool grow = passes();
+        if constexpr (S::kInt8)
+            if (grow) {
+                // A V row of zeros must not set the base, whose scale says
+                // nothing: taken as 0 it counts as the smallest, which keeps
+                // the row's sum in range (a scale that is not finite makes
+                // the result NaN and stays).  V is there only now: where the
+                // base stays, nothing waits for it before the products.
+#pragma unroll
+                for (int x = 0; x < PG; ++x) {
+                    uint32_t full[4];
+#pragma unroll
+                    for (int y = 0; y < 4; ++y) {
+                        uint32_t any = 0u;
+#pragma unroll
+                        for (int j = 0; j < VW / VP; ++j)
+#pragma unroll
+                            for (int z = 0; z < VP; ++z) any |= vr[x][y][j][z];
+                        full[y] = __ballot_sync(0xffffffffu, any != 0u);
+                    }
+                    // Key 2 c + (y & 1) + (y >> 1) * 8 is row y of the lanes
+                    // with that c; this thread's scales are of g and g + 8.
+                    const uint32_t lanes = 0x11111111u << (g >> 1);
+#pragma unroll
+                    for (int y = 0; y < 2; ++y)
+                        if (!((g & 1 ? full[2 * y + 1] : full[2 * y]) & lanes) && isfinite(vsc[x][y])) vsc[x][y] = 0.0f;
+                }
+                grow = passes();
+            }
+        if (grow) {
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll

@@ -544,11 +544,12 @@ __global__ void __launch_bounds__(Tile<TV, TC, HD>::kThreads, 1)
             // The products issued before these scores are then done too.
             if (!(ok = __all_sync(0xffffffffu, wait(&ctl->s_full[s], (uint32_t)(n & 1), ctl)))) break;
             fence_after();
-            const float *ks = nullptr, *vs = nullptr;
+            const float *ks = nullptr;
+            float *vs = nullptr;
             if constexpr (T::kInt8) {
                 if (!(ok = __all_sync(0xffffffffu, wait(&ctl->scl_full[i % D], (uint32_t)((i / D) & 1), ctl)))) break;
                 ks = s_scl + (i % D * 2) * KT;
-                vs = ks + KT;
+                vs = s_scl + (i % D * 2 + 1) * KT;
             }
             // Key e of the tile is visible up to e_hi, and then above e_lo or below e_sk.
             const int e_hi = pos - j0, e_lo = a.window ? pos - a.window - j0 : -1, e_sk = a.window ? a.sinks - j0 : 0;
@@ -616,20 +617,59 @@ __global__ void __launch_bounds__(Tile<TV, TC, HD>::kThreads, 1)
                     if (!none(j0 + e + lane)) vm = fmaxf(vm, fabsf(vs[e + lane]));
 #pragma unroll
                 for (int off = 16; off; off >>= 1) vm = fmaxf(vm, __shfl_xor_sync(0xffffffffu, vm, off));
-                const bool pass = bm + scale_log2(vm) > m + (8.0f + T::kAbove);
+                const float top = m + (8.0f + T::kAbove);
+                const bool pass = bm + scale_log2(vm) > top;
                 bm = -INFINITY;
                 if (__any_sync(0xffffffffu, pass)) {
 #pragma unroll 1
-                    for (int ch = 0; ch < KT / CH; ++ch) {
-                        const float lv = scale_log2(vs[ch * CH + lane]);
-                        uint32_t x[CH];
-                        tmem_ld32(ts + ch * CH, x);
-                        wait_ld();
-                        finish(x, ch);
+                    for (bool first = true;; first = false) {
+                        bm = -INFINITY;
+#pragma unroll 1
+                        for (int ch = 0; ch < KT / CH; ++ch) {
+                            const float lv = scale_log2(vs[ch * CH + lane]);
+                            uint32_t x[CH];
+                            tmem_ld32(ts + ch * CH, x);
+                            wait_ld();
+                            finish(x, ch);
 #pragma unroll
-                        for (int e = 0; e < CH; ++e)
-                            bm = fmaxf(bm, fmaf(__uint_as_float(x[e]), c, __shfl_sync(0xffffffffu, lv, e)));
+                            for (int e = 0; e < CH; ++e)
+                                bm = fmaxf(bm, fmaf(__uint_as_float(x[e]), c, __shfl_sync(0xffffffffu, lv, e)));
+                        }
+                        if (!first || !__any_sync(0xffffffffu, bm > top)) break;
+                        // Nor may a V row of zeros set the base, whose scale
+                        // says nothing.  The tile's V rows are widened
+                        // without these weights; each lane looks at four.
+                        if (!(ok = __all_sync(0xffffffffu, wait(&ctl->v_full[i % NS], (uint32_t)((i / NS) & 1), ctl)))) break;
+                        const uint8_t *v = s_v + (size_t)(i % NS) * T::kTileBytes;
+                        uint32_t zero = 0u;
+#pragma unroll
+                        for (int ch = 0; ch < KT / CH; ++ch) {
+                            // (One 16-byte piece of the row nearly always says it.)
+                            const int key = ch * CH + lane;
+                            const uint4 w = *(const uint4 *)(v + key / kPage * (PN * kPage * 128) + key % kPage * 128 + (lane & 7) * 16);
+                            zero |= (w.x | w.y | w.z | w.w) == 0u ? 1u << ch : 0u;
+                        }
+                        if (!__any_sync(0xffffffffu, zero)) break;
+#pragma unroll 1
+                        for (int ch = 0; ch < KT / CH; ++ch) {
+                            const int key = ch * CH + lane;
+                            uint32_t any = 0u;
+#pragma unroll 1
+                            for (int y = 0; y < PN * 8; ++y) {
+                                const uint4 w = *(const uint4 *)(v + (key / kPage * PN + y / 8) * (kPage * 128) + key % kPage * 128 + ((y + lane) & 7) * 16);
+                                any |= w.x | w.y | w.z | w.w;
+                            }
+                            // Taken as 0 the scale counts as the smallest,
+                            // which keeps the row's sum in range; one that is
+                            // not finite makes the result NaN and stays.  (The
+                            // other warps of this tile may read either.)
+                            if (!any && isfinite(vs[key])) vs[key] = 0.0f;
+                        }
+                        // The slot's next copy comes through the async proxy.
+                        fence_proxy_async_smem();
+                        __syncwarp();
                     }
+                    if (!ok) break;
                 }
             }
             if (__any_sync(0xffffffffu, bm > m + (8.0f + T::kAbove))) {

@@ -79,3 +79,51 @@ def test_value_scales_of_keys_with_little_weight(values, hd, octaves, down):
         scale_values(s, i, p, octaves)
     s.refresh()
     s.check()
+
+
+def written(starts, counts, heads, hd, values, size, zeros, seed):
+    """A step whose whole sequences went through kv_write: V about `size`,
+    its rows zero at the positions `zeros` (a function of a sequence)."""
+    import torch
+    import llm_inference_edu_b200 as qb
+    s = Step(starts, counts, heads, 2, hd, values, "int8", seed=seed)
+    ends = [a + c for a, c in zip(starts, counts)]
+    rng = np.random.default_rng(seed + 1)
+    x = rng.standard_normal((2, sum(ends), 2, hd)).astype(np.float32)
+    x[1] *= size
+    for i, e in enumerate(ends):
+        rows = x[1, sum(ends[:i]):sum(ends[:i]) + e]
+        rows[[p for p in zeros(i) if p < e]] = 0
+    k, v = (torch.from_numpy(t).to(s.q.dtype).cuda() for t in x)
+    qb.kv_write(k, v, s.cache, qb.PagedPlan(s.cache, s.tables, [0] * len(ends), ends, heads, dtype=values))
+    s.refresh()
+    return s
+
+
+@pytest.mark.parametrize("values,hd", SIZES)
+@pytest.mark.parametrize("size", [1.0, 1e-2, 1e-3, 1e-5, 1e-7, 1e-9, 1e-18])
+def test_value_rows_of_zeros(values, hd, size):
+    """A stored row of zeros has scale 1 whatever the others' scales are."""
+    starts, counts = [40, 0, 300, 129, 90, 2500], [60, 30, 1, 2, 150, 1]
+    few = lambda i: [5, 17, 33, 34, 100, 131] if i != 4 else range(32, 200)  # noqa: E731 (whole pages and tiles of zeros)
+    written(starts, counts, 14, hd, values, size, few, seed=3).check()
+
+
+@pytest.mark.parametrize("values,hd", SIZES)
+@pytest.mark.parametrize("size", [1.0, 1e-4, 1e-9])
+@pytest.mark.parametrize("up", [25, 45])
+def test_value_row_of_zeros_with_most_of_the_weight(values, hd, size, up):
+    """A first token that takes the attention and has no value: what is left
+    of the others is small, and exact."""
+    s = written(STARTS, COUNTS, 14, hd, values, size, lambda i: [0], seed=up)
+    shift_scores(s, [(i, 0) for i in range(len(STARTS))], up)
+    s.refresh()
+    s.check()
+
+
+@pytest.mark.parametrize("values,hd", SIZES)
+def test_values_that_are_all_zero(values, hd):
+    s = written(STARTS, COUNTS, 14, hd, values, 1.0, lambda i: range(300), seed=1)
+    got = s.attend()
+    seen = np.repeat(STARTS, COUNTS) < 300
+    assert seen.sum() == sum(COUNTS) - 1 and (got[seen] == 0).all()
