@@ -91,6 +91,12 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
+// The square root of 2^x.  Sums of weights are brought to another base by its
+// two factors: over INT8 pages a base holds a V row's scale, so two may lie
+// further apart than a float reaches while both sums count.  (A context under
+// the lower base is then nothing next to the other's.)
+__device__ __forceinline__ float ex2_half(float x) { return ex2(0.5f * x); }
+
 // The kernels of one call follow each other by programmatic dependent launch:
 // a kernel may start while the one before it still runs.  depend_wait waits
 // for everything before to be complete; a kernel that writes only its own

@@ -53,15 +53,16 @@ __device__ __forceinline__ void merge_parts(const float *w, const Merge &mg, int
         }
 #pragma unroll
         for (int x = 0; x < N; ++x) mn = fmaxf(mn, mz[x]);
-        const float base = mn == -INFINITY ? 0.0f : mn, f = exp2f(m - base);
+        // (In two factors: ex2_half.)
+        const float base = mn == -INFINITY ? 0.0f : mn, h = exp2f(0.5f * (m - base)), f = h * h;
         m = mn;
-        l *= f;
+        l = l * h * h;
 #pragma unroll
         for (int i = 0; i < V; ++i) o[i] *= f;
 #pragma unroll
         for (int x = 0; x < N; ++x) {
-            const float e = exp2f(mz[x] - base);
-            l = fmaf(e, lz[x], l);
+            const float hx = exp2f(0.5f * (mz[x] - base)), e = hx * hx;
+            l = fmaf(lz[x] * hx, hx, l);
 #pragma unroll
             for (int i = 0; i < V; ++i) o[i] = fmaf(e, oz[x][i], o[i]);
         }
@@ -108,9 +109,9 @@ __global__ void __launch_bounds__(kMergeWarps * 32) merge_rows(const __grid_cons
         float v = 0.0f, ll = 0.0f;
 #pragma unroll
         for (int x = 0; x < kMergeWarps; ++x) {
-            const float f = exp2f(s_m[x] - base);
-            v = fmaf(f, s_o[x][d], v);
-            ll = fmaf(f, s_l[x], ll);
+            const float h = exp2f(0.5f * (s_m[x] - base));
+            v = fmaf(h * h, s_o[x][d], v);
+            ll = fmaf(s_l[x] * h, h, ll);
         }
         store_value(y, d, __fdiv_rn(v, ll));
     }

@@ -384,9 +384,9 @@ __global__ void __launch_bounds__(kStepWarps * 32, 3) attend_step(const __grid_c
 #pragma unroll
                 for (int y = 0; y < 2; ++y) {
                     const float mn = fmaxf(m[nt][y], bm[nt][y] - S::kAbove);
-                    const float f = m[nt][y] == mn ? 1.0f : ex2(m[nt][y] - mn);
+                    const float h = m[nt][y] == mn ? 1.0f : ex2_half(m[nt][y] - mn), f = h * h;
                     m[nt][y] = mn;
-                    l[nt][y] *= f;
+                    l[nt][y] = l[nt][y] * h * h;
 #pragma unroll
                     for (int t = 0; t < MT; ++t) {
                         o[nt][t][y] *= f;
@@ -521,8 +521,9 @@ __global__ void __launch_bounds__(kStepWarps * 32, 3) attend_step(const __grid_c
         float f[kStepWarps], ll = 0.0f;
 #pragma unroll
         for (int w = 0; w < kStepWarps; ++w) {
-            f[w] = s_m[w][r] == base ? 1.0f : ex2(s_m[w][r] - base);
-            ll = fmaf(f[w], s_l[w][r], ll);
+            const float h = s_m[w][r] == base ? 1.0f : ex2_half(s_m[w][r] - base);
+            f[w] = h * h;
+            ll = fmaf(s_l[w][r] * h, h, ll);
         }
         const size_t at = row_at(a, sq, it.kvh, it.row0 + r, (size_t)a.H * HD);
 #pragma unroll

@@ -267,9 +267,10 @@ __device__ __forceinline__ Join join(float m0, float l0, float m1, float l1) {
     Join j;
     j.m = fmaxf(m0, m1);
     const float base = j.m == -INFINITY ? 0.0f : j.m;
-    j.f0 = m0 == base ? 1.0f : ex2(m0 - base);
-    j.f1 = m1 == base ? 1.0f : ex2(m1 - base);
-    j.l = j.f0 * l0 + j.f1 * l1;
+    const float h0 = m0 == base ? 1.0f : ex2_half(m0 - base), h1 = m1 == base ? 1.0f : ex2_half(m1 - base);
+    j.f0 = h0 * h0;
+    j.f1 = h1 * h1;
+    j.l = l0 * h0 * h0 + l1 * h1 * h1;
     return j;
 }
 
@@ -673,10 +674,10 @@ __global__ void __launch_bounds__(Tile<TV, TC, HD>::kThreads, 1)
                 }
             }
             if (__any_sync(0xffffffffu, bm > m + (8.0f + T::kAbove))) {
-                const float mn = fmaxf(m, bm - T::kAbove), f = m == mn ? 1.0f : ex2(m - mn);
+                const float mn = fmaxf(m, bm - T::kAbove), h = m == mn ? 1.0f : ex2_half(m - mn), f = h * h;
                 m = mn;
 #pragma unroll
-                for (int e = 0; e < 2; ++e) l2[e] = mul2(l2[e], make_float2(f, f));
+                for (int e = 0; e < 2; ++e) l2[e] = mul2(mul2(l2[e], make_float2(h, h)), make_float2(h, h));
                 if (!T::kWide && n > 0) {
 #pragma unroll 1
                     for (int d = 0; d < HD; d += 16) {

@@ -127,3 +127,31 @@ def test_values_that_are_all_zero(values, hd):
     got = s.attend()
     seen = np.repeat(STARTS, COUNTS) < 300
     assert seen.sum() == sum(COUNTS) - 1 and (got[seen] == 0).all()
+
+
+@pytest.mark.parametrize("values,hd", SIZES)
+@pytest.mark.parametrize("order", ["small first", "large first", "mixed", "zeros first"])
+def test_value_scales_further_apart_than_a_float(values, hd, order):
+    """Equal weights of values that differ by 2^150: the small ones count in
+    the denominator.  (Zeros first: rows of zeros, then scales of 2^60.)"""
+    import torch
+    starts, counts = [40, 0, 300, 129, 90, 6000], [60, 30, 1, 2, 150, 1]
+    s = Step(starts, counts, 14, 2, hd, values, "int8", seed=7)
+    rng = np.random.default_rng(5)
+    c = s.cache
+    for i, (a, n) in enumerate(zip(starts, counts)):
+        for j, page in enumerate(s.tables[i][:-(-(a + n) // 16)]):
+            late = j * 32 >= a + n
+            if order == "zeros first":
+                if late:
+                    c.v_scales[page] *= 2.0**60
+                else:
+                    c.v[page] = 0
+                    c.v_scales[page] = 1.0
+                continue
+            up = torch.from_numpy(rng.choice([-75.0, 75.0], (2, 16))).float().cuda()
+            if order != "mixed":
+                up[:] = 75.0 if late == (order == "small first") else -75.0
+            c.v_scales[page] *= torch.exp2(up)
+    s.refresh()
+    s.check()
