@@ -48,6 +48,11 @@ __device__ __forceinline__ float lg2(float x) {
     return y;
 }
 
+// Whether a K row's scale may take a score out of a float's range (a product of
+// scaled Q and bytes is below 2^28).  Rows that see one are done again by
+// attend_row; elsewhere a score of -inf means a hidden key.
+__device__ __forceinline__ bool wild_scale(float scale) { return !(fabsf(scale) <= 0x1p99f); }
+
 // log2 of a V row's scale as the base counts it: finite whatever the scale.
 __device__ __forceinline__ float scale_log2(float scale) {
     return fminf(fmaxf(lg2(fabsf(scale)), -kScaleSpan), kScaleSpan);

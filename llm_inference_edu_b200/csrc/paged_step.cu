@@ -230,6 +230,7 @@ __global__ void __launch_bounds__(kStepWarps * 32, 3) attend_step(const __grid_c
             for (int e = 0; e < 4; ++e) o[nt][t][e] = 0.0f;
     }
 
+    bool bad = false;
 #pragma unroll 1
     for (; i < it.i1; i += step) {
         float s[PG][NT][4];
@@ -291,8 +292,13 @@ __global__ void __launch_bounds__(kStepWarps * 32, 3) attend_step(const __grid_c
                 for (int e = 0; e < 4; ++e) {
                     float t = s[x][nt][e];
                     if constexpr (S::kInt8) t *= ksc[x][e >> 1];
-                    if (!whole[x] && !(i + x < it.i1 && sees(pos[nt][e & 1], j0 + g + (e >> 1) * 8, a.window, a.sinks)))
-                        t = -INFINITY;
+                    if (!whole[x]) {
+                        // A visible key's -inf would pass for a hidden key.
+                        if (i + x < it.i1 && sees(pos[nt][e & 1], j0 + g + (e >> 1) * 8, a.window, a.sinks))
+                            bad |= S::kInt8 && t == -INFINITY;
+                        else
+                            t = -INFINITY;
+                    }
                     s[x][nt][e] = t;
                 }
             if (!S::kInt8 && !whole[x]) {
@@ -477,7 +483,6 @@ __global__ void __launch_bounds__(kStepWarps * 32, 3) attend_step(const __grid_c
     // A result that is not finite may be a hidden value's doing (a key that
     // only some of the rows see, with weight 0 in the others) or the planes'
     // (an infinity times planes of both signs): such items go row by row.
-    bool bad = false;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -524,6 +529,11 @@ __global__ void __launch_bounds__(kStepWarps * 32, 3) attend_step(const __grid_c
             const float h = s_m[w][r] == base ? 1.0f : ex2_half(s_m[w][r] - base);
             f[w] = h * h;
             ll = fmaf(s_l[w][r] * h, h, ll);
+        }
+        if (S::kInt8 && ll == 0.0f) {
+            // It sees no key of these, or all scores left a float's range.
+            attend_row<TV, TC>(a, item, r, kPage, lane);
+            continue;
         }
         const size_t at = row_at(a, sq, it.kvh, it.row0 + r, (size_t)a.H * HD);
 #pragma unroll

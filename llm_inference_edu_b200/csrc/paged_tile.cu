@@ -537,7 +537,7 @@ __global__ void __launch_bounds__(Tile<TV, TC, HD>::kThreads, 1)
         const float c = T::kInt8 ? ctl->c[r] : a.c;
         float m = -INFINITY;   // in units of log2
         float2 l2[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
-        bool ok = true;
+        bool ok = true, wild = false;
 #pragma unroll 1
         for (int n = 0; n < n_steps; ++n) {
             const int i = shared ? n : 2 * n + s, j0 = key0(i);
@@ -615,7 +615,10 @@ __global__ void __launch_bounds__(Tile<TV, TC, HD>::kThreads, 1)
                 float vm = 0.0f;
 #pragma unroll
                 for (int e = 0; e < KT; e += 32)
-                    if (!none(j0 + e + lane)) vm = fmaxf(vm, fabsf(vs[e + lane]));
+                    if (!none(j0 + e + lane)) {
+                        vm = fmaxf(vm, fabsf(vs[e + lane]));
+                        wild |= wild_scale(ks[e + lane]);
+                    }
 #pragma unroll
                 for (int off = 16; off; off >>= 1) vm = fmaxf(vm, __shfl_xor_sync(0xffffffffu, vm, off));
                 const float top = m + (8.0f + T::kAbove);
@@ -711,21 +714,13 @@ __global__ void __launch_bounds__(Tile<TV, TC, HD>::kThreads, 1)
                     p[e].x = ex2(p[e].x);
                     p[e].y = ex2(p[e].y);
                     l2[e & 1] = add2(l2[e & 1], p[e]);
-                }
-                if constexpr (T::kInt8) {
-#pragma unroll
-                    for (int e = 0; e < CH / 2; e += 2) {
-                        const float4 f = *(const float4 *)(vs + ch * CH + 2 * e);
-                        const float2 u = mul2(p[e], make_float2(f.x, f.y)), w = mul2(p[e + 1], make_float2(f.z, f.w));
-                        if (whole) {
-                            p[e] = u;
-                            p[e + 1] = w;
-                        } else {
-                            // A hidden key's scale may be anything.
-                            p[e].x = p[e].x == 0.0f ? 0.0f : u.x;
-                            p[e].y = p[e].y == 0.0f ? 0.0f : u.y;
-                            p[e + 1].x = p[e + 1].x == 0.0f ? 0.0f : w.x;
-                            p[e + 1].y = p[e + 1].y == 0.0f ? 0.0f : w.y;
+                    if constexpr (T::kInt8) {
+                        p[e] = mul2(p[e], *(const float2 *)(vs + ch * CH + 2 * e));
+                        if (!whole) {
+                            // A hidden key's scale may be anything.  (A visible
+                            // one's NaN is the result's, whatever the weight.)
+                            p[e].x = x[2 * e] == 0xff800000u ? 0.0f : p[e].x;
+                            p[e].y = x[2 * e + 1] == 0xff800000u ? 0.0f : p[e].y;
                         }
                     }
                 }
@@ -768,6 +763,7 @@ __global__ void __launch_bounds__(Tile<TV, TC, HD>::kThreads, 1)
         const float2 lsum = add2(l2[0], l2[1]);
         const float l = lsum.x + lsum.y;
         const bool fin = __all_sync(0xffffffffu, wait_issued(&ctl->done, 0u) && ok && !ctl->abort_);
+        if (T::kInt8 && __any_sync(0xffffffffu, wild) && fin && r < it.rows) ctl->bad[r] = 1;
         fence_after();
         // Every copy and product has ended: stream 1's sums (and, where O is
         // not gathered, its O) for whoever writes the rows both streams had.

@@ -155,3 +155,43 @@ def test_value_scales_further_apart_than_a_float(values, hd, order):
             c.v_scales[page] *= torch.exp2(up)
     s.refresh()
     s.check()
+
+
+@pytest.mark.parametrize("values,hd", SIZES)
+@pytest.mark.parametrize("how", ["far below", "-inf"])
+def test_nan_scale_of_a_key_without_weight(values, hd, how):
+    """0 * NaN is NaN for every row that sees the key, wherever its page and
+    its tile end, and no other row notices."""
+    starts, counts = [40, 0, 300, 129, 90, 3], [60, 30, 1, 2, 150, 1]
+    where = [(0, 70), (0, 42), (1, 29), (2, 300), (3, 130), (4, 160), (5, 2)]
+    s = Step(starts, counts, 14, 2, hd, values, "int8", seed=12)
+    if how == "far below":
+        shift_scores(s, where, -300)
+    s.refresh()
+    want, bound = s.want()
+    spoiled = np.zeros(sum(counts), bool)
+    for i, p in where:
+        page, row = place(s, i, p)
+        s.cache.v_scales[page, :, row] = float("nan")
+        if how == "-inf":
+            # Scores of -inf, or of +inf, which make the row NaN by themselves.
+            s.cache.k_scales[page, :, row] = float("inf")
+        t0 = sum(counts[:i])
+        spoiled[t0 + max(p - starts[i], 0):t0 + counts[i]] = True
+    got = s.attend()
+    assert np.isnan(got[spoiled]).all()
+    assert (np.abs(got - want) <= bound)[~spoiled].all()
+
+
+@pytest.mark.parametrize("values,hd", SIZES)
+def test_scores_that_are_large_before_their_factor(values, hd):
+    """Tiny queries, huge keys: scaled Q times bytes times the key's scale
+    passes a float's range, the score itself does not.  A token that sees
+    only such scores, all negative, still has its result."""
+    starts, counts = [0, 0, 40, 0, 129], [1, 40, 60, 2, 1]
+    s = Step(starts, counts, 14, 2, hd, values, "int8", seed=21)
+    s.q.mul_(2.0**-100)
+    s.rows[:, :14] = s.q.float().cpu().numpy()
+    s.cache.k_scales.mul_(2.0**115)
+    s.refresh()
+    s.check()
