@@ -327,8 +327,9 @@ uint32_t qb_kv_read(const qb_paged_cache *cache, const qb_paged_plan *plan, cons
  * `workspace`: at least the plan's workspace_bytes, its content on entry
  * irrelevant; calls that can overlap in time need one each.
  * K's and V's pools may be the same memory.
- * QB_INVALID_PARAMETERS: scale not finite and positive, or Y shares memory
- * with Q (rows are read again where a result is not finite) or the cache. */
+ * QB_INVALID_PARAMETERS: scale not positive, or scale * log2(e) not finite in
+ * FP32; Y shares memory with Q (rows are read again where a result is not
+ * finite) or the cache. */
 uint32_t qb_paged_attention(const void *q, size_t q_len, size_t q_stride, const qb_paged_cache *cache,
                             const qb_paged_plan *plan, const int32_t *words, void *y, size_t y_len,
                             float scale, void *workspace, size_t workspace_bytes, void *stream);

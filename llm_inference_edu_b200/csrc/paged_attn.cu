@@ -154,7 +154,9 @@ uint32_t qb_paged_attention(const void *q, size_t q_len, size_t q_stride, const 
     const size_t width = plan->query_heads * plan->head_dim;
     if ((s = admit_rows(0, q_len, q_stride, width, plan->tokens))) return s;
     if ((s = admit_rows(2, y_len, width, width, plan->tokens))) return s;
-    if (!q || !y || !(isfinite(scale) && scale > 0.0f)) return QB_INVALID_PARAMETERS;
+    // Scores are taken in units of log2.
+    const float c = (float)((double)scale * 1.4426950408889634);
+    if (!q || !y || !(isfinite(c) && scale > 0.0f)) return QB_INVALID_PARAMETERS;
     const size_t size = plan->value_dtype == QB_PAGED_F32 ? 4 : 2;
     if (rows_meet(q, q_stride, y, width, width, plan->tokens, size) ||
         rows_in_cache(y, width, width, plan->tokens, size, cache))
@@ -177,7 +179,7 @@ uint32_t qb_paged_attention(const void *q, size_t q_len, size_t q_stride, const 
     // A window as long as a table row hides nothing.
     a.window = plan->window < plan->pages_per_sequence * kPage ? (int)plan->window : 0;
     a.sinks = (int)(plan->sinks < 0x7fffffffu ? plan->sinks : 0x7fffffffu);
-    a.c = (float)((double)scale * 1.4426950408889634);
+    a.c = c;
     a.q = q;
     a.q_stride = q_stride;
     a.y = y;
