@@ -323,7 +323,8 @@ def _paged_plan_words(tables, starts, counts, pages, kv_heads, head_dim, query_h
                            tables.shape[1], pages, kv_heads, head_dim, query_heads, window, sinks,
                            PAGED_DTYPES[value_dtype], PAGED_DTYPES[cache_dtype])
     plan = _lib.PagedPlanC()
-    size = 4096 + 4 * tables.size + 2 * int(counts.sum(dtype=np.int64))
+    # A guess; more tokens than the tables hold are refused whatever it is.
+    size = 4096 + 4 * tables.size + 2 * min(int(counts.sum(dtype=np.int64)), PAGE_TOKENS * tables.size)
     while True:
         words = np.empty(size, dtype=np.int32)
         status = lib().qb_paged_plan_build(C.byref(step), words.ctypes.data, size, C.byref(plan))
