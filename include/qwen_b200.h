@@ -327,6 +327,9 @@ uint32_t qb_kv_read(const qb_paged_cache *cache, const qb_paged_plan *plan, cons
  * `workspace`: at least the plan's workspace_bytes, its content on entry
  * irrelevant; calls that can overlap in time need one each.
  * K's and V's pools may be the same memory.
+ * The waits inside a kernel are bounded: a block of rows whose operands do
+ * not arrive within two seconds (a GPU given to others for so long) comes out
+ * as NaN; nothing else reports it.
  * QB_INVALID_PARAMETERS: scale not positive, or scale * log2(e) not finite in
  * FP32; Y shares memory with Q (rows are read again where a result is not
  * finite) or the cache. */

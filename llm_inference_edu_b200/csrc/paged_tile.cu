@@ -279,10 +279,13 @@ __device__ __forceinline__ Join join(float m0, float l0, float m1, float l1) {
 // sum.  Results go through shared memory (`stage`, 32 rows 144 bytes apart),
 // so that eight lanes write a row's 128 bytes (a lane a row: 80 against 75 us
 // on 2,001 tokens under a window of 1,001, with Q's loads four at a time).
+// An item that gave up (`fin` unset) leaves NaN, and not through shared
+// memory, where copies may still be landing.
 template <typename TV, int HD>
 __device__ __forceinline__ void put_rows(const Args &a, const Item &it, const SeqRec &sq, int r, int d,
-                                         float (&v)[128 / sizeof(TV)], float m, float l, uint8_t *stage, int lane) {
+                                         float (&v)[128 / sizeof(TV)], float m, float l, bool fin, uint8_t *stage, int lane) {
     constexpr int CB = 128 / (int)sizeof(TV);
+    if (!fin) l = __uint_as_float(0x7fffffffu);
     if (it.slot >= 0) {
         if (r >= it.rows) return;
 #pragma unroll
@@ -298,7 +301,7 @@ __device__ __forceinline__ void put_rows(const Args &a, const Item &it, const Se
     const float inv = __fdiv_rn(1.0f, l);
 #pragma unroll
     for (int e = 0; e < CB; ++e) v[e] *= inv;
-    if ((uintptr_t)a.y & 15) {
+    if (!fin || ((uintptr_t)a.y & 15)) {
         if (r < it.rows)
 #pragma unroll
             for (int e = 0; e < CB; ++e) store_value((TV *)a.y, at + e, v[e]);
@@ -762,7 +765,7 @@ __global__ void __launch_bounds__(Tile<TV, TC, HD>::kThreads, 1)
         }
         const float2 lsum = add2(l2[0], l2[1]);
         const float l = lsum.x + lsum.y;
-        const bool fin = __all_sync(0xffffffffu, wait_issued(&ctl->done, 0u) && ok && !ctl->abort_);
+        bool fin = __all_sync(0xffffffffu, wait_issued(&ctl->done, 0u) && ok && !ctl->abort_);
         if (T::kInt8 && __any_sync(0xffffffffu, wild) && fin && r < it.rows) ctl->bad[r] = 1;
         fence_after();
         // Every copy and product has ended: stream 1's sums (and, where O is
@@ -783,6 +786,8 @@ __global__ void __launch_bounds__(Tile<TV, TC, HD>::kThreads, 1)
                 }
             }
             asm volatile("bar.sync 1, %0;" ::"n"(T::kWide ? 384 : 256) : "memory");
+            // The other stream may have given up: what it left is not read.
+            fin = __all_sync(0xffffffffu, fin && !ctl->abort_);
         }
         if constexpr (!T::kWide) if (shared || s == 0) {
             Join j = {m, l, 1.0f, 0.0f};
@@ -803,8 +808,7 @@ __global__ void __launch_bounds__(Tile<TV, TC, HD>::kThreads, 1)
                         bad |= !isfinite(v[h + e]);
                     }
                 }
-                put_rows<uint16_t, HD>(a, it, sq, r, d, v, j.m, fin ? j.l : __uint_as_float(0x7fffffffu),
-                                       s_k + T::stage_off + warp * 4608, lane);
+                put_rows<uint16_t, HD>(a, it, sq, r, d, v, j.m, j.l, fin, s_k + T::stage_off + warp * 4608, lane);
             }
             if (bad && fin && r < it.rows) ctl->bad[r] = 1;
         }
@@ -848,8 +852,8 @@ __global__ void __launch_bounds__(Tile<TV, TC, HD>::kThreads, 1)
                 fence_before();
                 mbar_arrive(&ctl->o_empty[s]);
             }
-            const bool fin = __all_sync(0xffffffffu, ok);
             asm volatile("bar.sync 1, 384;" ::: "memory");
+            const bool fin = __all_sync(0xffffffffu, ok && !ctl->abort_);
             const float *s_ml = (const float *)s_k + 128 * (HD + 4);
             const Join j = join(s_ml[r], s_ml[128 + r], s_ml[256 + r], s_ml[384 + r]);
             bool bad = false;
@@ -862,8 +866,7 @@ __global__ void __launch_bounds__(Tile<TV, TC, HD>::kThreads, 1)
                     v[e + 1] = o[(d + e) / 2].y;
                     bad |= !isfinite(v[e]) | !isfinite(v[e + 1]);
                 }
-                put_rows<float, HD>(a, it, sq, r, d, v, j.m, fin ? j.l : __uint_as_float(0x7fffffffu),
-                                    s_k + T::stage_off + (warp - T::kGather) * 4608, lane);
+                put_rows<float, HD>(a, it, sq, r, d, v, j.m, j.l, fin, s_k + T::stage_off + (warp - T::kGather) * 4608, lane);
             }
             if (bad && fin && r < it.rows) ctl->bad[r] = 1;
         }
@@ -979,6 +982,9 @@ __global__ void __launch_bounds__(Tile<TV, TC, HD>::kThreads, 1)
                 if (!two || s == 1) commit(&ctl->v_empty[st], leader);
                 if (t + 2 < total) scores(t + 2);
             }
+            // Whoever sees `done` sees that this warp gave up.
+            __threadfence_block();
+            __syncwarp();
             commit(&ctl->done, leader);
             __syncwarp();
         } else if (warp == 10) {
