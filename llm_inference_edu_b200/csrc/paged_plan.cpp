@@ -213,7 +213,8 @@ uint32_t build(const qb_paged_step &s, int32_t *words, size_t capacity, qb_paged
         tokens += s.counts[i];
     }
     if (!tokens) return QB_ZERO_DIMENSION;
-    if (mul_ovf(tokens, s.query_heads, &rows) || rows > 0x3fffffffu || s.pages_per_sequence > 0x07ffffffu)
+    if (mul_ovf(tokens, s.query_heads, &rows) || rows > 0x3fffffffu ||
+        s.pages_per_sequence > 0x07fffff0u)  // (a tile past the last position is still an int32)
         return QB_DIMENSION_OVERFLOW;
     // Every page that a call of this plan touches: what the new tokens see
     // and what they are.  Entries of pages that left the window are not read.
