@@ -47,10 +47,9 @@ __device__ __forceinline__ size_t part_at(int rows, int hd, int r, int d, bool q
     return quads ? ((size_t)(d >> 2) * rows + r) * 4 + (d & 3) : (size_t)r * hd + d;
 }
 
-// Row blocks of the step kernel (mma.sync, one block of 8 rows per n8 tile)
-// and of the tile kernel (tcgen05, 128 rows an MMA); key units of each.
-// A sequence goes to the step kernel up to kStepRows rows: with more, the
-// step kernel would read the cache more than once.
+// A sequence goes to the step kernel (mma.sync, 8 rows an n8 tile) up to this
+// many packed rows: with more, the step kernel would read the cache more than
+// once.  Others go to the tile kernel (tcgen05, 128 rows an MMA).
 constexpr int kStepRows = 16;
 // The merge kernel's warps a CTA, and the parts up to which one takes a row.
 constexpr int kMergeWarps = 4, kMergeFew = 8;

@@ -22,8 +22,10 @@ struct RowArgs {
 
 constexpr int kRowWarps = 8;
 
-// A row's scale is its largest magnitude times this (one rounding, so within
-// a unit in the last place of the quotient by 127).
+// A row's scale is its largest magnitude times this.  Next to the quotient by
+// 127 (qb_quantize_int8's) it differs in the last place for 4 % of rows, and a
+// byte may differ where x / scale is that close to a half; either is within
+// half a scale of x.
 constexpr float kStep = 1.0f / 127.0f;
 
 // One warp a row, in any alignment: the row sits in registers between the
@@ -85,10 +87,11 @@ __global__ void __launch_bounds__(kRowWarps * 32) kv_read_rows(const __grid_cons
 }
 
 // The same in 16-byte pieces of the values, where widths and alignment allow
-// (lanes: pieces a row, a power of two up to 32).  Bound by HBM once there
-// are rows enough to keep loads in flight: each thread has kRun rows under
-// way, a block's worth apart.  8,192 tokens of 4 heads of 128 from FP32 to
-// INT8: 18 us for K and V (42 MB), two thirds of the issue slots; back: 15 us.
+// (lanes: pieces a row, a power of two up to 32).  Each thread has kRun rows
+// under way, a block's worth apart.  8,192 tokens of 4 heads of 128 from FP32
+// to INT8: 18 us for K and V (42 MB; HBM alone: 6.4), bound by issue, 38
+// instructions a piece of four values; back: 15 us, the latency of the slot
+// and then of the row.
 constexpr int kRun = 4;
 
 template <typename TV>
@@ -159,10 +162,10 @@ struct RowAt {
 // One row's E elements as INT8 with the row's scale (mb: the largest bit
 // pattern of the row's magnitudes).  x / scale rounded, halves away from
 // zero: added to 1.5 * 2^23 the product x * (1 / scale) rounds to the
-// integer that then lies in the low byte.  The product is within 2^-22 of
-// the FP32 quotient (relative, so 2e-5 here) and rounds alike unless it lies
-// that close to a half; there, and where it is no number, the quotient
-// itself decides.
+// integer that then lies in the low byte.  The product is within 2^-23 of
+// the FP32 quotient (relative: one rounding each; so 1.6e-5 here) and rounds
+// alike unless it lies that close to a half; there (taken as 1e-4), and where
+// it is no number, the quotient itself decides.
 template <int E>
 __device__ __forceinline__ float encode_row(const float (&v)[E], uint32_t mb, uint32_t (&out)[E / 4]) {
     const bool bad = mb >= 0x7f800000u;

@@ -20,8 +20,8 @@
 //
 // INT8 caches: what bounds them is the widening of the bytes on the integer
 // pipe, so they are widened to f16 (paged_attn.cuh).  64 sequences of 100 to
-// 8,191 positions at the 7B shape: 52 us widened to bf16, 48 us so (38 us as
-// the plan now cuts them and with the merge: 3.4 TB/s, 14.5 M instructions).
+// 8,191 positions at the 7B shape: 63 us widened to bf16, 48 us so (38 us as
+// the plan now cuts them and with the merge: 3.4 TB/s, 14.8 M instructions).
 #include "paged_attn.cuh"
 
 namespace qb {

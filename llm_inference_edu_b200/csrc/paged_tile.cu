@@ -20,11 +20,15 @@
 // most) is of the size of the result's own.
 // INT8 caches: pages are copied raw and widened to f16 by a warpgroup; two
 // planes of FP32 values, one of BF16 values (paged_attn.cuh).  Their scales
-// multiply scores and weights in the softmax.
+// multiply scores and weights in the softmax.  509 tokens behind 2,999 and 23
+// single ones, 28/4 heads of 128, FP32: 132 us, 8 of them for looking at each
+// key's own weight and V row where a base rises (once a stream as a rule).
+// Such rare code waits for its instructions: a warp stands two cycles without
+// one for each that it issues, so it is kept short.
 // FP32 values: each tile's product is gathered in FP32 by a warpgroup.
 // K tiles are K-major operands as TMA leaves them (128-byte swizzle, a box a
 // page); V tiles are the MN-major operand in the same layout.
-// 4,096 tokens behind 4,096, 28/4 heads of 128, BF16: 373 us, 967 TFLOP/s.
+// 4,096 tokens behind 4,096, 28/4 heads of 128, BF16: 370 us, 975 TFLOP/s.
 // A stream's softmax takes 1.7 k cycles a tile and its products 1.1 k, with
 // the other stream's in between: neither pipe is full.
 // Every wait is bounded: a role that gives up raises the abort flag, copies
@@ -481,48 +485,48 @@ __global__ void __launch_bounds__(Tile<TV, TC, HD>::kThreads, 1)
                     }
                 }
 #pragma unroll
-              for (int x = 0; x < kRun; ++x) {
-                const int u = u0 + 256 * x, r = u / (HD / 8), ch = u % (HD / 8);
-                if constexpr (!T::kWide && !T::kInt8) {
-                    *(uint4 *)(s_q + ((r >> 7) * PN + ch / 8) * 16384 + (r & 127) * 128 + (((ch & 7) ^ (r & 7)) << 4)) = raw[x][0];
-                } else {
-                float v[8];
+                for (int x = 0; x < kRun; ++x) {
+                    const int u = u0 + 256 * x, r = u / (HD / 8), ch = u % (HD / 8);
+                    if constexpr (!T::kWide && !T::kInt8) {
+                        *(uint4 *)(s_q + ((r >> 7) * PN + ch / 8) * 16384 + (r & 127) * 128 + (((ch & 7) ^ (r & 7)) << 4)) = raw[x][0];
+                    } else {
+                        float v[8];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = load_value((const TV *)raw[x], e);
-                const int rr = r & 127;
-                if constexpr (T::kInt8) {
-                    // The row's HD / 8 pieces are neighbouring lanes.
-                    uint32_t mb = 0;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) mb = max(mb, __float_as_uint(v[e]) & 0x7fffffffu);
-#pragma unroll
-                    for (int off = HD / 16; off; off >>= 1) mb = max(mb, __shfl_xor_sync(0xffffffffu, mb, off));
-                    const float up = row_scale(mb);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) v[e] *= up;
-                    if (ch == 0) ctl->c[r] = __fdiv_rn(a.c, up);
-                }
-#pragma unroll
-                for (int pl = 0; pl < NP; ++pl) {
-                    uint32_t w[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
+                        for (int e = 0; e < 8; ++e) v[e] = load_value((const TV *)raw[x], e);
+                        const int rr = r & 127;
                         if constexpr (T::kInt8) {
-                            w[e] = pack_f16(v[2 * e], v[2 * e + 1]);
-                            const float2 x = unpack_f16(w[e]);
-                            v[2 * e] -= x.x;
-                            v[2 * e + 1] -= x.y;
-                        } else {
-                            w[e] = pack_bf16(v[2 * e], v[2 * e + 1]);
-                            v[2 * e] -= bf16_lo(w[e]);
-                            v[2 * e + 1] -= bf16_hi(w[e]);
+                            // The row's HD / 8 pieces are neighbouring lanes.
+                            uint32_t mb = 0;
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) mb = max(mb, __float_as_uint(v[e]) & 0x7fffffffu);
+#pragma unroll
+                            for (int off = HD / 16; off; off >>= 1) mb = max(mb, __shfl_xor_sync(0xffffffffu, mb, off));
+                            const float up = row_scale(mb);
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) v[e] *= up;
+                            if (ch == 0) ctl->c[r] = __fdiv_rn(a.c, up);
+                        }
+#pragma unroll
+                        for (int pl = 0; pl < NP; ++pl) {
+                            uint32_t w[4];
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                if constexpr (T::kInt8) {
+                                    w[e] = pack_f16(v[2 * e], v[2 * e + 1]);
+                                    const float2 x = unpack_f16(w[e]);
+                                    v[2 * e] -= x.x;
+                                    v[2 * e + 1] -= x.y;
+                                } else {
+                                    w[e] = pack_bf16(v[2 * e], v[2 * e + 1]);
+                                    v[2 * e] -= bf16_lo(w[e]);
+                                    v[2 * e + 1] -= bf16_hi(w[e]);
+                                }
+                            }
+                            uint8_t *dst = s_q + ((r >> 7) * PN + pl * PN + ch / 8) * 16384 + rr * 128 + (((ch & 7) ^ (rr & 7)) << 4);
+                            *(uint4 *)dst = make_uint4(w[0], w[1], w[2], w[3]);
                         }
                     }
-                    uint8_t *dst = s_q + ((r >> 7) * PN + pl * PN + ch / 8) * 16384 + rr * 128 + (((ch & 7) ^ (rr & 7)) << 4);
-                    *(uint4 *)dst = make_uint4(w[0], w[1], w[2], w[3]);
                 }
-                }
-              }
             }
             if (T::kInt8) asm volatile("bar.sync 2, 256;" ::: "memory");
             fence_proxy_async_smem();
@@ -874,7 +878,7 @@ __global__ void __launch_bounds__(Tile<TV, TC, HD>::kThreads, 1)
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(T::kOtherRegs));
         if (warp == 8) {
             // Producers: BF16 boxes straight into the operand stages (K by this
-            // warp and warp 10, V by warp 11), INT8 pages raw into the pieces.
+            // warp, V by warp 11), INT8 pages raw into the pieces.
             if constexpr (!T::kInt8) {
                 produce(true);
             } else {
@@ -1122,7 +1126,9 @@ cudaError_t launch_tile(const Args &a, size_t pool_rows, cudaStream_t st) {
     if (!configured[dev].load()) {
         e = cudaFuncSetAttribute(attend_tile<TV, TC, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
         if (e != cudaSuccess) return e;
-        // The split of the registers counts on what the launch allots.
+        // The split of the registers counts on what the launch allots: with
+        // fewer a warpgroup would wait for its share forever, so a build that
+        // comes out otherwise is refused here.
         cudaFuncAttributes fa;
         e = cudaFuncGetAttributes(&fa, attend_tile<TV, TC, HD>);
         if (e != cudaSuccess) return e;
